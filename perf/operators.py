@@ -185,11 +185,7 @@ def prepare(case, seed):
         st.path = torch.empty(batch, PAGE, dtype=torch.int32, device=dev)
         st.count = torch.empty(batch, dtype=torch.int32, device=dev)
         st.next = torch.empty(batch, dtype=torch.int32, device=dev)
-        st.scratch = torch.zeros(n + 1, dtype=torch.int64, device=dev)
-        if own:
-            st.ops = importlib.import_module("daisi-llogos_b200.kernels.ops")
-        return st
-
+    XX
     nh, nkv, hd = HEADS[case["heads"]]
     lens = _lengths(case)
     st.lens = lens
