@@ -185,7 +185,10 @@ def prepare(case, seed):
         st.path = torch.empty(batch, PAGE, dtype=torch.int32, device=dev)
         st.count = torch.empty(batch, dtype=torch.int32, device=dev)
         st.next = torch.empty(batch, dtype=torch.int32, device=dev)
-    XX
+        if own:
+            st.ops = importlib.import_module("daisi-llogos_b200.kernels.ops")
+            st.scratch = torch.zeros(st.ops.tree_accept_scratch(n, batch), dtype=torch.int64, device=dev)
+        return st
     nh, nkv, hd = HEADS[case["heads"]]
     lens = _lengths(case)
     st.lens = lens
