@@ -1,0 +1,310 @@
+// Attention of trees of drafted tokens over the paged cache on the CUDA cores: float32 arithmetic, storage float32 or bfloat16, any head
+// sizes up to 384 for keys and values.  The true 32-bit path, and the fallback for what attention_tree_mma.cu does not take.
+//
+// Per sequence b, key/value head and query row r = (node i, head g of the group), with s_j = scale q_r . k_j over the visible keys j
+// (cache_args.h says which): out_r = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m}; a row that sees nothing gets zeros.  One pass over the keys
+// with a running maximum m and sum; a key's weight is exactly nothing where the row does not see it, whatever the key or value holds there
+// (positions behind the tree are never read, a node's value that another node does not see is not multiplied by zero).
+//
+// A block takes ROWS query rows of a (sequence, key/value head) and one of n_splits equal runs of its 32-key tiles; all heads of a group and
+// all nodes share a tile's keys and values through shared memory.  Products are 4 rows x 2 keys (scores) and 4 rows x 4 elements (values) a
+// thread, so that a float read from shared memory is used two to four times; the keys' rows are padded by 16 bytes, which spreads the
+// sixteen rows that a half warp reads over all banks.  Runs that share a row block leave partial results (sums, maximum, sum of weights); the
+// block that takes the last ticket joins them in their order, so results do not depend on who comes last.
+#include "common.cuh"
+#include "cache_args.h"
+
+LLG_API const char* llg_last_error() { return g_llg_error; }
+
+namespace {
+
+constexpr int TK = 32;            // keys per tile (half a page)
+constexpr int THREADS = 128;
+constexpr int MAX_HD = 384;
+constexpr int PART_EXTRA = 2;     // a partial row is [vd] sums, the maximum, the sum of weights
+
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p);
+template <>
+__device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <>
+__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
+  const uint2 r = *reinterpret_cast<const uint2*>(p);
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// Copies rows of `width` elements into shared memory as float32, zeros behind `width` up to `padded` and for rows that are not there.
+template <typename T, typename Row>
+__device__ __forceinline__ void stage(float* dst, int rows, int width, int padded, int stride, Row row) {
+  if ((width & 3) == 0) {
+    const int w4 = padded / 4;
+    for (int c = threadIdx.x; c < rows * w4; c += THREADS) {
+      const int r = c / w4, d = (c - r * w4) * 4;
+      const T* src = row(r);
+      *reinterpret_cast<float4*>(dst + r * stride + d) = (src && d < width) ? load4<T>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else {
+    for (int c = threadIdx.x; c < rows * padded; c += THREADS) {
+      const int r = c / padded, d = c - r * padded;
+      const T* src = row(r);
+      dst[r * stride + d] = (src && d < width) ? to_f32(src[d]) : 0.f;
+    }
+  }
+}
+
+// RY: rows per thread; a block's 8 rows of threads take 8 RY query rows.  VD: sums per row and thread, in steps of 64 value elements.
+template <typename T, int RY, int VD>
+__global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
+  constexpr int ROWS = 8 * RY;
+  extern __shared__ __align__(16) float smem[];
+  __shared__ long long bits[ROWS];
+  __shared__ int depth[ROWS], node_depth[LLG_TREE_NODES];
+  __shared__ int is_last;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int kp = (a.hd + 3) / 4 * 4, vp = (a.vd + 3) / 4 * 4;       // padded row sizes
+  const int ks = kp + 4, vs = vp + 4;
+  float* Qs = smem;                       // [ROWS][ks]
+  float* Ks = Qs + ROWS * ks;             // [TK][ks]
+  float* Vs = Ks + TK * ks;               // [TK][vs]
+  float* Ps = Vs + TK * vs;               // [ROWS][TK + 4]
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int G = a.nh / a.nkv;
+  const int b = blockIdx.z, split = blockIdx.x;
+  const int row_blocks = gridDim.y / a.nkv;
+  const int kvh = blockIdx.y / row_blocks, rb = blockIdx.y - kvh * row_blocks;
+  const int tok0 = a.cu_tokens[b];
+  const int n = min(min(a.cu_tokens[b + 1], a.n_tokens) - tok0, a.max_nodes);
+  const int row0 = rb * ROWS, n_rows = min(ROWS, n * G - row0);
+  if (n_rows <= 0) return;                // the same for all blocks of a row block: nobody waits for a ticket of theirs
+  const int lb = a.len_before[b], slot = a.slots[b], total = lb + n;
+  const T* qg = (const T*)a.q;
+  const T* kg = (const T*)a.k_pages;
+  const T* vg = (const T*)a.v_pages;
+
+  for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
+  for (int r = tid; r < ROWS; r += THREADS) {
+    const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
+    bits[r] = mine;
+    depth[r] = __popcll(mine) - 1;
+  }
+  stage<T>(Qs, ROWS, a.hd, kp, ks, [&](int r) -> const T* {
+    return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
+  });
+
+  const int lo = a.window > 0 ? max(0, lb - a.window) : 0;          // no row sees less than this (a row without any bit has depth -1)
+  const int t0 = lo / TK, t_end = (total + TK - 1) / TK;
+  const int per = (t_end - t0 + a.n_splits - 1) / a.n_splits;
+  const int t_from = t0 + split * per, t_to = min(t_end, t_from + per);
+
+  float m[RY], l[RY], o[RY][VD * 4];
+#pragma unroll
+  for (int r = 0; r < RY; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < VD * 4; ++e) o[r][e] = 0.f;
+  }
+  for (int t = t_from; t < t_to; ++t) {
+    const int p0 = t * TK;
+    __syncthreads();
+    stage<T>(Ks, TK, a.hd, kp, ks, [&](int r) -> const T* {
+      return p0 + r < total ? kg + kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0 + r, kvh, a.nkv) * a.hd : nullptr;
+    });
+    stage<T>(Vs, TK, a.vd, vp, vs, [&](int r) -> const T* {
+      return p0 + r < total ? vg + kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0 + r, kvh, a.nkv) * a.vd : nullptr;
+    });
+    __syncthreads();
+    float s[RY][2];
+#pragma unroll
+    for (int r = 0; r < RY; ++r) s[r][0] = s[r][1] = 0.f;
+    for (int d = 0; d < kp; d += 4) {
+      const float4 k0 = *reinterpret_cast<const float4*>(Ks + tx * ks + d);
+      const float4 k1 = *reinterpret_cast<const float4*>(Ks + (tx + 16) * ks + d);
+#pragma unroll
+      for (int r = 0; r < RY; ++r) {
+        const float4 q = *reinterpret_cast<const float4*>(Qs + (ty * RY + r) * ks + d);
+        s[r][0] += q.x * k0.x + q.y * k0.y + q.z * k0.z + q.w * k0.w;
+        s[r][1] += q.x * k1.x + q.y * k1.y + q.z * k1.z + q.w * k1.w;
+      }
+    }
+    // positions that some row may not see: the tree's, those behind it, the window's edge
+    const bool mixed = p0 + TK > lb || (a.window > 0 && p0 <= lb + n - a.window);
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const int row = ty * RY + r;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int p = p0 + tx + 16 * e, j = p - lb;
+        bool sees = true;
+        if (mixed) {
+          if (j < 0) sees = a.window <= 0 || depth[row] - j < a.window;
+          else sees = j < n && ((bits[row] >> j) & 1) && (a.window <= 0 || depth[row] - node_depth[j] < a.window);
+        }
+        s[r][e] = sees ? s[r][e] * a.scale : -INFINITY;
+        mx = fmaxf(mx, s[r][e]);
+      }
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+      const float m_new = fmaxf(m[r], mx);
+      const float corr = m_new == -INFINITY ? 1.f : expf(m[r] - m_new);
+      m[r] = m_new;
+      l[r] *= corr;
+#pragma unroll
+      for (int e = 0; e < VD * 4; ++e) o[r][e] *= corr;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p = s[r][e] == -INFINITY ? 0.f : expf(s[r][e] - m_new);
+        l[r] += p;
+        Ps[row * (TK + 4) + tx + 16 * e] = p;
+      }
+    }
+    __syncwarp();                          // a row's weights come from and go to the lanes of one warp
+    for (int j = 0; j < TK; ++j) {
+      float p[RY];
+#pragma unroll
+      for (int r = 0; r < RY; ++r) p[r] = Ps[(ty * RY + r) * (TK + 4) + j];
+#pragma unroll
+      for (int c = 0; c < VD; ++c) {
+        const int d = c * 64 + tx * 4;
+        if (d < vp) {
+          const float4 v = *reinterpret_cast<const float4*>(Vs + j * vs + d);
+#pragma unroll
+          for (int r = 0; r < RY; ++r) {
+            if (!mixed || p[r] != 0.f) {
+              o[r][c * 4 + 0] += p[r] * v.x;
+              o[r][c * 4 + 1] += p[r] * v.y;
+              o[r][c * 4 + 2] += p[r] * v.z;
+              o[r][c * 4 + 3] += p[r] * v.w;
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RY; ++r) {
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], k);
+  }
+  T* out = (T*)a.out;
+  const int slots_per_row = a.n_splits;
+  const long long first_row = ((long long)b * a.nkv + kvh) * a.max_nodes * G + row0;
+  const int pw = a.vd + PART_EXTRA;
+#pragma unroll
+  for (int r = 0; r < RY; ++r) {
+    const int row = ty * RY + r;
+    if (row >= n_rows) continue;
+    if (a.n_splits == 1) {
+      T* dst = out + ((long long)(tok0 + (row0 + row) / G) * a.nh + kvh * G + (row0 + row) % G) * a.vd;
+      const float inv = l[r] != 0.f ? 1.f / l[r] : 0.f;
+#pragma unroll
+      for (int e = 0; e < VD * 4; ++e) {
+        const int d = (e >> 2) * 64 + tx * 4 + (e & 3);
+        if (d < a.vd) dst[d] = from_f32<T>(o[r][e] * inv);
+      }
+    } else {
+      float* dst = a.part + ((first_row + row) * slots_per_row + split) * pw;
+      if (tx == 0) {
+        dst[a.vd] = m[r];
+        dst[a.vd + 1] = l[r];
+      }
+      if (m[r] == -INFINITY) continue;                              // nothing seen: nobody reads the sums
+#pragma unroll
+      for (int e = 0; e < VD * 4; ++e) {
+        const int d = (e >> 2) * 64 + tx * 4 + (e & 3);
+        if (d < a.vd) dst[d] = o[r][e];
+      }
+    }
+  }
+  if (a.n_splits == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    int* counter = a.counters + (b * a.nkv + kvh) * row_blocks + rb;
+    const int ticket = atomicAdd(counter, 1);
+    is_last = ticket == a.n_splits - 1;
+    if (is_last) *counter = 0;
+  }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  const int warp = tid >> 5, lane = tid & 31;
+  for (int row = warp; row < n_rows; row += THREADS / 32) {
+    const float* src = a.part + (first_row + row) * slots_per_row * pw;
+    float M = -INFINITY;
+    for (int s = 0; s < a.n_splits; ++s) M = fmaxf(M, __ldcg(src + (long long)s * pw + a.vd));
+    float L = 0.f, acc[MAX_HD / 32];
+#pragma unroll
+    for (int k = 0; k < MAX_HD / 32; ++k) acc[k] = 0.f;
+    for (int s = 0; s < a.n_splits; ++s) {
+      const float* p = src + (long long)s * pw;
+      const float ms = __ldcg(p + a.vd);
+      if (ms == -INFINITY) continue;
+      const float w = expf(ms - M);
+      L += w * __ldcg(p + a.vd + 1);
+#pragma unroll
+      for (int k = 0; k < MAX_HD / 32; ++k) {
+        const int d = lane + 32 * k;
+        if (d < a.vd) acc[k] += w * __ldcg(p + d);
+      }
+    }
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    T* dst = out + ((long long)(tok0 + (row0 + row) / G) * a.nh + kvh * G + (row0 + row) % G) * a.vd;
+#pragma unroll
+    for (int k = 0; k < MAX_HD / 32; ++k) {
+      const int d = lane + 32 * k;
+      if (d < a.vd) dst[d] = from_f32<T>(acc[k] * inv);
+    }
+  }
+}
+
+int rows_per_block(int rows) { return rows <= 8 ? 8 : 32; }
+
+template <typename T, int RY, int VD>
+int launch(const TreeArgs& a, cudaStream_t stream) {
+  const int kp = (a.hd + 3) / 4 * 4 + 4, vp = (a.vd + 3) / 4 * 4 + 4;
+  const size_t smem = sizeof(float) * ((size_t)(8 * RY + TK) * kp + (size_t)TK * vp + 8 * RY * (TK + 4));
+  auto kernel = attn_tree_kernel<T, RY, VD>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return llg_fail("attn_tree: shared memory %zu: %s", smem, cudaGetErrorString(e));
+  const int G = a.nh / a.nkv, blocks = (a.max_nodes * G + 8 * RY - 1) / (8 * RY);
+  LLG_REQUIRE((long long)blocks * a.nkv <= 65535 && a.n_seqs <= 65535, "attn_tree: %d row blocks of %d heads, %d sequences: more than a grid takes",
+              blocks, a.nkv, a.n_seqs);
+  e = llg_launch(kernel, dim3(a.n_splits, blocks * a.nkv, a.n_seqs), dim3(THREADS), smem, stream, a);
+  if (e != cudaSuccess) return llg_fail("attn_tree: launch: %s", cudaGetErrorString(e));
+  return llg_check_launch("attn_tree");
+}
+
+template <typename T>
+int dispatch(const TreeArgs& a, cudaStream_t stream) {
+  const bool few = rows_per_block(a.max_nodes * (a.nh / a.nkv)) == 8;
+  if (a.vd <= 64) return few ? launch<T, 1, 1>(a, stream) : launch<T, 4, 1>(a, stream);
+  if (a.vd <= 128) return few ? launch<T, 1, 2>(a, stream) : launch<T, 4, 2>(a, stream);
+  return few ? launch<T, 1, 6>(a, stream) : launch<T, 4, 6>(a, stream);
+}
+
+}  // namespace
+
+LLG_API int llg_tree_max_nodes() { return LLG_TREE_NODES; }
+
+// Query rows that a block takes where a tree has up to `rows` of them per key/value head: there are n_seqs * nkv * ceil(rows / this) counters.
+LLG_API int llg_attn_tree_rows(int rows) { return rows_per_block(rows); }
+
+// part: [n_seqs * nkv * max_nodes * group][n_splits][vd + 2] floats where n_splits > 1.
+LLG_API int llg_attn_tree_simt(const TreeArgs* args, int dtype, cudaStream_t stream) {
+  const TreeArgs& a = *args;
+  LLG_REQUIRE(a.nh > 0 && a.nkv > 0 && a.nh % a.nkv == 0, "attn_tree: %d heads are no multiple of %d key/value heads", a.nh, a.nkv);
+  LLG_REQUIRE(a.hd > 0 && a.hd <= MAX_HD && a.vd > 0 && a.vd <= MAX_HD, "attn_tree: heads of %d and %d elements (1 to %d)", a.hd, a.vd, MAX_HD);
+  LLG_REQUIRE(a.max_nodes > 0 && a.max_nodes <= LLG_TREE_NODES, "attn_tree: trees of up to %d nodes (1 to %d)", a.max_nodes, LLG_TREE_NODES);
+  LLG_REQUIRE(a.n_splits >= 1 && (a.n_splits == 1 || (a.part && a.counters)), "attn_tree: %d splits need scratch and counters", a.n_splits);
+  LLG_REQUIRE(a.window >= 0 && a.ring_pages > 0 && a.table_width >= a.ring_pages, "attn_tree: bad cache geometry");
+  LLG_REQUIRE(a.scale > 0.f, "attn_tree: the softmax scale must be positive");
+  if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
+  if (dtype == LLG_F32) return dispatch<float>(a, stream);
+  if (dtype == LLG_BF16) return dispatch<__nv_bfloat16>(a, stream);
+  return llg_fail("attn_tree: unknown dtype %d", dtype);
+}

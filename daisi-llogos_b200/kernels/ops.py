@@ -15,6 +15,7 @@ from ..csrc.build import load_library
 
 F32, BF16 = 0, 1
 PAGE = 64  # tokens per cache page; checked against the library at first use
+TREE_MAX_NODES = 64      # nodes of a drafted tree; checked against the library at first use
 
 
 class KernelError(RuntimeError):
@@ -366,6 +367,37 @@ class _MatrixMemoryArgs(Structure):
     ]
 
 
+class _TreeArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p), ("page_table", c_void_p),
+        ("table_width", c_int), ("ring_pages", c_int), ("slots", c_void_p), ("cu_tokens", c_void_p), ("len_before", c_void_p),
+        ("ancestors", c_void_p), ("out", c_void_p), ("part", c_void_p), ("counters", c_void_p),
+        ("n_seqs", c_int), ("n_tokens", c_int), ("max_nodes", c_int), ("n_pages", c_int),
+        ("nh", c_int), ("nkv", c_int), ("hd", c_int), ("vd", c_int), ("n_splits", c_int), ("max_len", c_int),
+        ("scale", c_float), ("window", c_int),
+    ]
+
+
+class _KeyWeightArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k_pages", c_void_p), ("page_table", c_void_p), ("table_width", c_int),
+        ("slots", c_void_p), ("cu_tokens", c_void_p), ("len_before", c_void_p), ("weights", c_void_p), ("weight_width", c_int),
+        ("stats", c_void_p), ("row_end", c_void_p), ("scores", c_void_p), ("counters", c_void_p),
+        ("n_seqs", c_int), ("n_tokens", c_int), ("nh", c_int), ("nkv", c_int), ("hd", c_int), ("last", c_int), ("chunks", c_int),
+        ("scale", c_float),
+    ]
+
+
+class _MoveArgs(Structure):
+    _fields_ = [
+        ("pools", c_void_p), ("n_layers", c_int), ("pools_per_layer", c_int), ("row_bytes", c_int * 2),
+        ("page_table", c_void_p), ("table_width", c_int), ("ring_pages", c_int), ("slots", c_void_p), ("base", c_void_p),
+        ("source", c_void_p), ("source_layer", c_longlong), ("source_seq", c_longlong), ("source_head", c_longlong),
+        ("count", c_void_p), ("weights", c_void_p), ("weight_layer", c_longlong), ("weight_width", c_int),
+        ("n_seqs", c_int), ("nkv", c_int), ("most", c_int),
+    ]
+
+
 class _SampleArgs(Structure):
     _fields_ = [
         ("logits", c_void_p), ("work", c_void_p), ("out", c_void_p), ("probs_out", c_void_p),
@@ -526,6 +558,20 @@ def _load_lib(name: str):
         lib.llg_grouped_linear.argtypes = [POINTER(_GroupedLinearArgs), c_int, c_int, c_void_p]
         lib.llg_moe_combine.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int,
                                         c_int, c_int, c_void_p, c_int, c_void_p]
+    elif name == "attention_tree":
+        lib.llg_attn_tree_simt.argtypes = [POINTER(_TreeArgs), c_int, c_void_p]
+        lib.llg_attn_tree_rows.argtypes = [c_int]
+        if lib.llg_tree_max_nodes() != TREE_MAX_NODES:
+            raise KernelError(f"the kernels take trees of {lib.llg_tree_max_nodes()} nodes, Python expects {TREE_MAX_NODES}")
+    elif name == "key_weights":
+        lib.llg_key_weights_simt.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
+    elif name == "cache_rows":
+        lib.llg_tree_accept.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p]
+        lib.llg_tree_walk.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
+        lib.llg_keep_keys.argtypes = [c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p,
+                                      c_int, c_int, c_void_p]
+        lib.llg_move_rows.argtypes = [POINTER(_MoveArgs), c_void_p]
     elif name == "init":
         lib.llg_fill_normal.argtypes = [c_void_p, c_int, c_longlong, c_ulonglong, ctypes.c_double, ctypes.c_double, c_void_p]
         lib.llg_fill.argtypes = [c_void_p, c_int, c_longlong, c_float, c_void_p]
@@ -2316,3 +2362,336 @@ def sample(logits: torch.Tensor, work: torch.Tensor, out: torch.Tensor, *, tempe
 
 
 _sample_scratch = {}
+
+
+# ---- drafted trees and shortened caches -----------------------------------------------
+
+def _on_one_device(what: str, *tensors) -> None:
+    """The tensors of a call lie on the current device, whose current stream the launch goes to."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise KernelError(f"{what}: tensors on {dev} and on {t.device}")
+    if dev.type == "cuda" and dev.index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        raise KernelError(f"{what}: tensors on {dev} while cuda:{torch.cuda.current_device()} is the current device")
+
+
+def _wide(what: str, *tensors) -> None:
+    """Storage that the kernels read 16 bytes at a time."""
+    for t in tensors:
+        if t.data_ptr() % 16:
+            raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} does not start on 16 bytes")
+
+
+def _shape(what: str, name: str, t: torch.Tensor, shape, dtype: Optional[torch.dtype] = None) -> None:
+    if tuple(t.shape) != tuple(shape):
+        raise KernelError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise KernelError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+
+
+def _step_layout(what: str, slots, cu_tokens, len_before, page_table) -> int:
+    """Sequences of a step; the layout's tensors are int32 of one length."""
+    b = slots.numel()
+    _shape(what, "slots", slots, (b,), torch.int32)
+    _shape(what, "len_before", len_before, (b,), torch.int32)
+    if cu_tokens is not None:
+        _shape(what, "cu_tokens", cu_tokens, (b + 1,), torch.int32)
+    if page_table.dim() != 2 or page_table.dtype != torch.int32:
+        raise KernelError(f"{what}: the page table is int32 [slots, pages]")
+    return b
+
+
+class TreePlan:
+    """How ``attn_tree`` will run for one batch shape.  Made by ``attn_tree_plan``; callers read ``scratch_floats`` and ``n_counters``."""
+
+    def __init__(self, kind: str, key, n_splits: int, max_nodes: int, max_len: int, scratch_floats: int, n_counters: int):
+        self.kind, self.key, self.n_splits, self.max_nodes, self.max_len = kind, key, n_splits, max_nodes, max_len
+        self.scratch_floats, self.n_counters = scratch_floats, n_counters
+
+
+def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int,
+                   value_dim: int = 0) -> TreePlan:
+    """The plan for ``n_seqs`` trees of at most ``max_nodes`` nodes (up to 64), behind which a sequence has at most ``max_len`` positions, the tree's
+    included."""
+    vd = value_dim or head_dim
+    _dtype_code(dtype)
+    if not 0 < max_nodes <= TREE_MAX_NODES:
+        raise KernelError(f"attn_tree: trees of up to {max_nodes} nodes (1 to {TREE_MAX_NODES})")
+    if n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads:
+        raise KernelError(f"attn_tree: {n_heads} heads are no multiple of {n_kv_heads} key/value heads")
+    if not (0 < head_dim <= ATTN_MAX_HEAD_DIM and 0 < vd <= ATTN_MAX_HEAD_DIM):
+        raise KernelError(f"attn_tree: heads of {head_dim} and {vd} elements (1 to {ATTN_MAX_HEAD_DIM})")
+    if n_seqs <= 0 or max_len <= 0:
+        raise KernelError("attn_tree: needs sequences and a bound on their lengths")
+    key = (dtype, n_seqs, n_heads, n_kv_heads, head_dim, vd)
+    lib = _lib("attention_tree")
+    rows = max_nodes * (n_heads // n_kv_heads)
+    per = lib.llg_attn_tree_rows(rows)
+    blocks = n_seqs * n_kv_heads * -(-rows // per)
+    tiles = -(-max_len // 32)
+    splits = max(1, min(-(-4 * sm_count() // blocks), -(-tiles // 4), 64))       # four blocks a multiprocessor, four tiles a block at least
+    return TreePlan("simt", key, splits, max_nodes, max_len, n_seqs * n_kv_heads * rows * splits * (vd + 2) if splits > 1 else 0, blocks)
+
+
+def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, ring_pages: int, slots: torch.Tensor,
+              cu_tokens: torch.Tensor, len_before: torch.Tensor, ancestors: torch.Tensor, out: torch.Tensor, scratch: torch.Tensor, *,
+              scale: float, window: int = 0, plan: TreePlan, counters: torch.Tensor) -> None:
+    """Attention of trees of drafted tokens over the paged cache.
+
+    Sequence b holds ``len_before[b]`` keys; its tree's nodes are the packed tokens ``cu_tokens[b] .. cu_tokens[b + 1]`` (at most
+    ``plan.max_nodes``), whose keys and values lie in the pages already, node i's at position ``len_before[b] + i``.  ``ancestors`` (int64
+    ``[N]``): bit j of a node's word says that it sees node j of its tree (its own bit included); a node sees every cached key
+    besides.  ``window`` W > 0: a node stands ``depth`` = (its bits) - 1 positions behind the cached keys and sees what stands less than W before
+    it.  ``q`` is ``[N, nh, hd]``, ``out`` ``[N, nh * vd]``; a node that sees nothing gets zeros, rows behind the last sequence are left as they
+    were.  What a node does not see has no part in its result, whatever is stored there.
+
+    ``plan`` (``attn_tree_plan`` for this batch shape) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left
+    zero) must hold; calls that may run at the same time need their own."""
+    what = "attn_tree"
+    n, nh, hd = q.shape
+    nkv, vd = k_pages.shape[1], v_pages.shape[3]
+    b = _step_layout(what, slots, cu_tokens, len_before, page_table)
+    if plan.key != (q.dtype, b, nh, nkv, hd, vd):
+        raise KernelError(f"attn_tree: the plan is for {plan.key}, the call for {(q.dtype, b, nh, nkv, hd, vd)}")
+    _shape(what, "k_pages", k_pages, (k_pages.shape[0], nkv, PAGE, hd), q.dtype)
+    _shape(what, "v_pages", v_pages, (k_pages.shape[0], nkv, PAGE, vd), q.dtype)
+    _shape(what, "ancestors", ancestors, (n,), torch.int64)
+    _shape(what, "out", out, (n, nh * vd), q.dtype)
+    if not scale > 0:
+        raise KernelError("attn_tree: the softmax scale must be positive")
+    if window < 0 or not 0 < ring_pages <= page_table.shape[1]:
+        raise KernelError(f"attn_tree: window {window}, {ring_pages} ring pages in a table of {page_table.shape[1]}")
+    if window > 0 and ring_pages * PAGE < min(window + PAGE, plan.max_len):
+        raise KernelError(f"attn_tree: a ring of {ring_pages} pages does not hold a window of {window} keys and a tree")
+    if window == 0 and ring_pages * PAGE < plan.max_len:
+        raise KernelError(f"attn_tree: {ring_pages} pages do not hold {plan.max_len} positions")
+    if scratch.dtype != torch.float32 or scratch.numel() < plan.scratch_floats:
+        raise KernelError(f"attn_tree: scratch of {scratch.numel()} {scratch.dtype}, {plan.scratch_floats} float32 needed")
+    if counters.dtype != torch.int32 or counters.numel() < plan.n_counters:
+        raise KernelError(f"attn_tree: {counters.numel()} counters of {counters.dtype}, {plan.n_counters} zeroed int32 needed")
+    _on_one_device(what, q, k_pages, v_pages, page_table, slots, cu_tokens, len_before, ancestors, out, scratch, counters)
+    a = _TreeArgs()
+    a.q, a.k_pages, a.v_pages = _ptr(q), _ptr(k_pages), _ptr(v_pages)
+    _wide(what, q, k_pages, v_pages, scratch)
+    a.page_table, a.table_width, a.ring_pages = _ptr(page_table), page_table.shape[1], ring_pages
+    a.slots, a.cu_tokens, a.len_before, a.ancestors = _ptr(slots), _ptr(cu_tokens), _ptr(len_before), _ptr(ancestors)
+    a.out, a.part, a.counters = _ptr(out), _ptr(scratch), _ptr(counters)
+    a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages = b, n, plan.max_nodes, k_pages.shape[0]
+    a.nh, a.nkv, a.hd, a.vd, a.n_splits, a.max_len = nh, nkv, hd, vd, plan.n_splits, plan.max_len
+    a.scale, a.window = float(scale), int(window)
+    lib = _lib("attention_tree")
+    _check(lib, lib.llg_attn_tree_simt(byref(a), _dt(q), _stream()))
+
+
+def tree_accept_scratch(n_tokens: int, n_seqs: int) -> int:
+    """int64 numbers of scratch that ``tree_accept`` wants for the logits of ``n_tokens`` nodes of ``n_seqs`` trees."""
+    return n_tokens + n_seqs
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor, path: torch.Tensor, n_path: torch.Tensor,
+                next_token: torch.Tensor, *, logits: Optional[torch.Tensor] = None, picked: Optional[torch.Tensor] = None,
+                scratch: Optional[torch.Tensor] = None) -> None:
+    """Which path of every drafted tree is confirmed.
+
+    Tree b's nodes are ``cu_tokens[b] .. cu_tokens[b + 1]`` (at most 64) with their ``tokens`` and ``parents`` (int32 ``[N]``; a parent is a place
+    within the tree and lies before its node; node 0 is the token that is certain already, parent -1).  What follows a node is
+    ``picked[node]`` (int32, a sampler's draws), or the largest of ``logits[node]`` (float32 ``[N, vocab]``; of equal ones the lowest id, NaN
+    never).  The path starts at node 0 and goes on to the first child whose token is what follows.  ``path`` (int32 ``[B, 64]``) gets its
+    nodes, filled up with -1, ``n_path`` their number, and ``next_token`` what follows the last (of a tree without nodes: 0 and -1).
+
+    ``scratch`` (with ``logits``): int64, ``tree_accept_scratch`` numbers, zero when first used, left zero; one call at a time."""
+    what = "tree_accept"
+    n, b = tokens.numel(), n_path.numel()
+    if (logits is None) == (picked is None):
+        raise KernelError("tree_accept: either logits or picked tokens")
+    _shape(what, "tokens", tokens, (n,), torch.int32)
+    _shape(what, "parents", parents, (n,), torch.int32)
+    _shape(what, "cu_tokens", cu_tokens, (b + 1,), torch.int32)
+    _shape(what, "path", path, (b, TREE_MAX_NODES), torch.int32)
+    _shape(what, "n_path", n_path, (b,), torch.int32)
+    _shape(what, "next_token", next_token, (b,), torch.int32)
+    if n == 0 or b == 0:
+        raise KernelError("tree_accept: no trees, or none with a node")
+    if picked is not None:
+        _shape(what, "picked", picked, (n,), torch.int32)
+        _on_one_device(what, tokens, parents, cu_tokens, path, n_path, next_token, picked)
+        ptrs = [_ptr(t) for t in (picked, tokens, parents, cu_tokens)]
+        lib = _lib("cache_rows")
+        _check(lib, lib.llg_tree_walk(*ptrs, b, _ptr(path), _ptr(n_path), _ptr(next_token), _stream()))
+        return
+    if logits.dim() != 2:
+        raise KernelError(f"tree_accept: logits of shape {tuple(logits.shape)}, expected [nodes, vocabulary]")
+    _shape(what, "logits", logits, (n, logits.shape[1]), torch.float32)
+    if scratch is None or scratch.dtype != torch.int64 or scratch.numel() < n + b:
+        raise KernelError(f"tree_accept: needs {n + b} zeroed int64 of scratch")
+    _on_one_device(what, tokens, parents, cu_tokens, path, n_path, next_token, logits, scratch)
+    ptrs = [_ptr(t) for t in (tokens, parents, cu_tokens)]
+    lib = _lib("cache_rows")
+    _check(lib, lib.llg_tree_accept(_ptr(logits), logits.shape[1], *ptrs, b, n, _ptr(scratch), _ptr(path), _ptr(n_path), _ptr(next_token), _stream()))
+
+
+class KeyWeightPlan:
+    """How ``key_weights`` will run for one batch shape.  Made by ``key_weights_plan``; callers read ``scratch_floats`` and ``n_counters``."""
+
+    def __init__(self, kind: str, key, last: int, max_len: int, chunks: int, stats: int, ends: int, scores: int, n_counters: int):
+        self.kind, self.key, self.last, self.max_len, self.chunks = kind, key, last, max_len, chunks
+        self.stats, self.ends, self.scores, self.n_counters = stats, ends, scores, n_counters
+        self.scratch_floats = stats + ends + scores
+
+
+def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> KeyWeightPlan:
+    """The plan for ``n_seqs`` sequences whose last ``last`` queries are looked at and which have at most ``max_len`` keys, the step's included."""
+    _dtype_code(dtype)
+    if n_kv_heads <= 0 or n_heads <= 0 or n_heads % n_kv_heads:
+        raise KernelError(f"key_weights: {n_heads} heads are no multiple of {n_kv_heads} key/value heads")
+    if not 0 < head_dim <= ATTN_MAX_HEAD_DIM:
+        raise KernelError(f"key_weights: heads of {head_dim} elements (1 to {ATTN_MAX_HEAD_DIM})")
+    if n_seqs <= 0 or last <= 0 or max_len <= 0:
+        raise KernelError("key_weights: needs sequences, queries and a bound on the lengths")
+    lib = _lib("key_weights")
+    keys = lib.llg_key_weights_keys()
+    chunks, rows = -(-max_len // keys), n_heads // n_kv_heads * last
+    total = n_seqs * n_kv_heads * rows
+    scores = total * chunks * keys if rows <= lib.llg_key_weights_store_rows() else 0
+    return KeyWeightPlan("simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, chunks, -(-2 * total * chunks // 4) * 4,
+                         -(-2 * total // 4) * 4, scores, n_seqs * n_kv_heads)
+
+
+def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, cu_tokens: torch.Tensor,
+                len_before: torch.Tensor, weights: torch.Tensor, scratch: torch.Tensor, *, scale: float, last: int, plan: KeyWeightPlan,
+                counters: torch.Tensor) -> None:
+    """Adds up what the step's newest queries give each key: the softmax weights of the last ``last`` queries of every sequence (all of them
+    where it brings fewer), over the heads of a group.  ``weights`` (float32 ``[slots, nkv, width]``): entry j of a sequence's slot becomes ``(j <
+    len_before ? the entry : 0) + the sum`` for all its keys, the step's included; entries behind them and other slots' rows are left as
+    they were.  The keys lie in the pages already (a cache that keeps every key).
+
+    ``plan`` (``key_weights_plan``) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left zero) must hold; calls
+    that may run at the same time need their own.  A slot may be in a step once."""
+    what = "key_weights"
+    n, nh, hd = q.shape
+    nkv = k_pages.shape[1]
+    b = _step_layout(what, slots, cu_tokens, len_before, page_table)
+    if plan.key != (q.dtype, b, nh, nkv, hd) or plan.last != last:
+        raise KernelError(f"key_weights: the plan is for {plan.key} and {plan.last} queries, the call for {(q.dtype, b, nh, nkv, hd)} and {last}")
+    _shape(what, "k_pages", k_pages, (k_pages.shape[0], nkv, PAGE, hd), q.dtype)
+    if weights.dim() != 3:
+        raise KernelError(f"key_weights: weights of shape {tuple(weights.shape)}, expected [slots, heads, positions]")
+    _shape(what, "weights", weights, (page_table.shape[0], nkv, weights.shape[2]), torch.float32)
+    if plan.max_len > weights.shape[2] or plan.max_len > page_table.shape[1] * PAGE:
+        raise KernelError(f"key_weights: {plan.max_len} keys, {weights.shape[2]} weights a row and {page_table.shape[1]} pages")
+    if not scale > 0:
+        raise KernelError("key_weights: the softmax scale must be positive")
+    if scratch.dtype != torch.float32 or scratch.numel() < plan.scratch_floats:
+        raise KernelError(f"key_weights: scratch of {scratch.numel()} {scratch.dtype}, {plan.scratch_floats} float32 needed")
+    if counters.dtype != torch.int32 or counters.numel() < plan.n_counters:
+        raise KernelError(f"key_weights: {counters.numel()} counters of {counters.dtype}, {plan.n_counters} zeroed int32 needed")
+    _on_one_device(what, q, k_pages, page_table, slots, cu_tokens, len_before, weights, scratch, counters)
+    a = _KeyWeightArgs()
+    a.q, a.k_pages = _ptr(q), _ptr(k_pages)
+    _wide(what, q, k_pages, scratch)
+    a.page_table, a.table_width = _ptr(page_table), page_table.shape[1]
+    a.slots, a.cu_tokens, a.len_before = _ptr(slots), _ptr(cu_tokens), _ptr(len_before)
+    a.weights, a.weight_width = _ptr(weights), weights.shape[2]
+    base = _ptr(scratch)
+    a.stats, a.row_end = base, base + 4 * plan.stats
+    a.scores = base + 4 * (plan.stats + plan.ends) if plan.scores else None
+    a.counters = _ptr(counters)
+    a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last, a.chunks = b, n, nh, nkv, hd, last, plan.chunks
+    a.scale = float(scale)
+    lib = _lib("key_weights")
+    _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), _stream()), kernels=2)
+
+
+def keep_keys(weights: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, chosen: torch.Tensor, *, first: int,
+              recent: int, max_len: Optional[int] = None) -> None:
+    """Which keys stay when sequences are cut to ``keep[b]`` of their ``lengths[b]`` keys (int32 ``[B]``), in every layer and key/value head by
+    itself: the ``first`` positions, the newest ``recent``, and of the others those of largest ``weights`` (float32 ``[layers, slots, nkv,
+    width]``; of equal ones the lower position, NaN last).  Where the first and the newest are more than ``keep`` already, the lowest of them.
+    ``chosen`` (int32 ``[layers, B, nkv, most]``, most >= every ``keep``) gets the positions in ascending order; places behind ``keep[b]`` are
+    left as they were.  ``max_len``: a bound on the lengths (default: the weights' width), which fewer registers serve."""
+    what = "keep_keys"
+    if weights.dim() != 4 or chosen.dim() != 4:
+        raise KernelError("keep_keys: weights are [layers, slots, heads, positions], the chosen [layers, sequences, heads, most]")
+    layers, n_slots, nkv, width = weights.shape
+    b, most = slots.numel(), chosen.shape[3]
+    _shape(what, "weights", weights, weights.shape, torch.float32)
+    for name, t in (("slots", slots), ("lengths", lengths), ("keep", keep)):
+        _shape(what, name, t, (b,), torch.int32)
+    _shape(what, "chosen", chosen, (layers, b, nkv, most), torch.int32)
+    bound = width if max_len is None else int(max_len)
+    if not 0 < bound <= width:
+        raise KernelError(f"keep_keys: lengths up to {bound} in rows of {width} weights")
+    if first < 0 or recent < 0:
+        raise KernelError(f"keep_keys: first {first} and recent {recent} must not be negative")
+    _on_one_device(what, weights, slots, lengths, keep, chosen)
+    w, s = _ptr(weights), _ptr(slots)
+    lib = _lib("cache_rows")
+    _check(lib, lib.llg_keep_keys(w, n_slots * nkv * width, width, nkv, layers, b, s, _ptr(lengths), _ptr(keep), int(first), int(recent),
+                                  _ptr(chosen), most, bound, _stream()))
+
+
+class CacheRows:
+    """The key and value pages of several layers that share a page table, whose rows are moved together (``move``): one launch for all of them.
+    ``k_pages`` and ``v_pages``: a tensor ``[pages, nkv, 64, head size]`` per layer (``v_pages`` None: the values are the keys); ``weights``
+    (float32 ``[layers, slots, nkv, width]``, or None): the keys' weights, moved along."""
+
+    def __init__(self, k_pages, v_pages=None, weights: Optional[torch.Tensor] = None):
+        self.k, self.v = list(k_pages), None if v_pages is None else list(v_pages)      # kept alive: the addresses below are theirs
+        what = "CacheRows"
+        if not self.k or (self.v is not None and len(self.v) != len(self.k)):
+            raise KernelError(f"CacheRows: key pages of {len(self.k)} layers, value pages of {len(self.v or [])}")
+        first = self.k[0]
+        if first.dim() != 4 or first.shape[2] != PAGE:
+            raise KernelError(f"CacheRows: pages of shape {tuple(first.shape)}, expected [pages, heads, {PAGE}, head size]")
+        _dt(first)
+        self.n_pages, self.nkv = first.shape[:2]
+        for t in self.k:
+            _shape(what, "a layer's key pages", t, first.shape, first.dtype)
+        for t in self.v or ():
+            _shape(what, "a layer's value pages", t, (self.n_pages, self.nkv, PAGE, self.v[0].shape[3]), first.dtype)
+        self.weights = weights
+        if weights is not None:
+            if weights.dim() != 4 or weights.shape[0] != len(self.k) or weights.shape[2] != self.nkv or weights.dtype != torch.float32:
+                raise KernelError(f"CacheRows: weights of shape {tuple(weights.shape)}, expected float32 [{len(self.k)}, slots, {self.nkv}, positions]")
+        _on_one_device(what, *self.k, *(self.v or ()), weights)
+        pools = [p for i in range(len(self.k)) for p in ([_ptr(self.k[i])] + ([_ptr(self.v[i])] if self.v is not None else []))]
+        _wide(what, *self.k, *(self.v or ()))
+        self.pools = torch.tensor(pools, dtype=torch.int64, device=first.device)
+        a = self.args = _MoveArgs()
+        a.pools, a.n_layers, a.pools_per_layer = self.pools.data_ptr(), len(self.k), 1 if self.v is None else 2
+        a.row_bytes[0] = first.shape[3] * first.element_size()
+        a.row_bytes[1] = 0 if self.v is None else self.v[0].shape[3] * first.element_size()
+        a.nkv = self.nkv
+        if weights is not None:
+            a.weights, a.weight_layer, a.weight_width = _ptr(weights), weights[0].numel(), weights.shape[3]
+
+    def move(self, page_table: torch.Tensor, ring_pages: int, slots: torch.Tensor, base: torch.Tensor, source: torch.Tensor,
+             count: torch.Tensor) -> None:
+        """In every layer, sequence b (slot ``slots[b]``) and key/value head h, the row of position ``base[b] + source[l, b, h, j]`` becomes the row
+        of position ``base[b] + j``, for ``j < count[b]`` (int32 ``[B]``, at most the width of ``source``).  ``source`` is int32 ``[layers or 1,
+        B, heads or 1, width]``: one list for all layers or heads where that is 1.  A list ascends (each place once), so that nothing is
+        needed after it was overwritten; a slot may be in a call once.  Other rows are left as they were."""
+        what = "CacheRows.move"
+        b = _step_layout(what, slots, None, base, page_table)
+        _shape(what, "count", count, (b,), torch.int32)
+        if source.dim() != 4 or source.dtype != torch.int32 or source.shape[0] not in (1, len(self.k)) or source.shape[1] != b \
+                or source.shape[2] not in (1, self.nkv):
+            raise KernelError(f"CacheRows.move: sources of shape {tuple(source.shape)} and {source.dtype}, expected int32 [1 or {len(self.k)}, {b}, "
+                              f"1 or {self.nkv}, places]")
+        if not 0 < ring_pages <= page_table.shape[1]:
+            raise KernelError(f"CacheRows.move: {ring_pages} ring pages in a table of {page_table.shape[1]}")
+        if self.weights is not None and self.weights.shape[1] != page_table.shape[0]:
+            raise KernelError(f"CacheRows.move: weights of {self.weights.shape[1]} slots, a page table of {page_table.shape[0]}")
+        _on_one_device(what, self.k[0], page_table, slots, base, source, count)
+        a = _MoveArgs()
+        ctypes.pointer(a)[0] = self.args
+        a.page_table, a.table_width, a.ring_pages = _ptr(page_table), page_table.shape[1], ring_pages
+        a.slots, a.base, a.source, a.count = _ptr(slots), _ptr(base), _ptr(source), _ptr(count)
+        width = source.shape[3]
+        a.source_seq = source.shape[2] * width
+        a.source_layer = b * a.source_seq if source.shape[0] > 1 else 0
+        a.source_head = width if source.shape[2] > 1 else 0
+        a.n_seqs, a.most = b, width
+        lib = _lib("cache_rows")
+        _check(lib, lib.llg_move_rows(byref(a), _stream()))
