@@ -48,6 +48,7 @@ SOURCES: Dict[str, List[str]] = {
     "addnorm": ["addnorm.cu", "common.cuh", "kernel_args.h"],
     "moe": ["moe.cu", "common.cuh", "kernel_args.h"],
     "attention_tree": ["attention_tree.cu", "common.cuh", "cache_args.h"],
+    "attention_tree_mma": ["attention_tree_mma.cu", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "key_weights": ["key_weights.cu", "key_weights.cuh", "common.cuh", "cache_args.h"],
     "cache_rows": ["cache_rows.cu", "common.cuh", "cache_args.h"],
 }

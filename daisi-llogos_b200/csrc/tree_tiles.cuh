@@ -1,0 +1,206 @@
+// What the tensor-core kernels for drafted trees share (attention_tree_mma.cu, attention_tree_tc.cu): barriers with limits, TMA boxes of cache pages,
+// the softmax's arithmetic, and the list of work that blocks cut into runs.
+#pragma once
+#include "common.cuh"
+#include "cache_args.h"
+
+#include <cuda.h>
+
+#include <mutex>
+
+namespace {
+
+typedef __nv_bfloat16 bf16;
+constexpr int TK = 64;                       // keys per tile = one cache page
+constexpr int MAX_SEQS = 1024;               // sequences whose work fits the plan in shared memory
+constexpr int PART_PAD = 4;                  // a partial row is its sums, the maximum, the sum of weights, and 2 unused: rows stay 16-byte aligned
+constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// false when the limit ran out or another role of the block gave up
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = now_ns();
+  int spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 1023) == 0) {
+      if (*abort_flag) return false;
+      if (now_ns() - t0 > WAIT_LIMIT_NS) return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// x: first element of the box along the head dimension (0 or 64: a multiple of 8 elements, 16 bytes), y: first row
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+// 2^x by the special-function unit alone; arguments are <= 0 or -inf, or bounded by the caller
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^d for a whole number d <= 0 (or -inf), exactly
+__device__ __forceinline__ float pow2_whole(float d) {
+  return d < -126.f ? 0.f : __int_as_float((127 + (int)d) << 23);
+}
+// whether one of two packed bfloat16 numbers is infinite or NaN
+__device__ __forceinline__ bool not_finite(uint32_t x) {
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// A sequence's tree: its nodes, cached keys, and the key tiles that its rows look at.
+struct TreeShape {
+  int tok0, n, lb, t_first, tiles;
+};
+__device__ __forceinline__ TreeShape tree_shape(const TreeArgs& a, int b) {
+  TreeShape s;
+  s.tok0 = a.cu_tokens[b];
+  s.n = max(0, min(min(a.cu_tokens[b + 1], a.n_tokens) - s.tok0, a.max_nodes));
+  s.lb = a.len_before[b];
+  // no row sees less than this under a window (a row without any bit stands one place before the root)
+  s.t_first = a.window > 0 ? max(0, s.lb - a.window) / TK : 0;
+  s.tiles = s.n > 0 ? (s.lb + s.n + TK - 1) / TK - s.t_first : 0;
+  return s;
+}
+
+// The work of a launch is one list: sequence by sequence, key/value head by key/value head, row block by row block, key tile by key tile.
+// Blocks cut it into equal runs; sums[b] and blocks[b] are the units and the row blocks of one head in the sequences before b.
+struct Unit {
+  int b, kvh, rb, t;
+};
+__device__ __forceinline__ Unit locate(const int* sums, const int* blocks, int n_seqs, int nkv, long long u) {
+  int lo = 0, hi = n_seqs - 1;                     // last b with nkv * sums[b] <= u
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long long)nkv * sums[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  Unit c;
+  c.b = lo;
+  const int rbs = blocks[lo + 1] - blocks[lo], tiles = (sums[lo + 1] - sums[lo]) / rbs;
+  const int r = (int)(u - (long long)nkv * sums[lo]), pair = r / tiles;
+  c.t = r - pair * tiles;
+  c.kvh = pair / rbs;
+  c.rb = pair - c.kvh * rbs;
+  return c;
+}
+
+// All threads of a block: sums[] and blocks[] for row blocks of `rows` query rows.  `warp_total`: two numbers per warp.
+template <int THREADS>
+__device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, int* sums, int* blocks, int2* warp_total) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.nh / a.nkv;
+  const int per = (a.n_seqs + THREADS - 1) / THREADS;
+  const int b0 = tid * per, b1 = min(a.n_seqs, b0 + per);
+  int units = 0, rbs = 0;
+  for (int b = b0; b < b1; ++b) {
+    const TreeShape s = tree_shape(a, b);
+    const int r = (s.n * G + rows - 1) / rows;
+    units += r * s.tiles;
+    rbs += r;
+  }
+  int iu = units, ir = rbs;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int pu = __shfl_up_sync(0xffffffffu, iu, o), pr = __shfl_up_sync(0xffffffffu, ir, o);
+    if (lane >= o) {
+      iu += pu;
+      ir += pr;
+    }
+  }
+  if (lane == 31) warp_total[warp] = make_int2(iu, ir);
+  __syncthreads();
+  int su = iu - units, sr = ir - rbs;
+  for (int w = 0; w < warp; ++w) {
+    su += warp_total[w].x;
+    sr += warp_total[w].y;
+  }
+  if (tid == 0) sums[0] = blocks[0] = 0;
+  for (int b = b0; b < b1; ++b) {
+    const TreeShape s = tree_shape(a, b);
+    const int r = (s.n * G + rows - 1) / rows;
+    su += r * s.tiles;
+    sr += r;
+    sums[b + 1] = su;
+    blocks[b + 1] = sr;
+  }
+  __syncthreads();
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = (EncodeTiledFn)p;
+  });
+  return fn;
+}
+
+// Boxes of 64 rows x 64 head dimensions (128 bytes, swizzled) out of the pages seen as [pages x kv heads x 64][hd]; what lies behind hd reads as 0.
+inline bool page_map(const void* base, long long rows, int hd, CUtensorMap* result) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint32_t estr[2] = {1, 1};
+  cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)hd * 2};
+  cuuint32_t box[2] = {64, (cuuint32_t)TK};
+  return fn(result, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a launch wants of its arguments.
+inline int check_tree(const TreeArgs& a, const char* what) {
+  LLG_REQUIRE(a.nh > 0 && a.nkv > 0 && a.nh % a.nkv == 0, "%s: %d heads are no multiple of %d key/value heads", what, a.nh, a.nkv);
+  LLG_REQUIRE(a.max_nodes > 0 && a.max_nodes <= LLG_TREE_NODES, "%s: trees of up to %d nodes (1 to %d)", what, a.max_nodes, LLG_TREE_NODES);
+  LLG_REQUIRE(a.n_seqs <= MAX_SEQS, "%s: %d sequences (at most %d)", what, a.n_seqs, MAX_SEQS);
+  LLG_REQUIRE(a.window >= 0 && a.ring_pages > 0 && a.table_width >= a.ring_pages, "%s: bad cache geometry", what);
+  LLG_REQUIRE(a.scale > 0.f, "%s: the softmax scale must be positive", what);
+  LLG_REQUIRE(a.part && a.counters && a.max_len > 0 && a.n_pages > 0, "%s: needs scratch, counters, a bound on the lengths and pages", what);
+  LLG_REQUIRE((uintptr_t)a.k_pages % 16 == 0 && (uintptr_t)a.v_pages % 16 == 0 && (uintptr_t)a.q % 16 == 0, "%s: storage must be 16-byte aligned", what);
+  LLG_REQUIRE((long long)a.n_pages * a.nkv * TK < 2147483647LL, "%s: too many page rows for a tensor map coordinate", what);
+  return 0;
+}
+
+}  // namespace

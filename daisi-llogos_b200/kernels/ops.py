@@ -563,6 +563,13 @@ def _load_lib(name: str):
         lib.llg_attn_tree_rows.argtypes = [c_int]
         if lib.llg_tree_max_nodes() != TREE_MAX_NODES:
             raise KernelError(f"the kernels take trees of {lib.llg_tree_max_nodes()} nodes, Python expects {TREE_MAX_NODES}")
+    elif name == "attention_tree_mma":
+        lib.llg_attn_tree_mma.argtypes = [POINTER(_TreeArgs), c_void_p]
+        lib.llg_attn_tree_mma_supported.argtypes = [c_int, c_int, c_int]
+        lib.llg_attn_tree_mma_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
+        lib.llg_attn_tree_mma_scratch_floats.restype = c_longlong
+        lib.llg_attn_tree_mma_counters.argtypes = [c_int, c_int, c_int]
+        lib.llg_attn_tree_mma_status.restype = c_int
     elif name == "key_weights":
         lib.llg_key_weights_simt.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
     elif name == "cache_rows":
@@ -2402,6 +2409,9 @@ def _step_layout(what: str, slots, cu_tokens, len_before, page_table) -> int:
     return b
 
 
+USE_MMA_TREE = True          # tests switch it off to reach the CUDA-core kernel with bfloat16
+
+
 class TreePlan:
     """How ``attn_tree`` will run for one batch shape.  Made by ``attn_tree_plan``; callers read ``scratch_floats`` and ``n_counters``."""
 
@@ -2425,8 +2435,13 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
     if n_seqs <= 0 or max_len <= 0:
         raise KernelError("attn_tree: needs sequences and a bound on their lengths")
     key = (dtype, n_seqs, n_heads, n_kv_heads, head_dim, vd)
-    lib = _lib("attention_tree")
     rows = max_nodes * (n_heads // n_kv_heads)
+    if USE_MMA_TREE and dtype == torch.bfloat16:
+        lib = _lib("attention_tree_mma")
+        if lib.llg_attn_tree_mma_supported(head_dim, vd, n_seqs):
+            return TreePlan("mma", key, 1, max_nodes, max_len, lib.llg_attn_tree_mma_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, vd, max_len),
+                            lib.llg_attn_tree_mma_counters(n_seqs, rows, n_kv_heads))
+    lib = _lib("attention_tree")
     per = lib.llg_attn_tree_rows(rows)
     blocks = n_seqs * n_kv_heads * -(-rows // per)
     tiles = -(-max_len // 32)
@@ -2480,8 +2495,17 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages = b, n, plan.max_nodes, k_pages.shape[0]
     a.nh, a.nkv, a.hd, a.vd, a.n_splits, a.max_len = nh, nkv, hd, vd, plan.n_splits, plan.max_len
     a.scale, a.window = float(scale), int(window)
-    lib = _lib("attention_tree")
-    _check(lib, lib.llg_attn_tree_simt(byref(a), _dt(q), _stream()))
+    if plan.kind == "mma":
+        lib = _lib("attention_tree_mma")
+        _check(lib, lib.llg_attn_tree_mma(byref(a), _stream()))
+    else:
+        lib = _lib("attention_tree")
+        _check(lib, lib.llg_attn_tree_simt(byref(a), _dt(q), _stream()))
+
+
+def attn_tree_status() -> int:
+    """Error code that the tensor-core kernels for drafted trees recorded when a wait ran out (0 = none); synchronises."""
+    return _lib("attention_tree_mma").llg_attn_tree_mma_status()
 
 
 def tree_accept_scratch(n_tokens: int, n_seqs: int) -> int:

@@ -217,6 +217,17 @@ def test_the_same_bits_twice_in_a_graph_and_on_another_stream(ops, dtype, hd):
         assert ((got - want).abs() <= slack + 1e-7).all()
 
 
+@pytest.mark.parametrize("hd,vd", [(64, 64), (128, 128), (80, 48), (8, 128)])
+def test_bfloat16_trees_on_the_cuda_cores(ops, hd, vd, monkeypatch):
+    monkeypatch.setattr(ops, "USE_MMA_TREE", False)
+    Case(BF16, 8, 2, hd, [70, 0, 600, 64], [5, 3, 64, 1], vd=vd, seed=hd).check(ops)
+
+
+def test_no_wait_has_run_out(ops):
+    """Behind the tests above: none of their launches gave a wait up."""
+    assert ops.attn_tree_status() == 0
+
+
 def test_pages_far_behind(ops):
     """Pools of more than 2^32 bytes and 2^31 elements: the last pages are the sequence's."""
     nkv, hd, n_pages = 8, 128, 34000
