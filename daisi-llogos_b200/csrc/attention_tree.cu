@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   for (int r = 0; r < RY; ++r) {
 #pragma unroll
     for (int k = 8; k > 0; k >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], k);
+    if (l[r] != l[r] && m[r] == -INFINITY) m[r] = 0.f;               // scores that are no numbers: the row has to show it
   }
   T* out = (T*)a.out;
   const int slots_per_row = a.n_splits;

@@ -322,6 +322,7 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+      if (l[r] != l[r] && m[r] == -INFINITY) m[r] = 0.f;             // scores that are no numbers: the row has to show it
     }
     const int rbs = row_blocks[cur.b + 1] - row_blocks[cur.b];
     const long long pair = (long long)a.nkv * row_blocks[cur.b] + (long long)cur.kvh * rbs + cur.rb;

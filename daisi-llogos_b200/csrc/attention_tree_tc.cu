@@ -1,0 +1,670 @@
+// Attention of large trees of drafted tokens over the paged cache on the 5th-generation tensor cores (tcgen05), bfloat16, head sizes 64 and 128.
+// What a node sees is said in cache_args.h, the formula in attention_tree.cu.
+//
+// With more than 64 query rows (nodes x heads of a group) mma.sync is what takes the time, not the cache.  Here a block takes 128 rows, which are
+// the lanes of tensor memory, and two groups of four softmax warps share the keys: the first group takes the even key tiles of the block's
+// run, the second the odd ones, each with scores S[128 x 64] (two buffers) and an accumulator O[128 x head] of its own in tensor memory, a
+// lane that issues its products, and two copying warps for both.  Thread r of a group owns row r, so a row's softmax needs no exchange; a
+// group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of), so a block passes a tile
+// every 1,000, where the memory system brings one every 1,400.
+//
+//   work       The units (sequence, key/value head, 128 rows, key tile) of the batch are one list that blocks, one a multiprocessor, cut into equal
+//              runs (tree_tiles.cuh); a run's keys and values are copied ahead across the ends of its segments.
+//   softmax    As in attention_tc.cu: weights 2^(x - M) with a whole number M that is raised only when a tile's weights add up to more than
+//              2^14, float32 sums, weights rounded to bfloat16 once.
+//   masks      A tile that holds nodes, the tree's end or the window's edge gives every row a 64-bit word of what it sees.  In such a tile a value
+//              that is not finite must not meet a weight of zero: the group looks its values over, and where it finds one adds the tile's products
+//              up itself, in tensor memory, leaving out what a row does not see; the issuing lane then leaves that tile out.
+//   joining    At a segment's end the groups' accumulators are added up; a segment that is not its rows' whole list of keys leaves partial rows
+//              and takes a ticket, and who has the last one joins them in the runs' order.
+//
+// Every wait is bounded (llg_attn_tree_tc_status); every role comes to the block's end, where tensor memory is freed.  No load uses cluster multicast.
+#include "tree_tiles.cuh"
+
+LLG_API const char* llg_last_error() { return g_llg_error; }
+
+namespace {
+
+constexpr int BQ = 128;                       // rows of a block: lanes of tensor memory
+constexpr int GROUPS = 2, WORKERS = GROUPS * BQ;
+constexpr int ISSUE_WARP = WORKERS / 32, K_LOAD_WARP = ISSUE_WARP + 1, V_LOAD_WARP = ISSUE_WARP + 2, ISSUE_WARP_2 = ISSUE_WARP + 3;
+constexpr int THREADS = (ISSUE_WARP_2 + 1) * 32;
+constexpr int TMEM_COLS = 512;
+constexpr uint32_t G_COLS = 256, O_COL = 128;       // a group's columns: S 2 x 64, O from column 128
+
+// 0 ok; waits that ran out: 1 scores, 2 accumulator, 4 free stage, 5 tile or queries copied, 6 weights, 7 copies at the end, 8 a meeting; 3 shared memory not aligned
+__device__ int g_error = 0;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// K-major operand, rows of 128 bytes with the 128-byte swizzle, 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// MN-major operand: 64 elements of the MN dimension in one swizzled 128-byte row per k, the next 64 `lbo_bytes` further
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, uint32_t lbo_bytes) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(pred));
+  return pred != 0;
+}
+// byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a tile of 128-byte rows with the 128-byte swizzle
+__device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+
+// ST: stages of keys, and of values; even, so that a stage belongs to one group
+template <int HD, int ST>
+__global__ void __launch_bounds__(THREADS, 1)
+attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeArgs a) {
+  static_assert(ST % 2 == 0, "the groups take turns with the tiles: a stage's phases are waited for by one of them");
+  constexpr int KB = HD / 64, Q_BYTES = KB * BQ * 128, KV_BYTES = KB * TK * 128, CPR = HD / 8;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char* Qs = smem;
+  unsigned char* Ks = Qs + Q_BYTES;                  // [ST]
+  unsigned char* Vs = Ks + ST * KV_BYTES;            // [ST]
+  __shared__ uint64_t k_full[ST], k_free[ST], v_full[ST], v_free[ST];
+  __shared__ uint64_t s_full[GROUPS][2], p_ready[GROUPS][2], o_done[GROUPS], q_ready[GROUPS], meet_bar, group_bar[GROUPS];
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag, last_ticket;
+  __shared__ int wild[GROUPS][3], leave_out[GROUPS][2];
+  __shared__ float2 share[GROUPS][BQ];               // each group's maximum and sum of a row
+  __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1];
+  __shared__ int2 warp_total[THREADS / 32];
+
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if ((smem_u32(smem) & 1023u) != 0) {               // uniform over the block
+    if (tid == 0) atomicCAS(&g_error, 0, 3);
+    return;
+  }
+  plan_units<THREADS>(a, BQ, sums, row_blocks, warp_total);
+  const int G = a.nh / a.nkv;
+  const long long units = (long long)a.nkv * sums[a.n_seqs];
+  const long long chunk = (units + gridDim.x - 1) / gridDim.x;
+  const long long u0 = (long long)blockIdx.x * chunk, u1 = min(units, u0 + chunk);
+  if (u0 >= u1) return;                              // uniform over the block
+  const int n_units = (int)(u1 - u0);
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_free[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_free[s], 1);
+    }
+    for (int g = 0; g < GROUPS; ++g) {
+      mbar_init(&s_full[g][0], 1);
+      mbar_init(&s_full[g][1], 1);
+      mbar_init(&p_ready[g][0], BQ / 32);
+      mbar_init(&p_ready[g][1], BQ / 32);
+      mbar_init(&o_done[g], 1);
+      mbar_init(&group_bar[g], BQ);
+      mbar_init(&q_ready[g], WORKERS);
+      wild[g][0] = wild[g][1] = wild[g][2] = 0;
+      leave_out[g][0] = leave_out[g][1] = 0;
+    }
+    mbar_init(&meet_bar, WORKERS);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    warp_whole();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
+                 "r"((uint32_t)TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  // (not before: a block of the next kernel must not take tensor memory ahead of this one and then wait for it)
+  pdl_launch_dependents();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_base_slot;
+  volatile int* abortp = &abort_flag;
+  auto give_up = [&](int code) {
+    if (!*abortp) { *abortp = 1; atomicCAS(&g_error, 0, code); }
+  };
+
+  if (warp == K_LOAD_WARP || warp == V_LOAD_WARP) {
+    // ---- copies: the lanes look up the pages of 32 tiles side by side, then each in turn issues its tile's boxes ----
+    const bool keys = warp == K_LOAD_WARP;
+    unsigned char* base = keys ? Ks : Vs;
+    uint64_t* full = keys ? k_full : v_full;
+    uint64_t* freeb = keys ? k_free : v_free;
+    const CUtensorMap* map = keys ? &map_k : &map_v;
+    if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    int issued = 0;
+    bool fine = true;
+    for (int first = 0; first < n_units && fine; first += 32) {
+      const int idx = first + lane;
+      int row = 0;
+      if (idx < n_units) {
+        const Unit c = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + idx);
+        const int tile = tree_shape(a, c.b).t_first + c.t;
+        const int page = a.page_table[(long long)a.slots[c.b] * a.table_width + tile % a.ring_pages];
+        row = (page * a.nkv + c.kvh) * TK;
+      }
+      const int n_here = min(32, n_units - first);
+      for (int k = 0; k < n_here && fine; ++k) {
+        if (lane == k) {
+          const int i = first + k, st = i % ST;
+          if (i >= ST && !mbar_wait(&freeb[st], (i / ST - 1) & 1, abortp)) {
+            give_up(4);
+            fine = false;
+          } else {
+            mbar_expect_tx(&full[st], KV_BYTES);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) tma_load_2d(smem_u32(base + st * KV_BYTES + kb * (TK * 128)), map, kb * 64, row, &full[st]);
+          }
+        }
+        fine = __shfl_sync(0xffffffffu, (int)fine, k) != 0;
+        if (fine) ++issued;
+      }
+    }
+    // copies still write into this block's shared memory until their barrier completes
+    if (lane == 0) {
+      for (int i = max(0, issued - ST); i < issued; ++i) {
+        const unsigned long long t0 = now_ns();
+        while (!mbar_try_wait(&full[i % ST], (i / ST) & 1)) {
+          if (now_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(&g_error, 0, 7); break; }
+        }
+      }
+    }
+  } else if (warp == ISSUE_WARP || warp == ISSUE_WARP_2) {
+    // ---- products: a lane per group issues them -------------------------------------------------------
+    if (elect_one()) {
+      const int g = warp == ISSUE_WARP ? 0 : 1;
+      constexpr uint32_t IDESC_S = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+      constexpr uint32_t IDESC_O = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+      bool ok = true;
+      auto wait_or_fail = [&](uint64_t* bar, uint32_t parity, int code) {
+        if (!ok) return;
+        if (!mbar_wait(bar, parity, abortp)) {
+          give_up(code);
+          ok = false;
+        }
+      };
+      // Tile i of the run is the group's tile c = i / 2.  Scores into buffer c % 2, which O += P(c-2) V(c-2) has read by then; a segment's first
+      // tile comes when all of the earlier ones are done, and waits for the last of them (a wait by parity sees one phase back).
+      auto issue_scores = [&](int i, bool first) {
+        const int c = i >> 1;
+        wait_or_fail(&k_full[i % ST], (i / ST) & 1, 5);
+        if (first ? c >= 1 : c >= 2) wait_or_fail(&o_done[g], (first ? c - 1 : c) & 1, 6);
+        if (!ok) return;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t qa = smem_u32(Qs), ka = smem_u32(Ks + (i % ST) * KV_BYTES);
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          const uint32_t blk = ks >> 2, kk = ks & 3;
+          umma_bf16(tmem + g * G_COLS + (uint32_t)(c & 1) * TK, desc_kmajor(qa + blk * (BQ * 128) + kk * 32),
+                    desc_kmajor(ka + blk * (TK * 128) + kk * 32), IDESC_S, ks != 0);
+        }
+        umma_commit(&s_full[g][c & 1]);
+        umma_commit(&k_free[i % ST]);
+      };
+      int i0 = 0;
+      uint32_t segments = 0;                           // of this group: those in which it has a tile
+      while (i0 < n_units && ok) {
+        const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
+        const int tiles = (sums[cur.b + 1] - sums[cur.b]) / (row_blocks[cur.b + 1] - row_blocks[cur.b]);
+        const int i1 = min(n_units, i0 + tiles - cur.t);
+        int i = i0 + ((i0 ^ g) & 1);
+        bool started = false;
+        if (i < i1) {
+          wait_or_fail(&q_ready[g], segments++ & 1, 5);
+          issue_scores(i, true);
+        }
+        for (; i < i1 && ok; i += 2) {
+          const int c = i >> 1;
+          if (i + 2 < i1) issue_scores(i + 2, false);
+          wait_or_fail(&v_full[i % ST], (i / ST) & 1, 5);
+          wait_or_fail(&p_ready[g][c & 1], (c >> 1) & 1, 6);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          if (*reinterpret_cast<volatile int*>(&leave_out[g][c & 1])) {
+            umma_commit(&o_done[g]);                   // the group has added this tile up itself, and gives its values back itself
+          } else {
+            const uint32_t pa = tmem + g * G_COLS + (uint32_t)(c & 1) * TK, va = smem_u32(Vs + (i % ST) * KV_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk)
+              umma_bf16_ts(tmem + g * G_COLS + O_COL, pa + kk * 8, desc_mnmajor(va + kk * 2048, TK * 128), IDESC_O, started || kk != 0);
+            umma_commit(&o_done[g]);
+            umma_commit(&v_free[i % ST]);
+          }
+          started = true;
+        }
+        i0 = i1;
+      }
+    }
+  } else {
+    // ---- softmax: thread r of group g owns row r -------------------------------------------------------
+    const int g = tid / BQ, r = tid % BQ, gw = (tid % BQ) >> 5;       // gw: warp inside the group = its lane quarter
+    const uint32_t quarter = (uint32_t)(gw * 32) << 16, lane_base = tmem + g * G_COLS + quarter;
+    const float sc = a.scale * LOG2E;
+    const float sum_bound = 16384.0f;
+    uint32_t meets = 0, group_meets = 0;
+    // Meetings of all softmax threads, and of a group's: waits with a limit.  The answer is the warp's.
+    auto meet = [&]() -> bool {
+      mbar_arrive(&meet_bar);
+      const bool met = mbar_wait(&meet_bar, meets & 1, abortp);
+      ++meets;
+      if (!met) give_up(8);
+      return warp_all(met);
+    };
+    auto group_meet = [&]() -> bool {
+      mbar_arrive(&group_bar[g]);
+      const bool met = mbar_wait(&group_bar[g], group_meets & 1, abortp);
+      ++group_meets;
+      if (!met) give_up(8);
+      return warp_all(met);
+    };
+    int looked = 0;                                     // tiles that the group has looked over for values that are not finite
+    int i0 = 0;
+    bool ok = true;
+    while (i0 < n_units && ok) {
+      const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
+      const TreeShape sh = tree_shape(a, cur.b);
+      const int i1 = min(n_units, i0 + sh.tiles - cur.t);
+      const int row0 = cur.rb * BQ, n_rows = min(BQ, sh.n * G - row0);
+      const bool live = r < n_rows;
+      const int node = live ? (row0 + r) / G : 0, head = live ? cur.kvh * G + (row0 + r) - node * G : 0;
+      // queries: all softmax threads copy; rows behind the last are zeros
+      {
+        const int ch = tid % CPR;
+        for (int row = tid / CPR; row < BQ; row += WORKERS / CPR) {
+          const bool valid = row < n_rows;
+          const int at = valid ? row0 + row : 0, nd = at / G;
+          const bf16* src = (const bf16*)a.q + ((long long)(sh.tok0 + nd) * a.nh + cur.kvh * G + at - nd * G) * HD + ch * 8;
+          cp_async16(smem_u32(Qs) + (uint32_t)((ch >> 3) * (BQ * 128)) + swz(row, ch & 7), src, valid);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      unsigned long long bits = live ? (unsigned long long)a.ancestors[sh.tok0 + node] : 0ull;
+      const int depth = __popcll(bits) - 1;
+      bits &= sh.n >= 64 ? ~0ull : (1ull << sh.n) - 1;
+      if (a.window > 0 && depth >= a.window)            // of its ancestors, those less than a window above it
+        for (int j = 0; j < sh.n; ++j)
+          if (((bits >> j) & 1) && depth - (__popcll(a.ancestors[sh.tok0 + j]) - 1) >= a.window) bits &= ~(1ull << j);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      fence_async_smem();
+      // each issuing lane is told of the segments in which its group has a tile, and no others: it cannot fall behind by a phase
+      if (i0 + (i0 & 1) < i1) mbar_arrive(&q_ready[0]);
+      if (i0 + ((i0 & 1) ^ 1) < i1) mbar_arrive(&q_ready[1]);
+
+      float m_run = -INFINITY, l_run = 0.f;
+      const int own0 = i0 + ((i0 ^ g) & 1);
+      for (int i = own0; i < i1; i += 2) {
+        const int c = i >> 1;
+        const bool first = i == own0, last = i + 2 >= i1;
+        const bool scored = mbar_wait(&s_full[g][c & 1], (c >> 1) & 1, abortp);
+        if (!scored) give_up(1);
+        ok = warp_all(scored);
+        if (!ok) break;                      // uniform
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int p0 = (sh.t_first + cur.t + i - i0) * TK;
+        float sv[TK];
+        {
+          uint32_t r0_[16], r1_[16], r2_[16], r3_[16];
+          const uint32_t sa = lane_base + (uint32_t)(c & 1) * TK;
+          tmem_ld16(sa, r0_);
+          tmem_ld16(sa + 16, r1_);
+          tmem_ld16(sa + 32, r2_);
+          tmem_ld16(sa + 48, r3_);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            sv[x] = __uint_as_float(r0_[x]);
+            sv[16 + x] = __uint_as_float(r1_[x]);
+            sv[32 + x] = __uint_as_float(r2_[x]);
+            sv[48 + x] = __uint_as_float(r3_[x]);
+          }
+        }
+        const bool mixed = p0 + TK > sh.lb || (a.window > 0 && p0 <= sh.lb + sh.n - a.window);      // the same for the block
+        bool by_hand = false;
+        if (mixed) {                          // uniform
+          const int shift = sh.lb - p0;      // places of the tile that are cached keys
+          unsigned long long cached = shift >= 64 ? ~0ull : shift > 0 ? (1ull << shift) - 1 : 0ull;
+          if (a.window > 0) {
+            const int from = shift + depth - a.window + 1;
+            cached = from >= 64 ? 0ull : from > 0 ? cached & (~0ull << from) : cached;
+          }
+          const unsigned long long nodes = shift >= 64 ? 0ull : shift >= 0 ? bits << shift : shift > -64 ? bits >> -shift : 0ull;
+          const unsigned long long seen = cached | nodes;
+          const uint32_t s_lo = (uint32_t)seen, s_hi = (uint32_t)(seen >> 32);
+#pragma unroll
+          for (int x = 0; x < TK; ++x) sv[x] = ((x < 32 ? s_lo : s_hi) >> (x & 31)) & 1 ? sv[x] : -INFINITY;
+          // the group looks the tile's values over
+          const bool landed = mbar_wait(&v_full[i % ST], (i / ST) & 1, abortp);
+          if (!landed) give_up(5);
+          bool found = false;
+          if (landed) {
+            const uint4* v = reinterpret_cast<const uint4*>(Vs + (i % ST) * KV_BYTES);
+#pragma unroll
+            for (int x = 0; x < KV_BYTES / 16 / BQ; ++x) {
+              const uint4 y = v[x * BQ + r];
+              found |= not_finite(y.x) || not_finite(y.y) || not_finite(y.z) || not_finite(y.w);
+            }
+          }
+          if (found) *reinterpret_cast<volatile int*>(&wild[g][looked % 3]) = 1;
+          if (r == 0) *reinterpret_cast<volatile int*>(&wild[g][(looked + 1) % 3]) = 0;      // last read before the meeting ahead of this one
+          ok = warp_all(landed);
+          ok = group_meet() && ok;
+          if (!ok) break;                    // uniform
+          by_hand = *reinterpret_cast<volatile int*>(&wild[g][looked % 3]) != 0;
+          ++looked;
+        }
+        uint32_t pk[TK / 2];
+        float psum;
+        auto weights = [&](float m) {
+          const float ms = m == -INFINITY ? 0.f : m;
+          const float2 sc2 = make_float2(sc, sc), nms2 = make_float2(-ms, -ms);
+          float2 ps2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+          for (int e = 0; e < TK / 2; ++e) {
+            const float2 x = __ffma2_rn(make_float2(sv[2 * e], sv[2 * e + 1]), sc2, nms2);
+            const float2 w = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            ps2[e & 1] = __fadd2_rn(ps2[e & 1], w);
+            pk[e] = pack_bf16(w.x, w.y);
+          }
+          psum = (ps2[0].x + ps2[0].y) + (ps2[1].x + ps2[1].y);
+        };
+        float corr = 1.f;
+        bool fits = false, rescale = false;              // the latter one answer for the warp
+#pragma unroll 1
+        for (int pass = first; ; ++pass) {
+          if (pass == 1) {
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < TK; x += 8) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mx4[k] = max3(mx4[k], sv[x + 2 * k], sv[x + 2 * k + 1]);
+            }
+            const float mxs = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
+            const float m_new = fits ? m_run : fmaxf(m_run, ceilf(mxs));
+            corr = m_new == m_run || m_new == -INFINITY ? 1.f : pow2_whole(m_run - m_new);
+            m_run = m_new;
+            rescale = !warp_all(corr == 1.f);
+          }
+          weights(m_run);
+          fits = m_run != -INFINITY && psum <= sum_bound;
+          if (pass == 1 || warp_all(fits)) break;        // uniform
+        }
+        l_run = l_run * corr + psum;
+        if (!by_hand) {                                  // uniform
+          warp_whole();
+#pragma unroll
+          for (int c16 = 0; c16 < TK / 32; ++c16)        // uniform
+            tmem_st16(lane_base + (uint32_t)(c & 1) * TK + c16 * 16, reinterpret_cast<const uint32_t(&)[16]>(pk[c16 * 16]));
+        }
+        // O += P(c-1) V(c-1) has finished: before O is touched, and at the segment's last tile (a wait by parity sees one phase back)
+        const bool touch = !first && (rescale || by_hand);
+        if (touch || (!first && last)) {
+          const bool added = mbar_wait(&o_done[g], (c - 1) & 1, abortp);
+          if (!added) give_up(2);
+          ok = warp_all(added);
+          if (!ok) break;                                // uniform
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (touch || by_hand) {                          // uniform
+          const unsigned char* vt = Vs + (i % ST) * KV_BYTES;
+#pragma unroll 1
+          for (int c0 = 0; c0 < HD; c0 += 16) {          // uniform
+            uint32_t rr[16];
+            warp_whole();
+            if (!first) {                                // uniform
+              tmem_ld16(lane_base + O_COL + c0, rr);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            }
+#pragma unroll
+            for (int x = 0; x < 16; ++x) rr[x] = first ? 0u : __float_as_uint(__uint_as_float(rr[x]) * corr);
+            if (by_hand) {                               // uniform
+              const unsigned char* vb = vt + (c0 >> 6) * (TK * 128);
+              const int ch = (c0 & 63) >> 3;
+#pragma unroll 1
+              for (int k2 = 0; k2 < TK / 2; ++k2) {
+                uint32_t w2 = 0;
+#pragma unroll
+                for (int e = 0; e < TK / 2; ++e) w2 = e == k2 ? pk[e] : w2;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float w = __uint_as_float(e ? w2 & 0xffff0000u : w2 << 16);
+                  const int k = 2 * k2 + e;
+                  if (w != 0.f) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                      const uint4 y = *reinterpret_cast<const uint4*>(vb + swz(k, ch + q));
+                      const uint32_t yy[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                      for (int z = 0; z < 4; ++z) {
+                        rr[q * 8 + 2 * z] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] << 16), __uint_as_float(rr[q * 8 + 2 * z])));
+                        rr[q * 8 + 2 * z + 1] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] & 0xffff0000u), __uint_as_float(rr[q * 8 + 2 * z + 1])));
+                      }
+                    }
+                  }
+                }
+              }
+            }
+            warp_whole();
+            tmem_st16(lane_base + O_COL + c0, rr);
+          }
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        if (mixed) {                                     // uniform: only such a tile changes what the issuing lane reads here
+          if (by_hand) {
+            ok = group_meet();                           // all of the group have read the values
+            if (!ok) break;                              // uniform
+            if (r == 0) mbar_arrive(&v_free[i % ST]);
+          }
+          if (r == 0) *reinterpret_cast<volatile int*>(&leave_out[g][c & 1]) = by_hand;
+        } else if (r == 0) {
+          *reinterpret_cast<volatile int*>(&leave_out[g][c & 1]) = 0;
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[g][c & 1]);
+        if (last) {
+          const bool added = mbar_wait(&o_done[g], c & 1, abortp);
+          if (!added) give_up(2);
+          ok = warp_all(added);
+        }
+      }
+      if (!ok) break;                                    // uniform
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      // ---- the segment's result: the groups' accumulators added up, each thread half of its row's columns ------------
+      if (l_run != l_run && m_run == -INFINITY) m_run = 0.f;       // scores that are no numbers: the row has to show it
+      share[g][r] = make_float2(m_run, l_run);
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      ok = meet();
+      if (!ok) break;                                    // uniform
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const float2 ml0 = share[0][r], ml1 = share[1][r];
+      const float M = fmaxf(ml0.x, ml1.x);
+      float w0 = ml0.x == -INFINITY ? 0.f : pow2_whole(ml0.x - M), w1 = ml1.x == -INFINITY ? 0.f : pow2_whole(ml1.x - M);
+      const float L = ml0.y * w0 + ml1.y * w1;
+      const bool some0 = ml0.x != -INFINITY, some1 = ml1.x != -INFINITY;      // (an accumulator without a tile holds anything)
+      const int rbs = row_blocks[cur.b + 1] - row_blocks[cur.b];
+      const long long pair = (long long)a.nkv * row_blocks[cur.b] + (long long)cur.kvh * rbs + cur.rb;
+      const long long p_first = (long long)a.nkv * sums[cur.b] + ((long long)cur.kvh * rbs + cur.rb) * sh.tiles;
+      const int blk_first = (int)(p_first / chunk), blk_last = (int)((p_first + sh.tiles - 1) / chunk);
+      const bool whole = blk_first == blk_last;
+      constexpr int PW = HD + PART_PAD;
+      float* mine = a.part + (blockIdx.x + pair) * (long long)(BQ * PW) + r * PW;
+      bf16* dst = (bf16*)a.out + ((long long)(sh.tok0 + node) * a.nh + head) * HD;
+      if (whole) {
+        const float inv = L != 0.f ? 1.f / L : 0.f;
+        w0 *= inv;
+        w1 *= inv;
+      } else if (g == 0 && live) {
+        *reinterpret_cast<float2*>(mine + HD) = make_float2(M, L);
+      }
+      const uint32_t orow = tmem + O_COL + quarter;
+#pragma unroll 1
+      for (int c0 = g * (HD / 2); c0 < (g + 1) * (HD / 2); c0 += 16) {       // uniform
+        uint32_t r0_[16], r1_[16];
+        warp_whole();
+        tmem_ld16(orow + c0, r0_);
+        tmem_ld16(orow + G_COLS + c0, r1_);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        float o[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          o[x] = some0 ? w0 * __uint_as_float(r0_[x]) : 0.f;
+          if (some1) o[x] = fmaf(w1, __uint_as_float(r1_[x]), o[x]);
+        }
+        if (live && whole) {
+          uint4 v0, v1;
+          v0.x = pack_bf16(o[0], o[1]); v0.y = pack_bf16(o[2], o[3]); v0.z = pack_bf16(o[4], o[5]); v0.w = pack_bf16(o[6], o[7]);
+          v1.x = pack_bf16(o[8], o[9]); v1.y = pack_bf16(o[10], o[11]); v1.z = pack_bf16(o[12], o[13]); v1.w = pack_bf16(o[14], o[15]);
+          *reinterpret_cast<uint4*>(dst + c0) = v0;
+          *reinterpret_cast<uint4*>(dst + c0 + 8) = v1;
+        } else if (live) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(mine + c0 + 4 * q) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // the next segment's products overwrite what was read
+      __syncwarp();
+      if (!whole) {
+        __threadfence();                                 // the partial rows are visible to the whole device ...
+        ok = meet();
+        if (!ok) break;                                  // uniform
+        if (tid == 0) {
+          const int ticket = atomicAdd(&a.counters[pair], 1);       // ... before the ticket is
+          last_ticket = ticket == blk_last - blk_first;
+          if (last_ticket) a.counters[pair] = 0;
+        }
+        __syncwarp();
+        ok = meet();
+        if (!ok) break;                                  // uniform
+        if (last_ticket) {
+          __threadfence();
+          for (int x = tid; x < n_rows * (HD / 4); x += WORKERS) {
+            const int row = x / (HD / 4), d = (x % (HD / 4)) * 4;
+            const float* p = a.part + (blk_first + pair) * (long long)(BQ * PW) + row * PW;
+            float Mj = -INFINITY, Lj = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = blk_first; k <= blk_last; ++k, p += BQ * PW) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + HD));
+              if (ml.x == -INFINITY) continue;
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(p + d));
+              const float top = fmaxf(Mj, ml.x), f = Mj == -INFINITY ? 0.f : pow2_whole(Mj - top), w = pow2_whole(ml.x - top);
+              Mj = top;
+              Lj = Lj * f + ml.y * w;
+              acc.x = acc.x * f + v.x * w;
+              acc.y = acc.y * f + v.y * w;
+              acc.z = acc.z * f + v.z * w;
+              acc.w = acc.w * f + v.w * w;
+            }
+            const float inv = Lj != 0.f ? 1.f / Lj : 0.f;
+            const int nd = (row0 + row) / G;
+            bf16* to = (bf16*)a.out + ((long long)(sh.tok0 + nd) * a.nh + cur.kvh * G + (row0 + row) - nd * G) * HD + d;
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+          }
+        }
+        __syncwarp();
+      }
+      ok = meet();                                       // shares, last_ticket and the queries' place are free again
+      i0 = i1;
+    }
+  }
+  // every role comes here, also after a wait that ran out: copies in flight have been waited for above
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    warp_whole();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM_COLS) : "memory");
+  }
+}
+
+int grid_blocks(int n_seqs, int nkv, int row_blocks, int max_len) {
+  const long long units = (long long)n_seqs * nkv * row_blocks * ((max_len + TK - 1) / TK), most = llg_sm_count();
+  return (int)(units < most ? (units < 1 ? 1 : units) : most);
+}
+
+template <int HD, int ST>
+int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t stream) {
+  constexpr int smem = (HD / 64) * (BQ * 128 + 2 * ST * TK * 128);      // more than half a multiprocessor's: tensor memory is a block's alone
+  cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return llg_fail("attn_tree_tc: shared memory %d: %s", smem, cudaGetErrorString(e));
+  e = llg_launch(attn_tree_tc_kernel<HD, ST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, a);
+  if (e != cudaSuccess) return llg_fail("attn_tree_tc: launch: %s", cudaGetErrorString(e));
+  return llg_check_launch("attn_tree_tc");
+}
+
+}  // namespace
+
+// 1 when this kernel takes the geometry (bfloat16 only).
+LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs) { return (hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS; }
+
+// Floats of scratch, and counters, of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
+LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int rows, int nkv, int hd, int max_len) {
+  const int rbs = (rows + BQ - 1) / BQ;
+  return ((long long)grid_blocks(n_seqs, nkv, rbs, max_len) + (long long)n_seqs * nkv * rbs) * BQ * (hd + PART_PAD);
+}
+LLG_API int llg_attn_tree_tc_counters(int n_seqs, int rows, int nkv) { return n_seqs * nkv * ((rows + BQ - 1) / BQ); }
+
+LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
+  const TreeArgs& a = *args;
+  if (check_tree(a, "attn_tree_tc")) return 1;
+  LLG_REQUIRE(llg_attn_tree_tc_supported(a.hd, a.vd, a.n_seqs), "attn_tree_tc: heads of %d and %d elements (64 or 128, the same)", a.hd, a.vd);
+  if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
+  CUtensorMap mk, mv;
+  const long long rows = (long long)a.n_pages * a.nkv * TK;
+  if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv))
+    return llg_fail("attn_tree_tc: cuTensorMapEncodeTiled failed or is not available");
+  const int rbs = (a.max_nodes * (a.nh / a.nkv) + BQ - 1) / BQ, blocks = grid_blocks(a.n_seqs, a.nkv, rbs, a.max_len);
+  return a.hd == 64 ? launch<64, 8>(a, mk, mv, blocks, stream) : launch<128, 4>(a, mk, mv, blocks, stream);
+}
+
+// Error code recorded when a wait ran out (0 = none); clears it.  Synchronises the device.
+LLG_API int llg_attn_tree_tc_status() {
+  int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
+  return v;
+}

@@ -49,6 +49,7 @@ SOURCES: Dict[str, List[str]] = {
     "moe": ["moe.cu", "common.cuh", "kernel_args.h"],
     "attention_tree": ["attention_tree.cu", "common.cuh", "cache_args.h"],
     "attention_tree_mma": ["attention_tree_mma.cu", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
+    "attention_tree_tc": ["attention_tree_tc.cu", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "key_weights": ["key_weights.cu", "key_weights.cuh", "common.cuh", "cache_args.h"],
     "cache_rows": ["cache_rows.cu", "common.cuh", "cache_args.h"],
 }

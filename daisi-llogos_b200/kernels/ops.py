@@ -570,6 +570,13 @@ def _load_lib(name: str):
         lib.llg_attn_tree_mma_scratch_floats.restype = c_longlong
         lib.llg_attn_tree_mma_counters.argtypes = [c_int, c_int, c_int]
         lib.llg_attn_tree_mma_status.restype = c_int
+    elif name == "attention_tree_tc":
+        lib.llg_attn_tree_tc.argtypes = [POINTER(_TreeArgs), c_void_p]
+        lib.llg_attn_tree_tc_supported.argtypes = [c_int, c_int, c_int]
+        lib.llg_attn_tree_tc_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int]
+        lib.llg_attn_tree_tc_scratch_floats.restype = c_longlong
+        lib.llg_attn_tree_tc_counters.argtypes = [c_int, c_int, c_int]
+        lib.llg_attn_tree_tc_status.restype = c_int
     elif name == "key_weights":
         lib.llg_key_weights_simt.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
     elif name == "cache_rows":
@@ -2409,6 +2416,8 @@ def _step_layout(what: str, slots, cu_tokens, len_before, page_table) -> int:
     return b
 
 
+USE_TC_TREE = True           # tests switch it off to reach the mma.sync kernel with many rows
+TREE_MMA_ROWS = 64           # query rows (nodes x heads of a group) up to which drafted trees' attention runs on mma.sync
 USE_MMA_TREE = True          # tests switch it off to reach the CUDA-core kernel with bfloat16
 
 
@@ -2436,6 +2445,11 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
         raise KernelError("attn_tree: needs sequences and a bound on their lengths")
     key = (dtype, n_seqs, n_heads, n_kv_heads, head_dim, vd)
     rows = max_nodes * (n_heads // n_kv_heads)
+    if USE_TC_TREE and dtype == torch.bfloat16 and rows > TREE_MMA_ROWS:
+        lib = _lib("attention_tree_tc")
+        if lib.llg_attn_tree_tc_supported(head_dim, vd, n_seqs):
+            return TreePlan("tc", key, 1, max_nodes, max_len, lib.llg_attn_tree_tc_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, max_len),
+                            lib.llg_attn_tree_tc_counters(n_seqs, rows, n_kv_heads))
     if USE_MMA_TREE and dtype == torch.bfloat16:
         lib = _lib("attention_tree_mma")
         if lib.llg_attn_tree_mma_supported(head_dim, vd, n_seqs):
@@ -2488,14 +2502,17 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     _on_one_device(what, q, k_pages, v_pages, page_table, slots, cu_tokens, len_before, ancestors, out, scratch, counters)
     a = _TreeArgs()
     a.q, a.k_pages, a.v_pages = _ptr(q), _ptr(k_pages), _ptr(v_pages)
-    _wide(what, q, k_pages, v_pages, scratch)
+    _wide(what, q, k_pages, v_pages, out, scratch)
     a.page_table, a.table_width, a.ring_pages = _ptr(page_table), page_table.shape[1], ring_pages
     a.slots, a.cu_tokens, a.len_before, a.ancestors = _ptr(slots), _ptr(cu_tokens), _ptr(len_before), _ptr(ancestors)
     a.out, a.part, a.counters = _ptr(out), _ptr(scratch), _ptr(counters)
     a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages = b, n, plan.max_nodes, k_pages.shape[0]
     a.nh, a.nkv, a.hd, a.vd, a.n_splits, a.max_len = nh, nkv, hd, vd, plan.n_splits, plan.max_len
     a.scale, a.window = float(scale), int(window)
-    if plan.kind == "mma":
+    if plan.kind == "tc":
+        lib = _lib("attention_tree_tc")
+        _check(lib, lib.llg_attn_tree_tc(byref(a), _stream()))
+    elif plan.kind == "mma":
         lib = _lib("attention_tree_mma")
         _check(lib, lib.llg_attn_tree_mma(byref(a), _stream()))
     else:
@@ -2505,7 +2522,7 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
 def attn_tree_status() -> int:
     """Error code that the tensor-core kernels for drafted trees recorded when a wait ran out (0 = none); synchronises."""
-    return _lib("attention_tree_mma").llg_attn_tree_mma_status()
+    return _lib("attention_tree_mma").llg_attn_tree_mma_status() or 100 * _lib("attention_tree_tc").llg_attn_tree_tc_status()
 
 
 def tree_accept_scratch(n_tokens: int, n_seqs: int) -> int:

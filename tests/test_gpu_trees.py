@@ -217,9 +217,57 @@ def test_the_same_bits_twice_in_a_graph_and_on_another_stream(ops, dtype, hd):
         assert ((got - want).abs() <= slack + 1e-7).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("before,nodes", [([0], [17]), ([0, 1, 2, 3], [20, 17, 64, 33]), ([40] * 40, [20] * 40), ([64, 700, 0, 9], [64, 33, 1, 2]),
+                                          ([5000], [64]), ([3000, 20], [40, 64])], ids=lambda x: "_".join(map(str, x[:4])))
+@pytest.mark.parametrize("nh,nkv", [(8, 2), (10, 2), (3, 3), (16, 1)])
+def test_many_rows(ops, hd, before, nodes, nh, nkv, monkeypatch):
+    """Row blocks of 128: one and several, whole and with a few rows, runs of one key tile and of many; on both matrix paths."""
+    c = Case(BF16, nh, nkv, hd, before, nodes, seed=hd + nh)
+    c.check(ops)
+    monkeypatch.setattr(ops, "USE_TC_TREE", False)
+    c.check(ops)
+
+
+@pytest.mark.parametrize("tc", [True, False], ids=["tc", "mma"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_what_many_rows_do_not_see_has_no_part(ops, hd, tc, monkeypatch):
+    """Values that are not finite, in a tree of many rows: at its first tile, at a later one, with rows that rise in between."""
+    monkeypatch.setattr(ops, "USE_TC_TREE", tc)
+    for before in (0, 30, 64, 200, 1000):
+        parents = [-1, 0, 0, 1, 2, 2, 4] + [6 + i for i in range(20)]
+        bits = T.tree_bits(parents)
+
+        def spoil(c):
+            c.v[0][before + 5] = float("nan")
+            c.v[0][before + 3, :, 1] = float("inf")
+            c.k[0][before + 3] *= 8
+        c = Case(BF16, 16, 2, hd, [before], [27], bits=[bits], seed=9, spoil=spoil)
+        out, _ = c.call(ops)
+        want, slack = c.want()
+        got = out.cpu().double().view(27, 16, hd)
+        clean = torch.tensor([i for i in range(27) if not bits[i] >> 5 & 1 and not bits[i] >> 3 & 1])
+        assert torch.isfinite(got[clean]).all() and len(clean) > 20
+        assert ((got - want.view(27, 16, hd)).abs()[clean] <= slack.view(27, 16, hd)[clean] + 1e-7).all()
+        assert torch.isnan(got[5]).all() and not torch.isfinite(got[3, :, 1]).any() and torch.isfinite(got[3, :, 2:]).all()
+
+
+@pytest.mark.parametrize("dtype,nh,hd", [(F32, 8, 64), (BF16, 8, 64), (BF16, 8, 20), (BF16, 32, 128)], ids=["f32", "mma", "simt", "tc"])
+def test_queries_that_are_no_numbers_show(ops, dtype, nh, hd):
+    c = Case(dtype, nh, 2, hd, [500, 70], [9, 3], seed=4)
+    c.args[0][2] = float("nan")
+    c.args[0][10, 1] = float("nan")
+    out, _ = c.call(ops)
+    out = out.view(12, nh, hd)
+    assert torch.isnan(out[2]).all() and torch.isnan(out[10, 1]).all()
+    out[2] = out[10, 1] = 0.0
+    assert torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("hd,vd", [(64, 64), (128, 128), (80, 48), (8, 128)])
 def test_bfloat16_trees_on_the_cuda_cores(ops, hd, vd, monkeypatch):
     monkeypatch.setattr(ops, "USE_MMA_TREE", False)
+    monkeypatch.setattr(ops, "USE_TC_TREE", False)
     Case(BF16, 8, 2, hd, [70, 0, 600, 64], [5, 3, 64, 1], vd=vd, seed=hd).check(ops)
 
 

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import test_prototypes as P
+import test_warp_whole as W
 import tree_plain as T
 
 ops = importlib.import_module("daisi-llogos_b200.kernels.ops")
@@ -25,6 +26,13 @@ def test_the_argument_blocks_are_those_of_the_header():
 def _fields(text, name):
     """As ``test_prototypes`` reads a structure, with array counts that are plain numbers."""
     return P._c_struct(text.replace("void* const* pools", "void* pools"), name, {})
+
+
+def test_the_warp_is_whole_where_tensor_memory_wants_it():
+    with open(os.path.join(P.CSRC, "attention_tree_tc.cu")) as f:
+        found = W.lines_that_want_the_warp(f.read())
+    assert len(found) >= 8, found
+    assert not [x for x in found if not x[2]]
 
 
 def tree_call(**change):
