@@ -14,8 +14,7 @@
 //              weights to bfloat16 does not depend on how the list was cut.
 //   masks      Only tiles that hold nodes, the tree's end or the window's edge look at bits.  In those a value that is not finite must not meet
 //              a weight of zero: a warp that finds one among its keys adds that tile's products up itself, leaving out what a row does not see.
-//   joining    A run that ends inside a (sequence, head, row block) leaves partial rows and takes a ticket; who has the last one joins them
-//              in the runs' order.
+//   joining    A run that ends inside a (sequence, head, row block) leaves partial rows, which a second kernel joins (tree_tiles.cuh).
 //
 // Every wait on an mbarrier is bounded (llg_attn_tree_mma_status).  No load uses cluster multicast.
 #include "tree_tiles.cuh"
@@ -59,8 +58,8 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   unsigned char* Vs = smem + STAGES * TILE_BYTES;
   __shared__ uint64_t full[STAGES], empty[STAGES], work_bar;
   __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1];
-  __shared__ int2 warp_total[THREADS / 32];
-  __shared__ int abort_flag, last_ticket;
+  __shared__ int3 warp_total[THREADS / 32];
+  __shared__ int abort_flag;
   __shared__ int node_depth[LLG_TREE_NODES];
   __shared__ float merge[WK > 1 ? WORK_WARPS : 1][WK > 1 ? 16 : 1][SLICE + 2];
   __shared__ float2 merge_ml[WK > 1 ? WORK_WARPS : 1][16];
@@ -85,11 +84,13 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  plan_units<THREADS>(a, ROWS, sums, row_blocks, warp_total);
+  plan_units<THREADS>(a, ROWS, sums, row_blocks, (int*)nullptr, warp_total, [](int, int, int) { return 0; });
   const int G = a.nh / a.nkv;
   const long long units = (long long)a.nkv * sums[a.n_seqs];
   const long long chunk = (units + gridDim.x - 1) / gridDim.x;
   const long long u0 = (long long)blockIdx.x * chunk, u1 = min(units, u0 + chunk);
+  typedef Place<HDP, ROWS> P;
+  if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
   volatile int* abortp = &abort_flag;
   const int n_units = (int)(u1 - u0);
@@ -325,12 +326,12 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       if (l[r] != l[r] && m[r] == -INFINITY) m[r] = 0.f;             // scores that are no numbers: the row has to show it
     }
     const int rbs = row_blocks[cur.b + 1] - row_blocks[cur.b];
-    const long long pair = (long long)a.nkv * row_blocks[cur.b] + (long long)cur.kvh * rbs + cur.rb;
-    const long long p_first = (long long)a.nkv * sums[cur.b] + ((long long)cur.kvh * rbs + cur.rb) * sh.tiles;   // the pair's first unit
+    const long long p_first = (long long)a.nkv * sums[cur.b] + ((long long)cur.kvh * rbs + cur.rb) * sh.tiles;   // the rows' first unit
     const int blk_first = (int)(p_first / chunk), blk_last = (int)((p_first + sh.tiles - 1) / chunk);
     const bool whole = blk_first == blk_last;
-    constexpr int PW = HDP + PART_PAD;
-    float* mine = a.part + (blockIdx.x + pair) * (long long)(ROWS * PW);
+    const int place = 2 * blockIdx.x + (u > u0);
+    if (!whole && cur.t == 0 && tid == 0)
+      P::notes(a.part, gridDim.x)[blockIdx.x] = Note{blk_last - blk_first + 1, place, n_rows, row0, sh.tok0, cur.kvh, {0, 0}};
     // two neighbouring columns of a row, already the run's own sum: to the output, or to the run's partial rows
     auto emit = [&](int r, int d, float x, float y, float M, float L) {
       if (r >= n_rows) return;
@@ -340,8 +341,8 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         bf16* dst = out + ((long long)(sh.tok0 + node) * a.nh + cur.kvh * G + head) * a.vd + d;
         if (d < a.vd) *reinterpret_cast<uint32_t*>(dst) = pack_bf16(x * inv, y * inv);      // (value sizes are even)
       } else {
-        *reinterpret_cast<float2*>(mine + r * PW + d) = make_float2(x, y);
-        if (d == 0) *reinterpret_cast<float2*>(mine + r * PW + HDP) = make_float2(M, L);
+        reinterpret_cast<float2*>(P::sums(a.part, place) + (d >> 2) * ROWS + r)[(d >> 1) & 1] = make_float2(x, y);
+        if (d == 0) P::ends(a.part, place)[r] = make_float2(M, L);
       }
     };
     if (WK == 1) {
@@ -385,44 +386,7 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         if (!work_sync()) return;
       }
     }
-    if (!whole) {
-      __threadfence();                     // the partial rows are visible to the whole device ...
-      if (!work_sync()) return;
-      if (tid == 0) {
-        const int ticket = atomicAdd(&a.counters[pair], 1);        // ... before the ticket is
-        last_ticket = ticket == blk_last - blk_first;
-        if (last_ticket) a.counters[pair] = 0;
-      }
-      if (!work_sync()) return;
-      if (last_ticket) {
-        __threadfence();
-        // four columns of a row per thread; runs in their order, the largest maximum found on the way (scaling by exact powers of two)
-        for (int x = tid; x < n_rows * (HDP / 4); x += WORK_WARPS * 32) {
-          const int r = x / (HDP / 4), d = (x % (HDP / 4)) * 4;
-          const float* p = a.part + (blk_first + pair) * (long long)(ROWS * PW) + r * PW;
-          float M = -INFINITY, L = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int k = blk_first; k <= blk_last; ++k, p += ROWS * PW) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + HDP));
-            if (ml.x == -INFINITY) continue;
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + d));
-            const float top = fmaxf(M, ml.x), f = M == -INFINITY ? 0.f : pow2_whole(M - top), w = pow2_whole(ml.x - top);
-            M = top;
-            L = L * f + ml.y * w;
-            acc.x = acc.x * f + v.x * w;
-            acc.y = acc.y * f + v.y * w;
-            acc.z = acc.z * f + v.z * w;
-            acc.w = acc.w * f + v.w * w;
-          }
-          const float inv = L != 0.f ? 1.f / L : 0.f;
-          const int node = (row0 + r) / G, head = (row0 + r) - node * G;
-          bf16* dst = out + ((long long)(sh.tok0 + node) * a.nh + cur.kvh * G + head) * a.vd + d;
-          if (d < a.vd) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-        }
-        // (the next segment's writes of last_ticket lie behind further meetings)
-      }
-    }
-    if (!work_sync()) return;              // node_depth, merge and last_ticket are free again
+    if (!work_sync()) return;              // node_depth and merge are free again
     u += n_seg;
   }
 }
@@ -433,7 +397,7 @@ int grid_blocks(int n_seqs, int nkv, int row_blocks, int max_len) {
   const long long resident = (long long)BLOCKS_PER_SM * llg_sm_count();
   const long long units = (long long)n_seqs * nkv * row_blocks * ((max_len + TK - 1) / TK);
   long long rounds = units / (resident * 48);
-  rounds = rounds < 1 ? 1 : (rounds > 4 ? 4 : rounds);
+  rounds = rounds < 1 ? 1 : (rounds > 2 ? 2 : rounds);
   const long long most = resident * rounds;
   return (int)(units < most ? (units < 1 ? 1 : units) : most);
 }
@@ -448,7 +412,13 @@ int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int 
   if (e != cudaSuccess) return llg_fail("attn_tree_mma: shared memory %d: %s", smem, cudaGetErrorString(e));
   e = llg_launch(attn_tree_mma_kernel<HDP, WR, STAGES>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_mma: launch: %s", cudaGetErrorString(e));
-  return llg_check_launch("attn_tree_mma");
+  if (llg_check_launch("attn_tree_mma")) return 1;
+  return launch_join<HDP, 16 * WR>(a, blocks, "attn_tree_mma", stream);
+}
+
+template <int HDP>
+long long scratch_of(int blocks, int wr) {
+  return wr == 1 ? Place<HDP, 16>::floats(blocks) : wr == 2 ? Place<HDP, 32>::floats(blocks) : Place<HDP, 64>::floats(blocks);
 }
 
 }  // namespace
@@ -458,14 +428,10 @@ LLG_API int llg_attn_tree_mma_supported(int hd, int vd, int n_seqs) {
   return hd >= 8 && hd <= 128 && hd % 8 == 0 && vd >= 8 && vd <= 128 && vd % 8 == 0 && n_seqs <= MAX_SEQS;
 }
 
-// Floats of scratch, and counters, of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
+// Floats of scratch of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
 LLG_API long long llg_attn_tree_mma_scratch_floats(int n_seqs, int rows, int nkv, int hd, int vd, int max_len) {
-  const int per = 16 * row_warps(rows), rbs = (rows + per - 1) / per, hdp = hd > 64 || vd > 64 ? 128 : 64;
-  return ((long long)grid_blocks(n_seqs, nkv, rbs, max_len) + (long long)n_seqs * nkv * rbs) * per * (hdp + PART_PAD);
-}
-LLG_API int llg_attn_tree_mma_counters(int n_seqs, int rows, int nkv) {
-  const int per = 16 * row_warps(rows);
-  return n_seqs * nkv * ((rows + per - 1) / per);
+  const int wr = row_warps(rows), per = 16 * wr, blocks = grid_blocks(n_seqs, nkv, (rows + per - 1) / per, max_len);
+  return hd > 64 || vd > 64 ? scratch_of<128>(blocks, wr) : scratch_of<64>(blocks, wr);
 }
 
 LLG_API int llg_attn_tree_mma(const TreeArgs* args, cudaStream_t stream) {

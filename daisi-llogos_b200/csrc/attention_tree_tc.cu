@@ -1,22 +1,23 @@
 // Attention of large trees of drafted tokens over the paged cache on the 5th-generation tensor cores (tcgen05), bfloat16, head sizes 64 and 128.
 // What a node sees is said in cache_args.h, the formula in attention_tree.cu.
 //
-// With more than 64 query rows (nodes x heads of a group) mma.sync is what takes the time, not the cache.  Here a block takes 128 rows, which are
-// the lanes of tensor memory, and two groups of four softmax warps share the keys: the first group takes the even key tiles of the block's
-// run, the second the odd ones, each with scores S[128 x 64] (two buffers) and an accumulator O[128 x head] of its own in tensor memory, a
-// lane that issues its products, and two copying warps for both.  Thread r of a group owns row r, so a row's softmax needs no exchange; a
-// group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of), so a block passes a tile
-// every 1,000, where the memory system brings one every 1,400.
+// With more than 64 query rows (nodes x heads of a group) mma.sync is what takes the time, not the cache.  Here 128 rows are the lanes of tensor
+// memory, and a block's two groups of four softmax warps each have scores S[128 x 64] (two buffers) and an accumulator O[128 x head] of their own
+// there, a lane that issues their products, and two copying warps for both.  Thread r of a group owns row r, so a row's softmax needs no
+// exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of).  A row block has up to
+// 256 rows.  With more than 128 (PLAIN) each group takes half of them and all key tiles: 2,000 cycles a tile.  Otherwise (SPLIT) both groups take
+// the rows and every second tile each: a tile every 1,000 cycles, where the memory system brings one every 1,400.  (Row blocks of 128 alone,
+// all of them SPLIT: every 128 rows read the keys again, sixteen full trees behind up to 8,192 keys 277 us.)
 //
-//   work       The units (sequence, key/value head, 128 rows, key tile) of the batch are one list that blocks, one a multiprocessor, cut into equal
-//              runs (tree_tiles.cuh); a run's keys and values are copied ahead across the ends of its segments.
+//   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
+//              of equal weight, a PLAIN tile 3 and a SPLIT tile 2; a run's keys and values are copied ahead across the ends of its segments.
 //   softmax    As in attention_tc.cu: weights 2^(x - M) with a whole number M that is raised only when a tile's weights add up to more than
 //              2^14, float32 sums, weights rounded to bfloat16 once.
 //   masks      A tile that holds nodes, the tree's end or the window's edge gives every row a 64-bit word of what it sees.  In such a tile a value
 //              that is not finite must not meet a weight of zero: the group looks its values over, and where it finds one adds the tile's products
 //              up itself, in tensor memory, leaving out what a row does not see; the issuing lane then leaves that tile out.
-//   joining    At a segment's end the groups' accumulators are added up; a segment that is not its rows' whole list of keys leaves partial rows
-//              and takes a ticket, and who has the last one joins them in the runs' order.
+//   joining    At a SPLIT segment's end the groups' accumulators are added up; a segment that is not its rows' whole list of keys leaves partial
+//              rows, which a second kernel joins (tree_tiles.cuh).
 //
 // Every wait is bounded (llg_attn_tree_tc_status); every role comes to the block's end, where tensor memory is freed.  No load uses cluster multicast.
 #include "tree_tiles.cuh"
@@ -26,6 +27,8 @@ LLG_API const char* llg_last_error() { return g_llg_error; }
 namespace {
 
 constexpr int BQ = 128;                       // rows of a block: lanes of tensor memory
+constexpr int ROWS = 2 * BQ;                  // of a row block, at most
+constexpr int PLAIN_WEIGHT = 3, SPLIT_WEIGHT = 2;
 constexpr int GROUPS = 2, WORKERS = GROUPS * BQ;
 constexpr int ISSUE_WARP = WORKERS / 32, K_LOAD_WARP = ISSUE_WARP + 1, V_LOAD_WARP = ISSUE_WARP + 2, ISSUE_WARP_2 = ISSUE_WARP + 3;
 constexpr int THREADS = (ISSUE_WARP_2 + 1) * 32;
@@ -98,24 +101,55 @@ __device__ __forceinline__ bool elect_one() {
 // byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a tile of 128-byte rows with the 128-byte swizzle
 __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4)); }
 
-// ST: stages of keys, and of values; even, so that a stage belongs to one group
+// A sequence's share of the list: tiles, row blocks of which the first `plain` have more than 128 rows, and the weight of one head.
+struct Share {
+  int tiles, rbs, plain;
+  long long weight;
+};
+// `weights[b]`: the weight of one head in the sequences before b
+__device__ __forceinline__ Share share_of(const int* sums, const int* blocks, const int* weights, int b) {
+  Share s;
+  s.rbs = blocks[b + 1] - blocks[b];
+  s.tiles = s.rbs > 0 ? (sums[b + 1] - sums[b]) / s.rbs : 0;
+  s.weight = weights[b + 1] - weights[b];
+  // weight = tiles (PLAIN_WEIGHT plain + SPLIT_WEIGHT (rbs - plain)), the weights one apart
+  s.plain = s.tiles > 0 ? (int)(s.weight / s.tiles) - SPLIT_WEIGHT * s.rbs : 0;
+  return s;
+}
+static_assert(PLAIN_WEIGHT == SPLIT_WEIGHT + 1, "share_of");
+
+// The first unit whose weight begins at w or behind it.
+__device__ __forceinline__ long long unit_at(const int* sums, const int* blocks, const int* weights, int n_seqs, int nkv, long long w) {
+  if (w >= (long long)nkv * weights[n_seqs]) return (long long)nkv * sums[n_seqs];
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long long)nkv * weights[mid] <= w) lo = mid;
+    else hi = mid - 1;
+  }
+  const Share s = share_of(sums, blocks, weights, lo);
+  const long long r = w - (long long)nkv * weights[lo], kvh = r / s.weight, in = r - kvh * s.weight, plain = (long long)PLAIN_WEIGHT * s.plain * s.tiles;
+  const long long at = in < plain ? (in + PLAIN_WEIGHT - 1) / PLAIN_WEIGHT : (long long)s.plain * s.tiles + (in - plain + SPLIT_WEIGHT - 1) / SPLIT_WEIGHT;
+  return (long long)nkv * sums[lo] + kvh * s.tiles * s.rbs + at;
+}
+
+// ST: stages of keys, and of values
 template <int HD, int ST>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeArgs a) {
-  static_assert(ST % 2 == 0, "the groups take turns with the tiles: a stage's phases are waited for by one of them");
   constexpr int KB = HD / 64, Q_BYTES = KB * BQ * 128, KV_BYTES = KB * TK * 128, CPR = HD / 8;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* Qs = smem;
-  unsigned char* Ks = Qs + Q_BYTES;                  // [ST]
+  unsigned char* Ks = Qs + GROUPS * Q_BYTES;         // [ST]
   unsigned char* Vs = Ks + ST * KV_BYTES;            // [ST]
   __shared__ uint64_t k_full[ST], k_free[ST], v_full[ST], v_free[ST];
   __shared__ uint64_t s_full[GROUPS][2], p_ready[GROUPS][2], o_done[GROUPS], q_ready[GROUPS], meet_bar, group_bar[GROUPS];
   __shared__ uint32_t tmem_base_slot;
-  __shared__ int abort_flag, last_ticket;
+  __shared__ int abort_flag;
   __shared__ int wild[GROUPS][3], leave_out[GROUPS][2];
   __shared__ float2 share[GROUPS][BQ];               // each group's maximum and sum of a row
-  __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1];
-  __shared__ int2 warp_total[THREADS / 32];
+  __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1], weigh[MAX_SEQS + 1];
+  __shared__ int3 warp_total[THREADS / 32];
 
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -123,19 +157,26 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (tid == 0) atomicCAS(&g_error, 0, 3);
     return;
   }
-  plan_units<THREADS>(a, BQ, sums, row_blocks, warp_total);
   const int G = a.nh / a.nkv;
-  const long long units = (long long)a.nkv * sums[a.n_seqs];
-  const long long chunk = (units + gridDim.x - 1) / gridDim.x;
-  const long long u0 = (long long)blockIdx.x * chunk, u1 = min(units, u0 + chunk);
+  plan_units<THREADS>(a, ROWS, sums, row_blocks, weigh, warp_total, [&](int rows, int rbs, int tiles) {
+    const int split = rbs > 0 && rows - (rbs - 1) * ROWS <= BQ;
+    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split);
+  });
+  // (a run's weight is at least a unit's, so no run between two others is without a unit)
+  const long long weight = (long long)a.nkv * weigh[a.n_seqs];
+  const long long chunk = max((long long)PLAIN_WEIGHT, (weight + gridDim.x - 1) / gridDim.x);
+  const long long u0 = unit_at(sums, row_blocks, weigh, a.n_seqs, a.nkv, blockIdx.x * chunk);
+  const long long u1 = unit_at(sums, row_blocks, weigh, a.n_seqs, a.nkv, (blockIdx.x + 1) * chunk);
+  typedef Place<HD, ROWS> P;
+  if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
   if (u0 >= u1) return;                              // uniform over the block
   const int n_units = (int)(u1 - u0);
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_free[s], 1);
+      mbar_init(&k_free[s], GROUPS);                 // both groups' lanes pass every tile, their own or not
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_free[s], 1);
+      mbar_init(&v_free[s], GROUPS);
     }
     for (int g = 0; g < GROUPS; ++g) {
       mbar_init(&s_full[g][0], 1);
@@ -229,15 +270,14 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           ok = false;
         }
       };
-      // Tile i of the run is the group's tile c = i / 2.  Scores into buffer c % 2, which O += P(c-2) V(c-2) has read by then; a segment's first
-      // tile comes when all of the earlier ones are done, and waits for the last of them (a wait by parity sees one phase back).
-      auto issue_scores = [&](int i, bool first) {
-        const int c = i >> 1;
+      // c: the group's tiles so far.  Scores into buffer c % 2, which O += P(c-2) V(c-2) has read by then; a segment's first tile comes
+      // when all of the earlier ones are done, and waits for the last of them (a wait by parity sees one phase back).
+      auto issue_scores = [&](int i, int c, uint32_t qa, bool first) {
         wait_or_fail(&k_full[i % ST], (i / ST) & 1, 5);
         if (first ? c >= 1 : c >= 2) wait_or_fail(&o_done[g], (first ? c - 1 : c) & 1, 6);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t qa = smem_u32(Qs), ka = smem_u32(Ks + (i % ST) * KV_BYTES);
+        const uint32_t ka = smem_u32(Ks + (i % ST) * KV_BYTES);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           const uint32_t blk = ks >> 2, kk = ks & 3;
@@ -247,23 +287,41 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         umma_commit(&s_full[g][c & 1]);
         umma_commit(&k_free[i % ST]);
       };
-      int i0 = 0;
+      // Tiles of the other group are given back as they arrive, in order: a lane sees every phase of every stage.
+      int k_at = 0, v_at = 0;
+      auto pass = [&](int& at, int to, uint64_t* full, uint64_t* freeb) {
+        for (; at < to && ok; ++at) {
+          wait_or_fail(&full[at % ST], (at / ST) & 1, 5);
+          if (ok) mbar_arrive(&freeb[at % ST]);
+        }
+      };
+      int i0 = 0, c = 0;
       uint32_t segments = 0;                           // of this group: those in which it has a tile
       while (i0 < n_units && ok) {
         const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
-        const int tiles = (sums[cur.b + 1] - sums[cur.b]) / (row_blocks[cur.b + 1] - row_blocks[cur.b]);
-        const int i1 = min(n_units, i0 + tiles - cur.t);
-        int i = i0 + ((i0 ^ g) & 1);
+        const Share sh = share_of(sums, row_blocks, weigh, cur.b);
+        const int i1 = min(n_units, i0 + sh.tiles - cur.t);
+        const bool plain = cur.rb < sh.plain;
+        const int step = plain ? 1 : 2;
+        const uint32_t qa = smem_u32(Qs + (plain ? g * Q_BYTES : 0));
+        int i = i0 + (plain ? 0 : g);
         bool started = false;
         if (i < i1) {
           wait_or_fail(&q_ready[g], segments++ & 1, 5);
-          issue_scores(i, true);
+          pass(k_at, i, k_full, k_free);
+          issue_scores(i, c, qa, true);
+          k_at = i + 1;
         }
-        for (; i < i1 && ok; i += 2) {
-          const int c = i >> 1;
-          if (i + 2 < i1) issue_scores(i + 2, false);
+        for (; i < i1 && ok; i += step, ++c) {
+          if (i + step < i1) {
+            pass(k_at, i + step, k_full, k_free);
+            issue_scores(i + step, c + 1, qa, false);
+            k_at = i + step + 1;
+          }
+          pass(v_at, i, v_full, v_free);
           wait_or_fail(&v_full[i % ST], (i / ST) & 1, 5);
           wait_or_fail(&p_ready[g][c & 1], (c >> 1) & 1, 6);
+          v_at = i + 1;
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (*reinterpret_cast<volatile int*>(&leave_out[g][c & 1])) {
@@ -278,6 +336,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           started = true;
         }
+        pass(k_at, i1, k_full, k_free);
+        pass(v_at, i1, v_full, v_free);
         i0 = i1;
       }
     }
@@ -304,23 +364,27 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       return warp_all(met);
     };
     int looked = 0;                                     // tiles that the group has looked over for values that are not finite
-    int i0 = 0;
+    int i0 = 0, c = 0;                                  // c: the group's tiles so far
     bool ok = true;
     while (i0 < n_units && ok) {
       const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
+      const Share list = share_of(sums, row_blocks, weigh, cur.b);
       const TreeShape sh = tree_shape(a, cur.b);
       const int i1 = min(n_units, i0 + sh.tiles - cur.t);
-      const int row0 = cur.rb * BQ, n_rows = min(BQ, sh.n * G - row0);
-      const bool live = r < n_rows;
-      const int node = live ? (row0 + r) / G : 0, head = live ? cur.kvh * G + (row0 + r) - node * G : 0;
+      const int row0 = cur.rb * ROWS, n_rows = min(ROWS, sh.n * G - row0);
+      const bool plain = cur.rb < list.plain;           // the same for the block
+      const int step = plain ? 1 : 2;
+      const int mine = plain ? g * BQ + r : r;          // this thread's row of the row block
+      const bool live = mine < n_rows;
+      const int node = live ? (row0 + mine) / G : 0, head = live ? cur.kvh * G + (row0 + mine) - node * G : 0;
       // queries: all softmax threads copy; rows behind the last are zeros
       {
         const int ch = tid % CPR;
-        for (int row = tid / CPR; row < BQ; row += WORKERS / CPR) {
+        for (int row = tid / CPR; row < (plain ? ROWS : BQ); row += WORKERS / CPR) {
           const bool valid = row < n_rows;
           const int at = valid ? row0 + row : 0, nd = at / G;
           const bf16* src = (const bf16*)a.q + ((long long)(sh.tok0 + nd) * a.nh + cur.kvh * G + at - nd * G) * HD + ch * 8;
-          cp_async16(smem_u32(Qs) + (uint32_t)((ch >> 3) * (BQ * 128)) + swz(row, ch & 7), src, valid);
+          cp_async16(smem_u32(Qs) + (uint32_t)(row / BQ * Q_BYTES + (ch >> 3) * (BQ * 128)) + swz(row % BQ, ch & 7), src, valid);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       }
@@ -333,14 +397,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       fence_async_smem();
       // each issuing lane is told of the segments in which its group has a tile, and no others: it cannot fall behind by a phase
-      if (i0 + (i0 & 1) < i1) mbar_arrive(&q_ready[0]);
-      if (i0 + ((i0 & 1) ^ 1) < i1) mbar_arrive(&q_ready[1]);
+      mbar_arrive(&q_ready[0]);
+      if (plain || i0 + 1 < i1) mbar_arrive(&q_ready[1]);
 
       float m_run = -INFINITY, l_run = 0.f;
-      const int own0 = i0 + ((i0 ^ g) & 1);
-      for (int i = own0; i < i1; i += 2) {
-        const int c = i >> 1;
-        const bool first = i == own0, last = i + 2 >= i1;
+      const int own0 = i0 + (plain ? 0 : g);
+      for (int i = own0; i < i1; i += step, ++c) {
+        const bool first = i == own0, last = i + step >= i1;
         const bool scored = mbar_wait(&s_full[g][c & 1], (c >> 1) & 1, abortp);
         if (!scored) give_up(1);
         ok = warp_all(scored);
@@ -515,46 +578,50 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       if (!ok) break;                                    // uniform
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      // ---- the segment's result: the groups' accumulators added up, each thread half of its row's columns ------------
+      // ---- the segment's result ---------------------------------------------------------------------------
       if (l_run != l_run && m_run == -INFINITY) m_run = 0.f;       // scores that are no numbers: the row has to show it
-      share[g][r] = make_float2(m_run, l_run);
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      ok = meet();
-      if (!ok) break;                                    // uniform
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const float2 ml0 = share[0][r], ml1 = share[1][r];
-      const float M = fmaxf(ml0.x, ml1.x);
-      float w0 = ml0.x == -INFINITY ? 0.f : pow2_whole(ml0.x - M), w1 = ml1.x == -INFINITY ? 0.f : pow2_whole(ml1.x - M);
-      const float L = ml0.y * w0 + ml1.y * w1;
-      const bool some0 = ml0.x != -INFINITY, some1 = ml1.x != -INFINITY;      // (an accumulator without a tile holds anything)
-      const int rbs = row_blocks[cur.b + 1] - row_blocks[cur.b];
-      const long long pair = (long long)a.nkv * row_blocks[cur.b] + (long long)cur.kvh * rbs + cur.rb;
-      const long long p_first = (long long)a.nkv * sums[cur.b] + ((long long)cur.kvh * rbs + cur.rb) * sh.tiles;
-      const int blk_first = (int)(p_first / chunk), blk_last = (int)((p_first + sh.tiles - 1) / chunk);
+      const long long head_first = (long long)a.nkv * weigh[cur.b] + cur.kvh * list.weight;
+      const long long w_first = head_first + (long long)list.tiles * (plain ? PLAIN_WEIGHT * cur.rb : PLAIN_WEIGHT * list.plain);
+      const int blk_first = (int)(w_first / chunk), blk_last = (int)((w_first + (long long)(list.tiles - 1) * (plain ? PLAIN_WEIGHT : SPLIT_WEIGHT)) / chunk);
       const bool whole = blk_first == blk_last;
-      constexpr int PW = HD + PART_PAD;
-      float* mine = a.part + (blockIdx.x + pair) * (long long)(BQ * PW) + r * PW;
-      bf16* dst = (bf16*)a.out + ((long long)(sh.tok0 + node) * a.nh + head) * HD;
-      if (whole) {
-        const float inv = L != 0.f ? 1.f / L : 0.f;
-        w0 *= inv;
-        w1 *= inv;
-      } else if (g == 0 && live) {
-        *reinterpret_cast<float2*>(mine + HD) = make_float2(M, L);
+      const int place = 2 * blockIdx.x + (i0 > 0);
+      if (!whole && cur.t == 0 && tid == 0)
+        P::notes(a.part, gridDim.x)[blockIdx.x] = Note{blk_last - blk_first + 1, place, n_rows, row0, sh.tok0, cur.kvh, {0, 0}};
+      float M = m_run, L = l_run, w0 = 1.f, w1 = 0.f;
+      bool some0 = m_run != -INFINITY, some1 = false;   // (an accumulator without a tile holds anything)
+      uint32_t from0 = lane_base + O_COL, from1 = 0;
+      if (!plain) {                                     // uniform: the groups meet, and each thread takes half of its row's columns
+        share[g][r] = make_float2(m_run, l_run);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        ok = meet();
+        if (!ok) break;                                 // uniform
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const float2 ml0 = share[0][r], ml1 = share[1][r];
+        M = fmaxf(ml0.x, ml1.x);
+        some0 = ml0.x != -INFINITY;
+        some1 = ml1.x != -INFINITY;
+        w0 = some0 ? pow2_whole(ml0.x - M) : 0.f;
+        w1 = some1 ? pow2_whole(ml1.x - M) : 0.f;
+        L = ml0.y * w0 + ml1.y * w1;
+        from0 = tmem + O_COL + quarter;
+        from1 = from0 + G_COLS;
       }
-      const uint32_t orow = tmem + O_COL + quarter;
+      const float inv = !whole ? 1.f : L != 0.f ? 1.f / L : 0.f;
+      bf16* dst = (bf16*)a.out + ((long long)(sh.tok0 + node) * a.nh + head) * HD;
+      if (!whole && live && (plain || g == 0)) P::ends(a.part, place)[mine] = make_float2(M, L);
 #pragma unroll 1
-      for (int c0 = g * (HD / 2); c0 < (g + 1) * (HD / 2); c0 += 16) {       // uniform
+      for (int c0 = plain ? 0 : g * (HD / 2); c0 < (plain ? HD : (g + 1) * (HD / 2)); c0 += 16) {       // uniform
         uint32_t r0_[16], r1_[16];
         warp_whole();
-        tmem_ld16(orow + c0, r0_);
-        tmem_ld16(orow + G_COLS + c0, r1_);
+        tmem_ld16(from0 + c0, r0_);
+        if (!plain) tmem_ld16(from1 + c0, r1_);          // uniform
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
         float o[16];
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
           o[x] = some0 ? w0 * __uint_as_float(r0_[x]) : 0.f;
-          if (some1) o[x] = fmaf(w1, __uint_as_float(r1_[x]), o[x]);
+          if (!plain && some1) o[x] = fmaf(w1, __uint_as_float(r1_[x]), o[x]);
+          o[x] *= inv;
         }
         if (live && whole) {
           uint4 v0, v1;
@@ -564,51 +631,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           *reinterpret_cast<uint4*>(dst + c0 + 8) = v1;
         } else if (live) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(mine + c0 + 4 * q) = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          for (int q = 0; q < 4; ++q)
+            P::sums(a.part, place)[(c0 / 4 + q) * ROWS + mine] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // the next segment's products overwrite what was read
       __syncwarp();
-      if (!whole) {
-        __threadfence();                                 // the partial rows are visible to the whole device ...
-        ok = meet();
-        if (!ok) break;                                  // uniform
-        if (tid == 0) {
-          const int ticket = atomicAdd(&a.counters[pair], 1);       // ... before the ticket is
-          last_ticket = ticket == blk_last - blk_first;
-          if (last_ticket) a.counters[pair] = 0;
-        }
-        __syncwarp();
-        ok = meet();
-        if (!ok) break;                                  // uniform
-        if (last_ticket) {
-          __threadfence();
-          for (int x = tid; x < n_rows * (HD / 4); x += WORKERS) {
-            const int row = x / (HD / 4), d = (x % (HD / 4)) * 4;
-            const float* p = a.part + (blk_first + pair) * (long long)(BQ * PW) + row * PW;
-            float Mj = -INFINITY, Lj = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = blk_first; k <= blk_last; ++k, p += BQ * PW) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + HD));
-              if (ml.x == -INFINITY) continue;
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(p + d));
-              const float top = fmaxf(Mj, ml.x), f = Mj == -INFINITY ? 0.f : pow2_whole(Mj - top), w = pow2_whole(ml.x - top);
-              Mj = top;
-              Lj = Lj * f + ml.y * w;
-              acc.x = acc.x * f + v.x * w;
-              acc.y = acc.y * f + v.y * w;
-              acc.z = acc.z * f + v.z * w;
-              acc.w = acc.w * f + v.w * w;
-            }
-            const float inv = Lj != 0.f ? 1.f / Lj : 0.f;
-            const int nd = (row0 + row) / G;
-            bf16* to = (bf16*)a.out + ((long long)(sh.tok0 + nd) * a.nh + cur.kvh * G + (row0 + row) - nd * G) * HD + d;
-            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-          }
-        }
-        __syncwarp();
-      }
-      ok = meet();                                       // shares, last_ticket and the queries' place are free again
+      ok = meet();                                       // shares and the queries' place are free again
       i0 = i1;
     }
   }
@@ -628,12 +657,13 @@ int grid_blocks(int n_seqs, int nkv, int row_blocks, int max_len) {
 
 template <int HD, int ST>
 int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t stream) {
-  constexpr int smem = (HD / 64) * (BQ * 128 + 2 * ST * TK * 128);      // more than half a multiprocessor's: tensor memory is a block's alone
+  constexpr int smem = (HD / 64) * (GROUPS * BQ * 128 + 2 * ST * TK * 128);      // more than half a multiprocessor's: tensor memory is a block's alone
   cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: shared memory %d: %s", smem, cudaGetErrorString(e));
   e = llg_launch(attn_tree_tc_kernel<HD, ST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: launch: %s", cudaGetErrorString(e));
-  return llg_check_launch("attn_tree_tc");
+  if (llg_check_launch("attn_tree_tc")) return 1;
+  return launch_join<HD, ROWS>(a, blocks, "attn_tree_tc", stream);
 }
 
 }  // namespace
@@ -641,12 +671,11 @@ int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int 
 // 1 when this kernel takes the geometry (bfloat16 only).
 LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs) { return (hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS; }
 
-// Floats of scratch, and counters, of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
+// Floats of scratch of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
 LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int rows, int nkv, int hd, int max_len) {
-  const int rbs = (rows + BQ - 1) / BQ;
-  return ((long long)grid_blocks(n_seqs, nkv, rbs, max_len) + (long long)n_seqs * nkv * rbs) * BQ * (hd + PART_PAD);
+  const int blocks = grid_blocks(n_seqs, nkv, (rows + ROWS - 1) / ROWS, max_len);
+  return hd == 64 ? Place<64, ROWS>::floats(blocks) : Place<128, ROWS>::floats(blocks);
 }
-LLG_API int llg_attn_tree_tc_counters(int n_seqs, int rows, int nkv) { return n_seqs * nkv * ((rows + BQ - 1) / BQ); }
 
 LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
   const TreeArgs& a = *args;
@@ -657,7 +686,7 @@ LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
   const long long rows = (long long)a.n_pages * a.nkv * TK;
   if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv))
     return llg_fail("attn_tree_tc: cuTensorMapEncodeTiled failed or is not available");
-  const int rbs = (a.max_nodes * (a.nh / a.nkv) + BQ - 1) / BQ, blocks = grid_blocks(a.n_seqs, a.nkv, rbs, a.max_len);
+  const int rbs = (a.max_nodes * (a.nh / a.nkv) + ROWS - 1) / ROWS, blocks = grid_blocks(a.n_seqs, a.nkv, rbs, a.max_len);
   return a.hd == 64 ? launch<64, 8>(a, mk, mv, blocks, stream) : launch<128, 4>(a, mk, mv, blocks, stream);
 }
 

@@ -13,7 +13,6 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int TK = 64;                       // keys per tile = one cache page
 constexpr int MAX_SEQS = 1024;               // sequences whose work fits the plan in shared memory
-constexpr int PART_PAD = 4;                  // a partial row is its sums, the maximum, the sum of weights, and 2 unused: rows stay 16-byte aligned
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -120,45 +119,144 @@ __device__ __forceinline__ Unit locate(const int* sums, const int* blocks, int n
   return c;
 }
 
-// All threads of a block: sums[] and blocks[] for row blocks of `rows` query rows.  `warp_total`: two numbers per warp.
-template <int THREADS>
-__device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, int* sums, int* blocks, int2* warp_total) {
+// All threads of a block: sums[], blocks[] and weights[] (what `weight(rows, row blocks, tiles)` gives a head, in the sequences before b) for row
+// blocks of `rows` query rows.
+template <int THREADS, typename Weight>
+__device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, int* sums, int* blocks, int* weights, int3* warp_total, Weight weight) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.nh / a.nkv;
   const int per = (a.n_seqs + THREADS - 1) / THREADS;
   const int b0 = tid * per, b1 = min(a.n_seqs, b0 + per);
-  int units = 0, rbs = 0;
+  int units = 0, rbs = 0, ws = 0;
   for (int b = b0; b < b1; ++b) {
     const TreeShape s = tree_shape(a, b);
     const int r = (s.n * G + rows - 1) / rows;
     units += r * s.tiles;
     rbs += r;
+    ws += weight(s.n * G, r, s.tiles);
   }
-  int iu = units, ir = rbs;
+  int iu = units, ir = rbs, iw = ws;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int pu = __shfl_up_sync(0xffffffffu, iu, o), pr = __shfl_up_sync(0xffffffffu, ir, o);
+    const int pu = __shfl_up_sync(0xffffffffu, iu, o), pr = __shfl_up_sync(0xffffffffu, ir, o), pw = __shfl_up_sync(0xffffffffu, iw, o);
     if (lane >= o) {
       iu += pu;
       ir += pr;
+      iw += pw;
     }
   }
-  if (lane == 31) warp_total[warp] = make_int2(iu, ir);
+  if (lane == 31) warp_total[warp] = make_int3(iu, ir, iw);
   __syncthreads();
-  int su = iu - units, sr = ir - rbs;
+  int su = iu - units, sr = ir - rbs, sw = iw - ws;
   for (int w = 0; w < warp; ++w) {
     su += warp_total[w].x;
     sr += warp_total[w].y;
+    sw += warp_total[w].z;
   }
-  if (tid == 0) sums[0] = blocks[0] = 0;
+  if (tid == 0) {
+    sums[0] = blocks[0] = 0;
+    if (weights) weights[0] = 0;
+  }
   for (int b = b0; b < b1; ++b) {
     const TreeShape s = tree_shape(a, b);
     const int r = (s.n * G + rows - 1) / rows;
     su += r * s.tiles;
     sr += r;
+    sw += weight(s.n * G, r, s.tiles);
     sums[b + 1] = su;
     blocks[b + 1] = sr;
+    if (weights) weights[b + 1] = sw;
   }
   __syncthreads();
+}
+
+// ---- joining runs that share rows -----------------------------------------------------------------------
+//
+// A run that ends inside a (sequence, head, row block), or begins inside one, leaves that segment as partial rows.  Only a run's first and last
+// segment can be such, so a block has two places for them: one for a segment that begins the run, one for a segment that ends it and does
+// not begin it.  A place holds the sums column by column ([HDP / 4][ROWS] of four columns each, so that threads with neighbouring rows write and
+// read neighbouring addresses), then every row's maximum and sum of weights.  Every block leaves one note: the segment that it begins and that
+// others go on with, if there is one.  A second kernel, a thread per row and 16 columns, joins what a note tells of in the runs' order.  (Joined by
+// the block that finished last, eight trees behind 8,190 keys took 12 us longer: one multiprocessor then read all of a pair's partial rows.)
+struct Note {
+  int parts, place, n_rows, row0, tok0, kvh, pad[2];      // parts 0: nothing; place: the first part's; the others lie at the beginning of their blocks' runs
+};
+
+template <int HDP, int ROWS>
+struct Place {
+  static constexpr long long FLOATS = (long long)ROWS * (HDP + 2);
+  __device__ static float4* sums(float* part, int place) { return reinterpret_cast<float4*>(part + place * FLOATS); }
+  __device__ static float2* ends(float* part, int place) { return reinterpret_cast<float2*>(part + place * FLOATS + (long long)ROWS * HDP); }
+  __host__ __device__ static long long floats(int blocks) { return 2 * blocks * FLOATS + blocks * (long long)(sizeof(Note) / 4); }
+  __device__ static Note* notes(float* part, int blocks) { return reinterpret_cast<Note*>(part + 2 * blocks * FLOATS); }
+};
+
+constexpr int JOIN_THREADS = 128, JOIN_COLS = 16;
+
+template <int HDP, int ROWS>
+__global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(TreeArgs a, int blocks) {
+  typedef Place<HDP, ROWS> P;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Note n = P::notes(a.part, blocks)[blockIdx.x];
+  if (n.parts <= 1) return;
+  const int item = blockIdx.y * JOIN_THREADS + threadIdx.x, row = item % ROWS, d0 = item / ROWS * JOIN_COLS;
+  if (row >= n.n_rows || d0 >= a.vd) return;
+  float M = -INFINITY, L = 0.f;
+  float4 acc[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int DEEP = 4;                                 // parts asked for at once
+  for (int k0 = 0; k0 < n.parts; k0 += DEEP) {
+    float2 ml[DEEP];
+    float4 v[DEEP][4];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+      const bool there = k0 + k < n.parts;
+      const int place = k0 + k == 0 ? n.place : 2 * (n.place / 2 + k0 + k);
+      ml[k] = there ? __ldcg(P::ends(a.part, place) + row) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        v[k][q] = there ? __ldcg(P::sums(a.part, place) + (d0 / 4 + q) * ROWS + row) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float top = M;
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) top = fmaxf(top, ml[k].x);
+    const float f = M == -INFINITY ? 0.f : pow2_whole(M - top);
+    M = top;
+    L *= f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { acc[q].x *= f; acc[q].y *= f; acc[q].z *= f; acc[q].w *= f; }
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+      if (ml[k].x == -INFINITY) continue;                 // a part in which the row sees nothing
+      const float w = pow2_whole(ml[k].x - M);
+      L += w * ml[k].y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        acc[q].x += w * v[k][q].x;
+        acc[q].y += w * v[k][q].y;
+        acc[q].z += w * v[k][q].z;
+        acc[q].w += w * v[k][q].w;
+      }
+    }
+  }
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  const int G = a.nh / a.nkv, node = (n.row0 + row) / G, head = n.kvh * G + (n.row0 + row) - node * G;
+  bf16* dst = (bf16*)a.out + ((long long)(n.tok0 + node) * a.nh + head) * a.vd + d0;
+#pragma unroll
+  for (int q = 0; q < 4; q += 2) {
+    if (d0 + 4 * q < a.vd)                                // (value sizes are multiples of 8)
+      *reinterpret_cast<uint4*>(dst + 4 * q) = make_uint4(pack_bf16(acc[q].x * inv, acc[q].y * inv), pack_bf16(acc[q].z * inv, acc[q].w * inv),
+                                                          pack_bf16(acc[q + 1].x * inv, acc[q + 1].y * inv), pack_bf16(acc[q + 1].z * inv, acc[q + 1].w * inv));
+  }
+}
+
+template <int HDP, int ROWS>
+inline int launch_join(const TreeArgs& a, int blocks, const char* what, cudaStream_t stream) {
+  cudaError_t e = llg_launch(tree_join_kernel<HDP, ROWS>, dim3(blocks, (ROWS * (HDP / JOIN_COLS) + JOIN_THREADS - 1) / JOIN_THREADS), dim3(JOIN_THREADS), 0,
+                             stream, a, blocks);
+  if (e != cudaSuccess) return llg_fail("%s: launch: %s", what, cudaGetErrorString(e));
+  return llg_check_launch(what);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -197,7 +295,7 @@ inline int check_tree(const TreeArgs& a, const char* what) {
   LLG_REQUIRE(a.n_seqs <= MAX_SEQS, "%s: %d sequences (at most %d)", what, a.n_seqs, MAX_SEQS);
   LLG_REQUIRE(a.window >= 0 && a.ring_pages > 0 && a.table_width >= a.ring_pages, "%s: bad cache geometry", what);
   LLG_REQUIRE(a.scale > 0.f, "%s: the softmax scale must be positive", what);
-  LLG_REQUIRE(a.part && a.counters && a.max_len > 0 && a.n_pages > 0, "%s: needs scratch, counters, a bound on the lengths and pages", what);
+  LLG_REQUIRE(a.part && a.max_len > 0 && a.n_pages > 0, "%s: needs scratch, a bound on the lengths and pages", what);
   LLG_REQUIRE((uintptr_t)a.k_pages % 16 == 0 && (uintptr_t)a.v_pages % 16 == 0 && (uintptr_t)a.q % 16 == 0, "%s: storage must be 16-byte aligned", what);
   LLG_REQUIRE((long long)a.n_pages * a.nkv * TK < 2147483647LL, "%s: too many page rows for a tensor map coordinate", what);
   return 0;

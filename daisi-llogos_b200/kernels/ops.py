@@ -568,14 +568,12 @@ def _load_lib(name: str):
         lib.llg_attn_tree_mma_supported.argtypes = [c_int, c_int, c_int]
         lib.llg_attn_tree_mma_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_mma_scratch_floats.restype = c_longlong
-        lib.llg_attn_tree_mma_counters.argtypes = [c_int, c_int, c_int]
         lib.llg_attn_tree_mma_status.restype = c_int
     elif name == "attention_tree_tc":
         lib.llg_attn_tree_tc.argtypes = [POINTER(_TreeArgs), c_void_p]
         lib.llg_attn_tree_tc_supported.argtypes = [c_int, c_int, c_int]
         lib.llg_attn_tree_tc_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_tc_scratch_floats.restype = c_longlong
-        lib.llg_attn_tree_tc_counters.argtypes = [c_int, c_int, c_int]
         lib.llg_attn_tree_tc_status.restype = c_int
     elif name == "key_weights":
         lib.llg_key_weights_simt.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
@@ -2448,13 +2446,12 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
     if USE_TC_TREE and dtype == torch.bfloat16 and rows > TREE_MMA_ROWS:
         lib = _lib("attention_tree_tc")
         if lib.llg_attn_tree_tc_supported(head_dim, vd, n_seqs):
-            return TreePlan("tc", key, 1, max_nodes, max_len, lib.llg_attn_tree_tc_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, max_len),
-                            lib.llg_attn_tree_tc_counters(n_seqs, rows, n_kv_heads))
+            return TreePlan("tc", key, 1, max_nodes, max_len, lib.llg_attn_tree_tc_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, max_len), 0)
     if USE_MMA_TREE and dtype == torch.bfloat16:
         lib = _lib("attention_tree_mma")
         if lib.llg_attn_tree_mma_supported(head_dim, vd, n_seqs):
             return TreePlan("mma", key, 1, max_nodes, max_len, lib.llg_attn_tree_mma_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, vd, max_len),
-                            lib.llg_attn_tree_mma_counters(n_seqs, rows, n_kv_heads))
+                            0)
     lib = _lib("attention_tree")
     per = lib.llg_attn_tree_rows(rows)
     blocks = n_seqs * n_kv_heads * -(-rows // per)
@@ -2511,10 +2508,10 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     a.scale, a.window = float(scale), int(window)
     if plan.kind == "tc":
         lib = _lib("attention_tree_tc")
-        _check(lib, lib.llg_attn_tree_tc(byref(a), _stream()))
+        _check(lib, lib.llg_attn_tree_tc(byref(a), _stream()), kernels=2)
     elif plan.kind == "mma":
         lib = _lib("attention_tree_mma")
-        _check(lib, lib.llg_attn_tree_mma(byref(a), _stream()))
+        _check(lib, lib.llg_attn_tree_mma(byref(a), _stream()), kernels=2)
     else:
         lib = _lib("attention_tree")
         _check(lib, lib.llg_attn_tree_simt(byref(a), _dt(q), _stream()))
