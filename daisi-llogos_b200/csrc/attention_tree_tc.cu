@@ -4,13 +4,15 @@
 // With more than 64 query rows (nodes x heads of a group) mma.sync is what takes the time, not the cache.  Here 128 rows are the lanes of tensor
 // memory, and a block's two groups of four softmax warps each have scores S[128 x 64] (two buffers) and an accumulator O[128 x head] of their own
 // there, a lane that issues their products, and two copying warps for both.  Thread r of a group owns row r, so a row's softmax needs no
-// exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of).  A row block has up to
-// 256 rows.  With more than 128 (PLAIN) each group takes half of them and all key tiles: 2,000 cycles a tile.  Otherwise (SPLIT) both groups take
-// the rows and every second tile each: a tile every 1,000 cycles, where the memory system brings one every 1,400.  (Row blocks of 128 alone,
-// all of them SPLIT: every 128 rows read the keys again, sixteen full trees behind up to 8,192 keys 277 us.)
+// exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of).  A tile of queries is as
+// many whole nodes as 128 rows hold, so that one TMA box of [nodes][heads of the group] brings it; a row block is one or two of them.  Two (PLAIN):
+// each group takes one, and all key tiles: 2,000 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one
+// every 1,000 cycles, where the memory system brings one every 1,400.  (Row blocks of 128 alone, all of them SPLIT: every 128 rows read
+// the keys again, sixteen full trees behind up to 8,192 keys 277 us.)
 //
 //   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
-//              of equal weight, a PLAIN tile 3 and a SPLIT tile 2; a run's keys and values are copied ahead across the ends of its segments.
+//              of equal weight, a PLAIN tile 3, a SPLIT tile 2 and a row block's end SEGMENT_WEIGHT; keys, values and queries of a run's next segment are
+//              copied while the last one ends.
 //   softmax    As in attention_tc.cu: weights 2^(x - M) with a whole number M that is raised only when a tile's weights add up to more than
 //              2^14, float32 sums, weights rounded to bfloat16 once.
 //   masks      A tile that holds nodes, the tree's end or the window's edge gives every row a 64-bit word of what it sees.  In such a tile a value
@@ -28,7 +30,7 @@ namespace {
 
 constexpr int BQ = 128;                       // rows of a block: lanes of tensor memory
 constexpr int ROWS = 2 * BQ;                  // of a row block, at most
-constexpr int PLAIN_WEIGHT = 3, SPLIT_WEIGHT = 2;
+constexpr int PLAIN_WEIGHT = 3, SPLIT_WEIGHT = 2, SEGMENT_WEIGHT = 6;
 constexpr int GROUPS = 2, WORKERS = GROUPS * BQ;
 constexpr int ISSUE_WARP = WORKERS / 32, K_LOAD_WARP = ISSUE_WARP + 1, V_LOAD_WARP = ISSUE_WARP + 2, ISSUE_WARP_2 = ISSUE_WARP + 3;
 constexpr int THREADS = (ISSUE_WARP_2 + 1) * 32;
@@ -38,11 +40,12 @@ constexpr uint32_t G_COLS = 256, O_COL = 128;       // a group's columns: S 2 x 
 // 0 ok; waits that ran out: 1 scores, 2 accumulator, 4 free stage, 5 tile or queries copied, 6 weights, 7 copies at the end, 8 a meeting; 3 shared memory not aligned
 __device__ int g_error = 0;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -112,8 +115,8 @@ __device__ __forceinline__ Share share_of(const int* sums, const int* blocks, co
   s.rbs = blocks[b + 1] - blocks[b];
   s.tiles = s.rbs > 0 ? (sums[b + 1] - sums[b]) / s.rbs : 0;
   s.weight = weights[b + 1] - weights[b];
-  // weight = tiles (PLAIN_WEIGHT plain + SPLIT_WEIGHT (rbs - plain)), the weights one apart
-  s.plain = s.tiles > 0 ? (int)(s.weight / s.tiles) - SPLIT_WEIGHT * s.rbs : 0;
+  // weight = tiles (PLAIN_WEIGHT plain + SPLIT_WEIGHT (rbs - plain)) + SEGMENT_WEIGHT rbs, the first two one apart
+  s.plain = s.tiles > 0 ? (int)((s.weight - SEGMENT_WEIGHT * s.rbs) / s.tiles) - SPLIT_WEIGHT * s.rbs : 0;
   return s;
 }
 static_assert(PLAIN_WEIGHT == SPLIT_WEIGHT + 1, "share_of");
@@ -128,22 +131,27 @@ __device__ __forceinline__ long long unit_at(const int* sums, const int* blocks,
     else hi = mid - 1;
   }
   const Share s = share_of(sums, blocks, weights, lo);
-  const long long r = w - (long long)nkv * weights[lo], kvh = r / s.weight, in = r - kvh * s.weight, plain = (long long)PLAIN_WEIGHT * s.plain * s.tiles;
-  const long long at = in < plain ? (in + PLAIN_WEIGHT - 1) / PLAIN_WEIGHT : (long long)s.plain * s.tiles + (in - plain + SPLIT_WEIGHT - 1) / SPLIT_WEIGHT;
-  return (long long)nkv * sums[lo] + kvh * s.tiles * s.rbs + at;
+  const long long r = w - (long long)nkv * weights[lo], kvh = r / s.weight, in = r - kvh * s.weight;
+  const long long block = (long long)PLAIN_WEIGHT * s.tiles + SEGMENT_WEIGHT, rb = min(in / block, (long long)s.plain), x = in - rb * block;
+  const int each = rb < s.plain ? PLAIN_WEIGHT : SPLIT_WEIGHT;
+  // (a row block's last SEGMENT_WEIGHT begins no unit)
+  return (long long)nkv * sums[lo] + kvh * s.tiles * s.rbs + rb * s.tiles + min((long long)s.tiles, (x + each - 1) / each);
 }
 
 // ST: stages of keys, and of values
 template <int HD, int ST>
 __global__ void __launch_bounds__(THREADS, 1)
-attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, TreeArgs a) {
-  constexpr int KB = HD / 64, Q_BYTES = KB * BQ * 128, KV_BYTES = KB * TK * 128, CPR = HD / 8;
+attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                    TreeArgs a) {
+  static_assert(ST % 2 == 0, "where the groups take turns with the tiles, a stage belongs to one of them: a wait for its next phase by parity means "
+                "something only to who has seen the last one");
+  constexpr int KB = HD / 64, Q_BYTES = KB * BQ * 128, KV_BYTES = KB * TK * 128;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* Qs = smem;
   unsigned char* Ks = Qs + GROUPS * Q_BYTES;         // [ST]
   unsigned char* Vs = Ks + ST * KV_BYTES;            // [ST]
   __shared__ uint64_t k_full[ST], k_free[ST], v_full[ST], v_free[ST];
-  __shared__ uint64_t s_full[GROUPS][2], p_ready[GROUPS][2], o_done[GROUPS], q_ready[GROUPS], meet_bar, group_bar[GROUPS];
+  __shared__ uint64_t s_full[GROUPS][2], p_ready[GROUPS][2], o_done[GROUPS], q_full, q_free, meet_bar, group_bar[GROUPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
   __shared__ int wild[GROUPS][3], leave_out[GROUPS][2];
@@ -157,10 +165,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (tid == 0) atomicCAS(&g_error, 0, 3);
     return;
   }
-  const int G = a.nh / a.nkv;
-  plan_units<THREADS>(a, ROWS, sums, row_blocks, weigh, warp_total, [&](int rows, int rbs, int tiles) {
-    const int split = rbs > 0 && rows - (rbs - 1) * ROWS <= BQ;
-    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split);
+  const int G = a.nh / a.nkv, tile_nodes = BQ / G, tile_rows = tile_nodes * G, block_rows = GROUPS * tile_rows;
+  plan_units<THREADS>(a, block_rows, sums, row_blocks, weigh, warp_total, [&](int rows, int rbs, int tiles) {
+    const int split = rbs > 0 && rows - (rbs - 1) * block_rows <= tile_rows;
+    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split) + SEGMENT_WEIGHT * rbs;
   });
   // (a run's weight is at least a unit's, so no run between two others is without a unit)
   const long long weight = (long long)a.nkv * weigh[a.n_seqs];
@@ -174,7 +182,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   if (tid == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_free[s], GROUPS);                 // both groups' lanes pass every tile, their own or not
+      mbar_init(&k_free[s], GROUPS);                 // (one group's lane alone arrives for both)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_free[s], GROUPS);
     }
@@ -185,10 +193,11 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       mbar_init(&p_ready[g][1], BQ / 32);
       mbar_init(&o_done[g], 1);
       mbar_init(&group_bar[g], BQ);
-      mbar_init(&q_ready[g], WORKERS);
       wild[g][0] = wild[g][1] = wild[g][2] = 0;
       leave_out[g][0] = leave_out[g][1] = 0;
     }
+    mbar_init(&q_full, 1);
+    mbar_init(&q_free, GROUPS);
     mbar_init(&meet_bar, WORKERS);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -219,22 +228,44 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint64_t* freeb = keys ? k_free : v_free;
     const CUtensorMap* map = keys ? &map_k : &map_v;
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-    int issued = 0;
+    // The values' warp brings each segment's queries too, ahead of its first values, when all of the last segment's scores are there.
+    int issued = 0, segments = 0;
     bool fine = true;
     for (int first = 0; first < n_units && fine; first += 32) {
       const int idx = first + lane;
-      int row = 0;
+      int row = 0, q_tok = 0, q_head = 0, q_tiles = 0;        // q_tiles: of queries, where a segment begins
       if (idx < n_units) {
         const Unit c = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + idx);
-        const int tile = tree_shape(a, c.b).t_first + c.t;
+        const TreeShape sh = tree_shape(a, c.b);
+        const int tile = sh.t_first + c.t;
+        if (!keys && (idx == 0 || c.t == 0)) {
+          q_tok = sh.tok0 + c.rb * GROUPS * tile_nodes;
+          q_head = c.kvh * G;
+          q_tiles = sh.n - c.rb * GROUPS * tile_nodes > tile_nodes ? 2 : 1;
+        }
         const int page = a.page_table[(long long)a.slots[c.b] * a.table_width + tile % a.ring_pages];
         row = (page * a.nkv + c.kvh) * TK;
       }
       const int n_here = min(32, n_units - first);
       for (int k = 0; k < n_here && fine; ++k) {
+        int sent = 0;
         if (lane == k) {
           const int i = first + k, st = i % ST;
-          if (i >= ST && !mbar_wait(&freeb[st], (i / ST - 1) & 1, abortp)) {
+          if (q_tiles > 0) {
+            if (segments > 0 && !mbar_wait(&q_free, (segments - 1) & 1, abortp)) {
+              give_up(4);
+              fine = false;
+            } else {
+              mbar_expect_tx(&q_full, q_tiles * KB * tile_rows * 128);
+              for (int t = 0; t < q_tiles; ++t)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+                  tma_load_3d(smem_u32(Qs + t * Q_BYTES + kb * (BQ * 128)), &map_q, kb * 64, q_head, q_tok + t * tile_nodes, &q_full);
+              sent = 1;
+            }
+          }
+          if (!fine) {
+          } else if (i >= ST && !mbar_wait(&freeb[st], (i / ST - 1) & 1, abortp)) {
             give_up(4);
             fine = false;
           } else {
@@ -244,6 +275,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         }
         fine = __shfl_sync(0xffffffffu, (int)fine, k) != 0;
+        segments += __shfl_sync(0xffffffffu, sent, k);
         if (fine) ++issued;
       }
     }
@@ -252,6 +284,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int i = max(0, issued - ST); i < issued; ++i) {
         const unsigned long long t0 = now_ns();
         while (!mbar_try_wait(&full[i % ST], (i / ST) & 1)) {
+          if (now_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(&g_error, 0, 7); break; }
+        }
+      }
+      if (segments > 0) {
+        const unsigned long long t0 = now_ns();
+        while (!mbar_try_wait(&q_full, (segments - 1) & 1)) {
           if (now_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(&g_error, 0, 7); break; }
         }
       }
@@ -272,7 +310,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       };
       // c: the group's tiles so far.  Scores into buffer c % 2, which O += P(c-2) V(c-2) has read by then; a segment's first tile comes
       // when all of the earlier ones are done, and waits for the last of them (a wait by parity sees one phase back).
-      auto issue_scores = [&](int i, int c, uint32_t qa, bool first) {
+      auto issue_scores = [&](int i, int c, uint32_t qa, bool first, bool plain) {
         wait_or_fail(&k_full[i % ST], (i / ST) & 1, 5);
         if (first ? c >= 1 : c >= 2) wait_or_fail(&o_done[g], (first ? c - 1 : c) & 1, 6);
         if (!ok) return;
@@ -286,18 +324,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         umma_commit(&s_full[g][c & 1]);
         umma_commit(&k_free[i % ST]);
-      };
-      // Tiles of the other group are given back as they arrive, in order: a lane sees every phase of every stage.
-      int k_at = 0, v_at = 0;
-      auto pass = [&](int& at, int to, uint64_t* full, uint64_t* freeb) {
-        for (; at < to && ok; ++at) {
-          wait_or_fail(&full[at % ST], (at / ST) & 1, 5);
-          if (ok) mbar_arrive(&freeb[at % ST]);
-        }
+        if (!plain) umma_commit(&k_free[i % ST]);
       };
       int i0 = 0, c = 0;
-      uint32_t segments = 0;                           // of this group: those in which it has a tile
-      while (i0 < n_units && ok) {
+      for (int seg = 0; i0 < n_units && ok; ++seg) {
         const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
         const Share sh = share_of(sums, row_blocks, weigh, cur.b);
         const int i1 = min(n_units, i0 + sh.tiles - cur.t);
@@ -306,22 +336,21 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const uint32_t qa = smem_u32(Qs + (plain ? g * Q_BYTES : 0));
         int i = i0 + (plain ? 0 : g);
         bool started = false;
-        if (i < i1) {
-          wait_or_fail(&q_ready[g], segments++ & 1, 5);
-          pass(k_at, i, k_full, k_free);
-          issue_scores(i, c, qa, true);
-          k_at = i + 1;
-        }
+        // Both lanes wait for every segment's queries and both give them back, with tiles or without: neither falls behind by a phase, and who
+        // has seen the queries knows that the keys of all earlier segments were used.
+        wait_or_fail(&q_full, seg & 1, 5);
+        if (i < i1) issue_scores(i, c, qa, true, plain);
+        if (ok && i + step >= i1) umma_commit(&q_free);
         for (; i < i1 && ok; i += step, ++c) {
           if (i + step < i1) {
-            pass(k_at, i + step, k_full, k_free);
-            issue_scores(i + step, c + 1, qa, false);
-            k_at = i + step + 1;
+            issue_scores(i + step, c + 1, qa, false, plain);
+            if (ok && i + 2 * step >= i1) umma_commit(&q_free);
           }
-          pass(v_at, i, v_full, v_free);
-          wait_or_fail(&v_full[i % ST], (i / ST) & 1, 5);
+          // (weights first: behind them lie the meetings of earlier segments, so all of their values were used)
           wait_or_fail(&p_ready[g][c & 1], (c >> 1) & 1, 6);
-          v_at = i + 1;
+          wait_or_fail(&v_full[i % ST], (i / ST) & 1, 5);
+          // (the last tile's product is waited for at the next segment's begin: the one ahead of it has to be done while that can be told)
+          if (c >= 1 && i + step >= i1) wait_or_fail(&o_done[g], (c - 1) & 1, 6);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           if (*reinterpret_cast<volatile int*>(&leave_out[g][c & 1])) {
@@ -333,11 +362,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
               umma_bf16_ts(tmem + g * G_COLS + O_COL, pa + kk * 8, desc_mnmajor(va + kk * 2048, TK * 128), IDESC_O, started || kk != 0);
             umma_commit(&o_done[g]);
             umma_commit(&v_free[i % ST]);
+            if (!plain) umma_commit(&v_free[i % ST]);
           }
           started = true;
         }
-        pass(k_at, i1, k_full, k_free);
-        pass(v_at, i1, v_full, v_free);
         i0 = i1;
       }
     }
@@ -366,40 +394,44 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     int looked = 0;                                     // tiles that the group has looked over for values that are not finite
     int i0 = 0, c = 0;                                  // c: the group's tiles so far
     bool ok = true;
+    // What a thread knows of a segment; the next one's is asked for before the last one ends.
+    struct Segment {
+      Unit at;
+      TreeShape sh;
+      Share list;
+      bool plain, live;
+      int row0, n_rows, mine, node, depth;
+      unsigned long long bits;
+    };
+    auto segment_at = [&](int i) -> Segment {
+      Segment x;
+      x.at = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i);
+      x.list = share_of(sums, row_blocks, weigh, x.at.b);
+      x.sh = tree_shape(a, x.at.b);
+      x.plain = x.at.rb < x.list.plain;                 // the same for the block
+      x.row0 = x.at.rb * block_rows;
+      x.n_rows = min(block_rows, x.sh.n * G - x.row0);
+      x.mine = x.plain ? g * tile_rows + r : r;         // this thread's row of the row block
+      x.live = r < tile_rows && x.mine < x.n_rows;
+      x.node = x.live ? (x.row0 + x.mine) / G : 0;
+      x.bits = x.live ? (unsigned long long)a.ancestors[x.sh.tok0 + x.node] : 0ull;
+      x.depth = __popcll(x.bits) - 1;
+      return x;
+    };
+    Segment next = segment_at(0);
     while (i0 < n_units && ok) {
-      const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
-      const Share list = share_of(sums, row_blocks, weigh, cur.b);
-      const TreeShape sh = tree_shape(a, cur.b);
-      const int i1 = min(n_units, i0 + sh.tiles - cur.t);
-      const int row0 = cur.rb * ROWS, n_rows = min(ROWS, sh.n * G - row0);
-      const bool plain = cur.rb < list.plain;           // the same for the block
-      const int step = plain ? 1 : 2;
-      const int mine = plain ? g * BQ + r : r;          // this thread's row of the row block
-      const bool live = mine < n_rows;
-      const int node = live ? (row0 + mine) / G : 0, head = live ? cur.kvh * G + (row0 + mine) - node * G : 0;
-      // queries: all softmax threads copy; rows behind the last are zeros
-      {
-        const int ch = tid % CPR;
-        for (int row = tid / CPR; row < (plain ? ROWS : BQ); row += WORKERS / CPR) {
-          const bool valid = row < n_rows;
-          const int at = valid ? row0 + row : 0, nd = at / G;
-          const bf16* src = (const bf16*)a.q + ((long long)(sh.tok0 + nd) * a.nh + cur.kvh * G + at - nd * G) * HD + ch * 8;
-          cp_async16(smem_u32(Qs) + (uint32_t)(row / BQ * Q_BYTES + (ch >> 3) * (BQ * 128)) + swz(row % BQ, ch & 7), src, valid);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-      unsigned long long bits = live ? (unsigned long long)a.ancestors[sh.tok0 + node] : 0ull;
-      const int depth = __popcll(bits) - 1;
+      const Unit cur = next.at;
+      const TreeShape sh = next.sh;
+      const Share list = next.list;
+      const bool plain = next.plain, live = next.live;
+      const int row0 = next.row0, n_rows = next.n_rows, mine = next.mine, node = next.node, depth = next.depth;
+      const int head = cur.kvh * G + row0 + mine - node * G;
+      const int i1 = min(n_units, i0 + sh.tiles - cur.t), step = plain ? 1 : 2;
+      unsigned long long bits = next.bits;
       bits &= sh.n >= 64 ? ~0ull : (1ull << sh.n) - 1;
       if (a.window > 0 && depth >= a.window)            // of its ancestors, those less than a window above it
         for (int j = 0; j < sh.n; ++j)
           if (((bits >> j) & 1) && depth - (__popcll(a.ancestors[sh.tok0 + j]) - 1) >= a.window) bits &= ~(1ull << j);
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      fence_async_smem();
-      // each issuing lane is told of the segments in which its group has a tile, and no others: it cannot fall behind by a phase
-      mbar_arrive(&q_ready[0]);
-      if (plain || i0 + 1 < i1) mbar_arrive(&q_ready[1]);
-
       float m_run = -INFINITY, l_run = 0.f;
       const int own0 = i0 + (plain ? 0 : g);
       for (int i = own0; i < i1; i += step, ++c) {
@@ -489,12 +521,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             const float mxs = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
             const float m_new = fits ? m_run : fmaxf(m_run, ceilf(mxs));
-            corr = m_new == m_run || m_new == -INFINITY ? 1.f : pow2_whole(m_run - m_new);
+            corr = m_new == m_run || m_new == -INFINITY || !live ? 1.f : pow2_whole(m_run - m_new);
             m_run = m_new;
             rescale = !warp_all(corr == 1.f);
           }
           weights(m_run);
-          fits = m_run != -INFINITY && psum <= sum_bound;
+          fits = !live || (m_run != -INFINITY && psum <= sum_bound);      // (a row that is none holds whatever lay in shared memory)
           if (pass == 1 || warp_all(fits)) break;        // uniform
         }
         l_run = l_run * corr + psum;
@@ -561,7 +593,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (by_hand) {
             ok = group_meet();                           // all of the group have read the values
             if (!ok) break;                              // uniform
-            if (r == 0) mbar_arrive(&v_free[i % ST]);
+            if (r == 0) {
+              mbar_arrive(&v_free[i % ST]);
+              if (!plain) mbar_arrive(&v_free[i % ST]);
+            }
           }
           if (r == 0) *reinterpret_cast<volatile int*>(&leave_out[g][c & 1]) = by_hand;
         } else if (r == 0) {
@@ -577,11 +612,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
       }
       if (!ok) break;                                    // uniform
+      if (i1 < n_units) next = segment_at(i1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // ---- the segment's result ---------------------------------------------------------------------------
       if (l_run != l_run && m_run == -INFINITY) m_run = 0.f;       // scores that are no numbers: the row has to show it
       const long long head_first = (long long)a.nkv * weigh[cur.b] + cur.kvh * list.weight;
-      const long long w_first = head_first + (long long)list.tiles * (plain ? PLAIN_WEIGHT * cur.rb : PLAIN_WEIGHT * list.plain);
+      const long long w_first = head_first + cur.rb * ((long long)PLAIN_WEIGHT * list.tiles + SEGMENT_WEIGHT);      // (only the last is not PLAIN)
       const int blk_first = (int)(w_first / chunk), blk_last = (int)((w_first + (long long)(list.tiles - 1) * (plain ? PLAIN_WEIGHT : SPLIT_WEIGHT)) / chunk);
       const bool whole = blk_first == blk_last;
       const int place = 2 * blockIdx.x + (i0 > 0);
@@ -637,7 +673,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // the next segment's products overwrite what was read
       __syncwarp();
-      ok = meet();                                       // shares and the queries' place are free again
+      if (!plain) ok = meet();                           // uniform: shares and both accumulators have been read
       i0 = i1;
     }
   }
@@ -650,17 +686,32 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
 }
 
+// Boxes of 64 elements x the heads of a group x the nodes of a tile out of the queries [tokens][heads][hd]: rows of 128 bytes, swizzled, node by node.
+bool query_map(const TreeArgs& a, CUtensorMap* result) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const int group = a.nh / a.nkv;
+  cuuint32_t estr[3] = {1, 1, 1};
+  cuuint64_t dims[3] = {(cuuint64_t)a.hd, (cuuint64_t)a.nh, (cuuint64_t)a.n_tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)a.hd * 2, (cuuint64_t)a.nh * a.hd * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(BQ / group)};
+  return fn(result, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int row_blocks_of(int nodes, int group) { return (nodes + GROUPS * (BQ / group) - 1) / (GROUPS * (BQ / group)); }
+
 int grid_blocks(int n_seqs, int nkv, int row_blocks, int max_len) {
   const long long units = (long long)n_seqs * nkv * row_blocks * ((max_len + TK - 1) / TK), most = llg_sm_count();
   return (int)(units < most ? (units < 1 ? 1 : units) : most);
 }
 
 template <int HD, int ST>
-int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t stream) {
+int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, int blocks, cudaStream_t stream) {
   constexpr int smem = (HD / 64) * (GROUPS * BQ * 128 + 2 * ST * TK * 128);      // more than half a multiprocessor's: tensor memory is a block's alone
   cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: shared memory %d: %s", smem, cudaGetErrorString(e));
-  e = llg_launch(attn_tree_tc_kernel<HD, ST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, a);
+  e = llg_launch(attn_tree_tc_kernel<HD, ST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, mq, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: launch: %s", cudaGetErrorString(e));
   if (llg_check_launch("attn_tree_tc")) return 1;
   return launch_join<HD, ROWS>(a, blocks, "attn_tree_tc", stream);
@@ -669,25 +720,28 @@ int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int 
 }  // namespace
 
 // 1 when this kernel takes the geometry (bfloat16 only).
-LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs) { return (hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS; }
+LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs, int group) {
+  return (hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS && group <= BQ;
+}
 
-// Floats of scratch of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
-LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int rows, int nkv, int hd, int max_len) {
-  const int blocks = grid_blocks(n_seqs, nkv, (rows + ROWS - 1) / ROWS, max_len);
+// Floats of scratch of a launch over trees of up to `nodes` nodes and sequences of up to `max_len` positions.
+LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int nodes, int nkv, int group, int hd, int max_len) {
+  const int blocks = grid_blocks(n_seqs, nkv, row_blocks_of(nodes, group), max_len);
   return hd == 64 ? Place<64, ROWS>::floats(blocks) : Place<128, ROWS>::floats(blocks);
 }
 
 LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
   const TreeArgs& a = *args;
   if (check_tree(a, "attn_tree_tc")) return 1;
-  LLG_REQUIRE(llg_attn_tree_tc_supported(a.hd, a.vd, a.n_seqs), "attn_tree_tc: heads of %d and %d elements (64 or 128, the same)", a.hd, a.vd);
+  LLG_REQUIRE(llg_attn_tree_tc_supported(a.hd, a.vd, a.n_seqs, a.nh / a.nkv),
+              "attn_tree_tc: heads of %d and %d elements (64 or 128, the same), %d of them a group (at most %d)", a.hd, a.vd, a.nh / a.nkv, BQ);
   if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq;
   const long long rows = (long long)a.n_pages * a.nkv * TK;
-  if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv))
+  if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv) || !query_map(a, &mq))
     return llg_fail("attn_tree_tc: cuTensorMapEncodeTiled failed or is not available");
-  const int rbs = (a.max_nodes * (a.nh / a.nkv) + ROWS - 1) / ROWS, blocks = grid_blocks(a.n_seqs, a.nkv, rbs, a.max_len);
-  return a.hd == 64 ? launch<64, 8>(a, mk, mv, blocks, stream) : launch<128, 4>(a, mk, mv, blocks, stream);
+  const int blocks = grid_blocks(a.n_seqs, a.nkv, row_blocks_of(a.max_nodes, a.nh / a.nkv), a.max_len);
+  return a.hd == 64 ? launch<64, 8>(a, mk, mv, mq, blocks, stream) : launch<128, 4>(a, mk, mv, mq, blocks, stream);
 }
 
 // Error code recorded when a wait ran out (0 = none); clears it.  Synchronises the device.
