@@ -57,11 +57,10 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   unsigned char* Ks = smem;                            // [STAGES][TILE_BYTES]
   unsigned char* Vs = smem + STAGES * TILE_BYTES;
   __shared__ uint64_t full[STAGES], empty[STAGES], work_bar;
-  __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1];
-  __shared__ int3 warp_total[THREADS / 32];
+  __shared__ Plan plan;
   __shared__ int abort_flag;
   __shared__ int node_depth[LLG_TREE_NODES];
-  __shared__ float merge[WK > 1 ? WORK_WARPS : 1][WK > 1 ? 16 : 1][SLICE + 2];
+  __shared__ __align__(16) float merge[WK > 1 ? WORK_WARPS : 1][WK > 1 ? 16 : 1][SLICE + 2];
   __shared__ float2 merge_ml[WK > 1 ? WORK_WARPS : 1][16];
 
   pdl_launch_dependents();
@@ -84,16 +83,16 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  plan_units<THREADS>(a, ROWS, sums, row_blocks, (int*)nullptr, warp_total, [](int, int, int) { return 0; });
+  plan_units<THREADS>(a, ROWS, plan, nullptr, [](int, int, int) { return 0; });
   const int G = a.nh / a.nkv;
-  const long long units = (long long)a.nkv * sums[a.n_seqs];
-  const long long chunk = (units + gridDim.x - 1) / gridDim.x;
-  const long long u0 = (long long)blockIdx.x * chunk, u1 = min(units, u0 + chunk);
+  const int units = a.nkv * plan.sums[a.n_seqs];
+  const int chunk = (unsigned)(units + gridDim.x - 1) / gridDim.x;
+  const int u0 = min(units, (int)blockIdx.x * chunk), u1 = min(units, u0 + chunk);
   typedef Place<HDP, ROWS> P;
   if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
   volatile int* abortp = &abort_flag;
-  const int n_units = (int)(u1 - u0);
+  const int n_units = u1 - u0;
 
   if (warp == WORK_WARPS) {
     // ---- copies: the lanes look up the pages of 32 tiles side by side, then each in turn issues its tile's boxes ----
@@ -103,9 +102,9 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       const int idx = base + lane;
       int row = 0;
       if (idx < n_units) {
-        const Unit c = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + idx);
-        const int tile = tree_shape(a, c.b).t_first + c.t;
-        const int page = a.page_table[(long long)a.slots[c.b] * a.table_width + tile % a.ring_pages];
+        const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + idx);
+        const TreeShape sh = tree_shape(a, plan, c.b);
+        const int page = a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages];
         row = (page * a.nkv + c.kvh) * TK;
       }
       const int n_here = min(32, n_units - base);
@@ -157,11 +156,11 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     return met;
   };
   int i = 0;                                            // tiles consumed so far
-  long long u = u0;
+  int u = u0;
   while (u < u1) {
-    const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u);
-    const TreeShape sh = tree_shape(a, cur.b);
-    const int n_seg = min(sh.tiles - cur.t, (int)(u1 - u));
+    const Unit cur = locate(plan, a.n_seqs, a.nkv, u);
+    const TreeShape sh = tree_shape(a, plan, cur.b);
+    const int n_seg = min(sh.tiles - cur.t, u1 - u);
     const int row0 = cur.rb * ROWS, n_rows = min(ROWS, sh.n * G - row0);
     // depths of the tree's nodes, for windows (read by tiles with nodes only; the last segment's readers are behind a work_sync)
     if (a.window > 0) {
@@ -325,9 +324,9 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if (l[r] != l[r] && m[r] == -INFINITY) m[r] = 0.f;             // scores that are no numbers: the row has to show it
     }
-    const int rbs = row_blocks[cur.b + 1] - row_blocks[cur.b];
-    const long long p_first = (long long)a.nkv * sums[cur.b] + ((long long)cur.kvh * rbs + cur.rb) * sh.tiles;   // the rows' first unit
-    const int blk_first = (int)(p_first / chunk), blk_last = (int)((p_first + sh.tiles - 1) / chunk);
+    const int rbs = plan.blocks[cur.b + 1] - plan.blocks[cur.b];
+    const unsigned p_first = a.nkv * plan.sums[cur.b] + (cur.kvh * rbs + cur.rb) * sh.tiles;      // the rows' first unit
+    const int blk_first = p_first / (unsigned)chunk, blk_last = (p_first + sh.tiles - 1) / (unsigned)chunk;
     const bool whole = blk_first == blk_last;
     const int place = 2 * blockIdx.x + (u > u0);
     if (!whole && cur.t == 0 && tid == 0)

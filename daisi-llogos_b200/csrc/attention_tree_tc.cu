@@ -29,8 +29,8 @@ LLG_API const char* llg_last_error() { return g_llg_error; }
 namespace {
 
 constexpr int BQ = 128;                       // rows of a block: lanes of tensor memory
-constexpr int ROWS = 2 * BQ;                  // of a row block, at most
-constexpr int PLAIN_WEIGHT = 3, SPLIT_WEIGHT = 2, SEGMENT_WEIGHT = 6;
+// what a run's parts take, measured: 2,800 cycles a PLAIN tile, 1,660 a SPLIT tile
+constexpr int PLAIN_WEIGHT = 5, SPLIT_WEIGHT = 3, SEGMENT_WEIGHT = 8;
 constexpr int GROUPS = 2, WORKERS = GROUPS * BQ;
 constexpr int ISSUE_WARP = WORKERS / 32, K_LOAD_WARP = ISSUE_WARP + 1, V_LOAD_WARP = ISSUE_WARP + 2, ISSUE_WARP_2 = ISSUE_WARP + 3;
 constexpr int THREADS = (ISSUE_WARP_2 + 1) * 32;
@@ -106,85 +106,70 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) { return (uint32_t)(
 
 // A sequence's share of the list: tiles, row blocks of which the first `plain` have more than 128 rows, and the weight of one head.
 struct Share {
-  int tiles, rbs, plain;
-  long long weight;
+  int tiles, rbs, plain, weight;
 };
-// `weights[b]`: the weight of one head in the sequences before b
-__device__ __forceinline__ Share share_of(const int* sums, const int* blocks, const int* weights, int b) {
+// `weigh[b]`: the weight of one head in the sequences before b
+__device__ __forceinline__ Share share_of(const Plan& p, const int* weigh, int b) {
   Share s;
-  s.rbs = blocks[b + 1] - blocks[b];
-  s.tiles = s.rbs > 0 ? (sums[b + 1] - sums[b]) / s.rbs : 0;
-  s.weight = weights[b + 1] - weights[b];
-  // weight = tiles (PLAIN_WEIGHT plain + SPLIT_WEIGHT (rbs - plain)) + SEGMENT_WEIGHT rbs, the first two one apart
-  s.plain = s.tiles > 0 ? (int)((s.weight - SEGMENT_WEIGHT * s.rbs) / s.tiles) - SPLIT_WEIGHT * s.rbs : 0;
+  s.rbs = p.blocks[b + 1] - p.blocks[b];
+  s.tiles = s.rbs > 0 ? (unsigned)(p.sums[b + 1] - p.sums[b]) / (unsigned)s.rbs : 0;
+  s.weight = weigh[b + 1] - weigh[b];
+  // weight = tiles (PLAIN_WEIGHT plain + SPLIT_WEIGHT (rbs - plain)) + SEGMENT_WEIGHT rbs
+  s.plain = s.tiles > 0 ? ((unsigned)(s.weight - SEGMENT_WEIGHT * s.rbs) / (unsigned)s.tiles - SPLIT_WEIGHT * s.rbs) / (PLAIN_WEIGHT - SPLIT_WEIGHT) : 0;
   return s;
 }
-static_assert(PLAIN_WEIGHT == SPLIT_WEIGHT + 1, "share_of");
 
 // The first unit whose weight begins at w or behind it.
-__device__ __forceinline__ long long unit_at(const int* sums, const int* blocks, const int* weights, int n_seqs, int nkv, long long w) {
-  if (w >= (long long)nkv * weights[n_seqs]) return (long long)nkv * sums[n_seqs];
+__device__ __forceinline__ int unit_at(const Plan& p, const int* weigh, int n_seqs, int nkv, int w) {
+  if (w >= nkv * weigh[n_seqs]) return nkv * p.sums[n_seqs];
   int lo = 0, hi = n_seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((long long)nkv * weights[mid] <= w) lo = mid;
+    if (nkv * weigh[mid] <= w) lo = mid;
     else hi = mid - 1;
   }
-  const Share s = share_of(sums, blocks, weights, lo);
-  const long long r = w - (long long)nkv * weights[lo], kvh = r / s.weight, in = r - kvh * s.weight;
-  const long long block = (long long)PLAIN_WEIGHT * s.tiles + SEGMENT_WEIGHT, rb = min(in / block, (long long)s.plain), x = in - rb * block;
-  const int each = rb < s.plain ? PLAIN_WEIGHT : SPLIT_WEIGHT;
+  const Share s = share_of(p, weigh, lo);
+  const unsigned r = w - nkv * weigh[lo], kvh = r / (unsigned)s.weight, in = r - kvh * s.weight;
+  const unsigned block = PLAIN_WEIGHT * s.tiles + SEGMENT_WEIGHT, rb = min(in / block, (unsigned)s.plain), x = in - rb * block;
+  const unsigned at = (int)rb < s.plain ? (x + PLAIN_WEIGHT - 1) / PLAIN_WEIGHT : (x + SPLIT_WEIGHT - 1) / SPLIT_WEIGHT;
   // (a row block's last SEGMENT_WEIGHT begins no unit)
-  return (long long)nkv * sums[lo] + kvh * s.tiles * s.rbs + rb * s.tiles + min((long long)s.tiles, (x + each - 1) / each);
+  return nkv * p.sums[lo] + kvh * s.tiles * s.rbs + rb * s.tiles + min((unsigned)s.tiles, at);
 }
 
-// ST: stages of keys, and of values
-template <int HD, int ST>
+// QT: tiles of queries that a row block may have (1: SPLIT alone).  KST, VST: stages of keys and of values.
+template <int HD, int QT, int KST, int VST>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
                     TreeArgs a) {
-  static_assert(ST % 2 == 0, "where the groups take turns with the tiles, a stage belongs to one of them: a wait for its next phase by parity means "
+  static_assert(KST % 2 == 0 && VST % 2 == 0, "where the groups take turns with the tiles, a stage belongs to one of them: a wait for its next phase by parity means "
                 "something only to who has seen the last one");
   constexpr int KB = HD / 64, Q_BYTES = KB * BQ * 128, KV_BYTES = KB * TK * 128;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* Qs = smem;
-  unsigned char* Ks = Qs + GROUPS * Q_BYTES;         // [ST]
-  unsigned char* Vs = Ks + ST * KV_BYTES;            // [ST]
-  __shared__ uint64_t k_full[ST], k_free[ST], v_full[ST], v_free[ST];
+  unsigned char* Ks = Qs + QT * Q_BYTES;             // [KST]
+  unsigned char* Vs = Ks + KST * KV_BYTES;           // [VST]
+  __shared__ uint64_t k_full[KST], k_free[KST], v_full[VST], v_free[VST];
   __shared__ uint64_t s_full[GROUPS][2], p_ready[GROUPS][2], o_done[GROUPS], q_full, q_free, meet_bar, group_bar[GROUPS];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
   __shared__ int wild[GROUPS][3], leave_out[GROUPS][2];
   __shared__ float2 share[GROUPS][BQ];               // each group's maximum and sum of a row
-  __shared__ int sums[MAX_SEQS + 1], row_blocks[MAX_SEQS + 1], weigh[MAX_SEQS + 1];
-  __shared__ int3 warp_total[THREADS / 32];
+  __shared__ Plan plan;
+  __shared__ int weigh[MAX_SEQS + 1];
 
-  pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((smem_u32(smem) & 1023u) != 0) {               // uniform over the block
     if (tid == 0) atomicCAS(&g_error, 0, 3);
     return;
   }
-  const int G = a.nh / a.nkv, tile_nodes = BQ / G, tile_rows = tile_nodes * G, block_rows = GROUPS * tile_rows;
-  plan_units<THREADS>(a, block_rows, sums, row_blocks, weigh, warp_total, [&](int rows, int rbs, int tiles) {
-    const int split = rbs > 0 && rows - (rbs - 1) * block_rows <= tile_rows;
-    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split) + SEGMENT_WEIGHT * rbs;
-  });
-  // (a run's weight is at least a unit's, so no run between two others is without a unit)
-  const long long weight = (long long)a.nkv * weigh[a.n_seqs];
-  const long long chunk = max((long long)PLAIN_WEIGHT, (weight + gridDim.x - 1) / gridDim.x);
-  const long long u0 = unit_at(sums, row_blocks, weigh, a.n_seqs, a.nkv, blockIdx.x * chunk);
-  const long long u1 = unit_at(sums, row_blocks, weigh, a.n_seqs, a.nkv, (blockIdx.x + 1) * chunk);
-  typedef Place<HD, ROWS> P;
-  if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
-  if (u0 >= u1) return;                              // uniform over the block
-  const int n_units = (int)(u1 - u0);
-  if (tid == 0) {
-    for (int s = 0; s < ST; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_free[s], GROUPS);                 // (one group's lane alone arrives for both)
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_free[s], GROUPS);
+  if (tid == K_LOAD_WARP * 32) {
+    for (int st = 0; st < KST; ++st) {
+      mbar_init(&k_full[st], 1);
+      mbar_init(&k_free[st], GROUPS);                // (where one group has a tile, its lane arrives for both)
+    }
+    for (int st = 0; st < VST; ++st) {
+      mbar_init(&v_full[st], 1);
+      mbar_init(&v_free[st], GROUPS);
     }
     for (int g = 0; g < GROUPS; ++g) {
       mbar_init(&s_full[g][0], 1);
@@ -202,7 +187,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  pdl_wait();
+  if (warp == ISSUE_WARP) {
     warp_whole();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
                  "r"((uint32_t)TMEM_COLS)
@@ -210,10 +196,22 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
+  const int G = a.nh / a.nkv, tile_nodes = BQ / G, tile_rows = tile_nodes * G, block_rows = QT * tile_rows;
+  plan_units<THREADS>(a, block_rows, plan, weigh, [&](int rows, int rbs, int tiles) {
+    const int split = QT == 1 ? rbs : rbs > 0 && rows - (rbs - 1) * block_rows <= tile_rows;
+    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split) + SEGMENT_WEIGHT * rbs;
+  });                                                // (its barriers also stand between the ones above and their use)
   // (not before: a block of the next kernel must not take tensor memory ahead of this one and then wait for it)
   pdl_launch_dependents();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // (a run's weight is at least a unit's, so no run between two others is without a unit)
+  const int weight = a.nkv * weigh[a.n_seqs];
+  const int chunk = max(PLAIN_WEIGHT, (int)((unsigned)(weight + gridDim.x - 1) / gridDim.x));
+  const int u0 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, (int)blockIdx.x * chunk));
+  const int u1 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, ((int)blockIdx.x + 1) * chunk));
+  typedef Place<HD, QT * BQ> P;
+  if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
+  const int n_units = u1 - u0;                       // (none: every role passes by)
   const uint32_t tmem = tmem_base_slot;
   volatile int* abortp = &abort_flag;
   auto give_up = [&](int code) {
@@ -226,6 +224,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     unsigned char* base = keys ? Ks : Vs;
     uint64_t* full = keys ? k_full : v_full;
     uint64_t* freeb = keys ? k_free : v_free;
+    const int stages = keys ? KST : VST;
     const CUtensorMap* map = keys ? &map_k : &map_v;
     if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     // The values' warp brings each segment's queries too, ahead of its first values, when all of the last segment's scores are there.
@@ -235,22 +234,21 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int idx = first + lane;
       int row = 0, q_tok = 0, q_head = 0, q_tiles = 0;        // q_tiles: of queries, where a segment begins
       if (idx < n_units) {
-        const Unit c = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + idx);
-        const TreeShape sh = tree_shape(a, c.b);
-        const int tile = sh.t_first + c.t;
+        const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + idx);
+        const TreeShape sh = tree_shape(a, plan, c.b);
         if (!keys && (idx == 0 || c.t == 0)) {
-          q_tok = sh.tok0 + c.rb * GROUPS * tile_nodes;
+          q_tok = sh.tok0 + c.rb * QT * tile_nodes;
           q_head = c.kvh * G;
-          q_tiles = sh.n - c.rb * GROUPS * tile_nodes > tile_nodes ? 2 : 1;
+          q_tiles = QT > 1 && sh.n - c.rb * QT * tile_nodes > tile_nodes ? 2 : 1;
         }
-        const int page = a.page_table[(long long)a.slots[c.b] * a.table_width + tile % a.ring_pages];
+        const int page = a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages];
         row = (page * a.nkv + c.kvh) * TK;
       }
       const int n_here = min(32, n_units - first);
       for (int k = 0; k < n_here && fine; ++k) {
         int sent = 0;
         if (lane == k) {
-          const int i = first + k, st = i % ST;
+          const int i = first + k, st = i % stages;
           if (q_tiles > 0) {
             if (segments > 0 && !mbar_wait(&q_free, (segments - 1) & 1, abortp)) {
               give_up(4);
@@ -265,7 +263,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
           }
           if (!fine) {
-          } else if (i >= ST && !mbar_wait(&freeb[st], (i / ST - 1) & 1, abortp)) {
+          } else if (i >= stages && !mbar_wait(&freeb[st], (i / stages - 1) & 1, abortp)) {
             give_up(4);
             fine = false;
           } else {
@@ -281,9 +279,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     // copies still write into this block's shared memory until their barrier completes
     if (lane == 0) {
-      for (int i = max(0, issued - ST); i < issued; ++i) {
+      for (int i = max(0, issued - stages); i < issued; ++i) {
         const unsigned long long t0 = now_ns();
-        while (!mbar_try_wait(&full[i % ST], (i / ST) & 1)) {
+        while (!mbar_try_wait(&full[i % stages], (i / stages) & 1)) {
           if (now_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(&g_error, 0, 7); break; }
         }
       }
@@ -311,11 +309,11 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // c: the group's tiles so far.  Scores into buffer c % 2, which O += P(c-2) V(c-2) has read by then; a segment's first tile comes
       // when all of the earlier ones are done, and waits for the last of them (a wait by parity sees one phase back).
       auto issue_scores = [&](int i, int c, uint32_t qa, bool first, bool plain) {
-        wait_or_fail(&k_full[i % ST], (i / ST) & 1, 5);
+        wait_or_fail(&k_full[i % KST], (i / KST) & 1, 5);
         if (first ? c >= 1 : c >= 2) wait_or_fail(&o_done[g], (first ? c - 1 : c) & 1, 6);
         if (!ok) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t ka = smem_u32(Ks + (i % ST) * KV_BYTES);
+        const uint32_t ka = smem_u32(Ks + (i % KST) * KV_BYTES);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks) {
           const uint32_t blk = ks >> 2, kk = ks & 3;
@@ -323,13 +321,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     desc_kmajor(ka + blk * (TK * 128) + kk * 32), IDESC_S, ks != 0);
         }
         umma_commit(&s_full[g][c & 1]);
-        umma_commit(&k_free[i % ST]);
-        if (!plain) umma_commit(&k_free[i % ST]);
+        umma_commit(&k_free[i % KST]);
+        if (!plain) umma_commit(&k_free[i % KST]);
       };
       int i0 = 0, c = 0;
       for (int seg = 0; i0 < n_units && ok; ++seg) {
-        const Unit cur = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i0);
-        const Share sh = share_of(sums, row_blocks, weigh, cur.b);
+        const Unit cur = locate(plan, a.n_seqs, a.nkv, u0 + i0);
+        const Share sh = share_of(plan, weigh, cur.b);
         const int i1 = min(n_units, i0 + sh.tiles - cur.t);
         const bool plain = cur.rb < sh.plain;
         const int step = plain ? 1 : 2;
@@ -348,7 +346,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
           // (weights first: behind them lie the meetings of earlier segments, so all of their values were used)
           wait_or_fail(&p_ready[g][c & 1], (c >> 1) & 1, 6);
-          wait_or_fail(&v_full[i % ST], (i / ST) & 1, 5);
+          wait_or_fail(&v_full[i % VST], (i / VST) & 1, 5);
           // (the last tile's product is waited for at the next segment's begin: the one ahead of it has to be done while that can be told)
           if (c >= 1 && i + step >= i1) wait_or_fail(&o_done[g], (c - 1) & 1, 6);
           if (!ok) break;
@@ -356,13 +354,13 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (*reinterpret_cast<volatile int*>(&leave_out[g][c & 1])) {
             umma_commit(&o_done[g]);                   // the group has added this tile up itself, and gives its values back itself
           } else {
-            const uint32_t pa = tmem + g * G_COLS + (uint32_t)(c & 1) * TK, va = smem_u32(Vs + (i % ST) * KV_BYTES);
+            const uint32_t pa = tmem + g * G_COLS + (uint32_t)(c & 1) * TK, va = smem_u32(Vs + (i % VST) * KV_BYTES);
 #pragma unroll
             for (int kk = 0; kk < TK / 16; ++kk)
               umma_bf16_ts(tmem + g * G_COLS + O_COL, pa + kk * 8, desc_mnmajor(va + kk * 2048, TK * 128), IDESC_O, started || kk != 0);
             umma_commit(&o_done[g]);
-            umma_commit(&v_free[i % ST]);
-            if (!plain) umma_commit(&v_free[i % ST]);
+            umma_commit(&v_free[i % VST]);
+            if (!plain) umma_commit(&v_free[i % VST]);
           }
           started = true;
         }
@@ -405,9 +403,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     };
     auto segment_at = [&](int i) -> Segment {
       Segment x;
-      x.at = locate(sums, row_blocks, a.n_seqs, a.nkv, u0 + i);
-      x.list = share_of(sums, row_blocks, weigh, x.at.b);
-      x.sh = tree_shape(a, x.at.b);
+      x.at = locate(plan, a.n_seqs, a.nkv, u0 + i);
+      x.list = share_of(plan, weigh, x.at.b);
+      x.sh = tree_shape(a, plan, x.at.b);
       x.plain = x.at.rb < x.list.plain;                 // the same for the block
       x.row0 = x.at.rb * block_rows;
       x.n_rows = min(block_rows, x.sh.n * G - x.row0);
@@ -418,7 +416,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       x.depth = __popcll(x.bits) - 1;
       return x;
     };
-    Segment next = segment_at(0);
+    Segment next;
+    if (n_units > 0) next = segment_at(0);
     while (i0 < n_units && ok) {
       const Unit cur = next.at;
       const TreeShape sh = next.sh;
@@ -474,11 +473,11 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
           for (int x = 0; x < TK; ++x) sv[x] = ((x < 32 ? s_lo : s_hi) >> (x & 31)) & 1 ? sv[x] : -INFINITY;
           // the group looks the tile's values over
-          const bool landed = mbar_wait(&v_full[i % ST], (i / ST) & 1, abortp);
+          const bool landed = mbar_wait(&v_full[i % VST], (i / VST) & 1, abortp);
           if (!landed) give_up(5);
           bool found = false;
           if (landed) {
-            const uint4* v = reinterpret_cast<const uint4*>(Vs + (i % ST) * KV_BYTES);
+            const uint4* v = reinterpret_cast<const uint4*>(Vs + (i % VST) * KV_BYTES);
 #pragma unroll
             for (int x = 0; x < KV_BYTES / 16 / BQ; ++x) {
               const uint4 y = v[x * BQ + r];
@@ -546,7 +545,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         if (touch || by_hand) {                          // uniform
-          const unsigned char* vt = Vs + (i % ST) * KV_BYTES;
+          const unsigned char* vt = Vs + (i % VST) * KV_BYTES;
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 16) {          // uniform
             uint32_t rr[16];
@@ -594,8 +593,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             ok = group_meet();                           // all of the group have read the values
             if (!ok) break;                              // uniform
             if (r == 0) {
-              mbar_arrive(&v_free[i % ST]);
-              if (!plain) mbar_arrive(&v_free[i % ST]);
+              mbar_arrive(&v_free[i % VST]);
+              if (!plain) mbar_arrive(&v_free[i % VST]);
             }
           }
           if (r == 0) *reinterpret_cast<volatile int*>(&leave_out[g][c & 1]) = by_hand;
@@ -616,9 +615,9 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       // ---- the segment's result ---------------------------------------------------------------------------
       if (l_run != l_run && m_run == -INFINITY) m_run = 0.f;       // scores that are no numbers: the row has to show it
-      const long long head_first = (long long)a.nkv * weigh[cur.b] + cur.kvh * list.weight;
-      const long long w_first = head_first + cur.rb * ((long long)PLAIN_WEIGHT * list.tiles + SEGMENT_WEIGHT);      // (only the last is not PLAIN)
-      const int blk_first = (int)(w_first / chunk), blk_last = (int)((w_first + (long long)(list.tiles - 1) * (plain ? PLAIN_WEIGHT : SPLIT_WEIGHT)) / chunk);
+      const int each = plain ? PLAIN_WEIGHT : SPLIT_WEIGHT, block = (cur.rb < list.plain || QT > 1 ? PLAIN_WEIGHT : SPLIT_WEIGHT) * list.tiles + SEGMENT_WEIGHT;
+      const unsigned w_first = a.nkv * weigh[cur.b] + cur.kvh * list.weight + cur.rb * block;      // (of two kinds only the last is not PLAIN)
+      const int blk_first = w_first / (unsigned)chunk, blk_last = (w_first + (list.tiles - 1) * each) / (unsigned)chunk;
       const bool whole = blk_first == blk_last;
       const int place = 2 * blockIdx.x + (i0 > 0);
       if (!whole && cur.t == 0 && tid == 0)
@@ -668,7 +667,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         } else if (live) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            P::sums(a.part, place)[(c0 / 4 + q) * ROWS + mine] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            P::sums(a.part, place)[(c0 / 4 + q) * (QT * BQ) + mine] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
         }
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");      // the next segment's products overwrite what was read
@@ -680,7 +679,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // every role comes here, also after a wait that ran out: copies in flight have been waited for above
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == 1) {
+  if (warp == ISSUE_WARP) {
     warp_whole();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)TMEM_COLS) : "memory");
   }
@@ -699,22 +698,26 @@ bool query_map(const TreeArgs& a, CUtensorMap* result) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int row_blocks_of(int nodes, int group) { return (nodes + GROUPS * (BQ / group) - 1) / (GROUPS * (BQ / group)); }
+// Tiles of queries that a row block may have: trees of one tile leave its place to another pair of key stages.
+int query_tiles(int nodes, int group) { return nodes <= BQ / group ? 1 : 2; }
 
-int grid_blocks(int n_seqs, int nkv, int row_blocks, int max_len) {
-  const long long units = (long long)n_seqs * nkv * row_blocks * ((max_len + TK - 1) / TK), most = llg_sm_count();
+int grid_blocks(const TreeArgs& a) {
+  const int per = query_tiles(a.max_nodes, a.nh / a.nkv) * (BQ / (a.nh / a.nkv));
+  const long long units = (long long)a.n_seqs * a.nkv * ((a.max_nodes + per - 1) / per) * ((a.max_len + TK - 1) / TK), most = llg_sm_count();
   return (int)(units < most ? (units < 1 ? 1 : units) : most);
 }
 
-template <int HD, int ST>
-int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, int blocks, cudaStream_t stream) {
-  constexpr int smem = (HD / 64) * (GROUPS * BQ * 128 + 2 * ST * TK * 128);      // more than half a multiprocessor's: tensor memory is a block's alone
-  cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <int HD, int QT, int KST, int VST>
+int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, cudaStream_t stream) {
+  constexpr int smem = (HD / 64) * (QT * BQ * 128 + (KST + VST) * TK * 128);
+  static_assert(smem > 116 * 1024, "more than half a multiprocessor's: tensor memory is a block's alone");
+  const int blocks = grid_blocks(a);
+  cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, QT, KST, VST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: shared memory %d: %s", smem, cudaGetErrorString(e));
-  e = llg_launch(attn_tree_tc_kernel<HD, ST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, mq, a);
+  e = llg_launch(attn_tree_tc_kernel<HD, QT, KST, VST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, mq, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: launch: %s", cudaGetErrorString(e));
   if (llg_check_launch("attn_tree_tc")) return 1;
-  return launch_join<HD, ROWS>(a, blocks, "attn_tree_tc", stream);
+  return launch_join<HD, QT * BQ>(a, blocks, "attn_tree_tc", stream);
 }
 
 }  // namespace
@@ -726,8 +729,15 @@ LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs, int group) {
 
 // Floats of scratch of a launch over trees of up to `nodes` nodes and sequences of up to `max_len` positions.
 LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int nodes, int nkv, int group, int hd, int max_len) {
-  const int blocks = grid_blocks(n_seqs, nkv, row_blocks_of(nodes, group), max_len);
-  return hd == 64 ? Place<64, ROWS>::floats(blocks) : Place<128, ROWS>::floats(blocks);
+  TreeArgs a = {};
+  a.n_seqs = n_seqs;
+  a.max_nodes = nodes;
+  a.nkv = nkv;
+  a.nh = nkv * group;
+  a.max_len = max_len;
+  const int blocks = grid_blocks(a);
+  if (query_tiles(nodes, group) == 1) return hd == 64 ? Place<64, BQ>::floats(blocks) : Place<128, BQ>::floats(blocks);
+  return hd == 64 ? Place<64, 2 * BQ>::floats(blocks) : Place<128, 2 * BQ>::floats(blocks);
 }
 
 LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
@@ -740,8 +750,9 @@ LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
   const long long rows = (long long)a.n_pages * a.nkv * TK;
   if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv) || !query_map(a, &mq))
     return llg_fail("attn_tree_tc: cuTensorMapEncodeTiled failed or is not available");
-  const int blocks = grid_blocks(a.n_seqs, a.nkv, row_blocks_of(a.max_nodes, a.nh / a.nkv), a.max_len);
-  return a.hd == 64 ? launch<64, 8>(a, mk, mv, mq, blocks, stream) : launch<128, 4>(a, mk, mv, mq, blocks, stream);
+  if (query_tiles(a.max_nodes, a.nh / a.nkv) == 1)
+    return a.hd == 64 ? launch<64, 1, 8, 8>(a, mk, mv, mq, stream) : launch<128, 1, 6, 4>(a, mk, mv, mq, stream);
+  return a.hd == 64 ? launch<64, 2, 8, 8>(a, mk, mv, mq, stream) : launch<128, 2, 4, 4>(a, mk, mv, mq, stream);
 }
 
 // Error code recorded when a wait ran out (0 = none); clears it.  Synchronises the device.

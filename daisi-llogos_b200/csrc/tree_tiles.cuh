@@ -84,55 +84,78 @@ __device__ __forceinline__ bool not_finite(uint32_t x) {
 
 // A sequence's tree: its nodes, cached keys, and the key tiles that its rows look at.
 struct TreeShape {
-  int tok0, n, lb, t_first, tiles;
+  int tok0, n, lb, slot, t_first, tiles;
 };
-__device__ __forceinline__ TreeShape tree_shape(const TreeArgs& a, int b) {
+
+// The work of a launch is one list: sequence by sequence, key/value head by key/value head, row block by row block, key tile by key tile.
+// Blocks cut it into equal runs.  Every block works the list out itself, in shared memory: per sequence the units, the row blocks and the weight of
+// one head in the sequences before it, and what there is to know of the first STAGED sequences.  (Counts are 32-bit: a division of 64
+// bits takes a hundred instructions, and a block's begin is a chain of them; the host refuses launches whose list is longer.)
+constexpr int STAGED = 128;
+struct Plan {
+  int sums[MAX_SEQS + 1], blocks[MAX_SEQS + 1];
+  int4 seq[STAGED];                                // tok0, n, lb, slot
+  int3 warp_total[32];
+};
+
+__device__ __forceinline__ TreeShape shape_of(const TreeArgs& a, int4 q) {
   TreeShape s;
-  s.tok0 = a.cu_tokens[b];
-  s.n = max(0, min(min(a.cu_tokens[b + 1], a.n_tokens) - s.tok0, a.max_nodes));
-  s.lb = a.len_before[b];
+  s.tok0 = q.x;
+  s.n = q.y;
+  s.lb = q.z;
+  s.slot = q.w;
   // no row sees less than this under a window (a row without any bit stands one place before the root)
   s.t_first = a.window > 0 ? max(0, s.lb - a.window) / TK : 0;
   s.tiles = s.n > 0 ? (s.lb + s.n + TK - 1) / TK - s.t_first : 0;
   return s;
 }
+__device__ __forceinline__ int4 fetch_seq(const TreeArgs& a, int b) {
+  const int t0 = a.cu_tokens[b], t1 = a.cu_tokens[b + 1], lb = a.len_before[b], slot = a.slots[b];
+  return make_int4(t0, max(0, min(min(t1, a.n_tokens) - t0, a.max_nodes)), lb, slot);
+}
+__device__ __forceinline__ TreeShape tree_shape(const TreeArgs& a, const Plan& p, int b) {
+  return shape_of(a, b < STAGED ? p.seq[b] : fetch_seq(a, b));
+}
 
-// The work of a launch is one list: sequence by sequence, key/value head by key/value head, row block by row block, key tile by key tile.
-// Blocks cut it into equal runs; sums[b] and blocks[b] are the units and the row blocks of one head in the sequences before b.
 struct Unit {
   int b, kvh, rb, t;
 };
-__device__ __forceinline__ Unit locate(const int* sums, const int* blocks, int n_seqs, int nkv, long long u) {
+__device__ __forceinline__ Unit locate(const Plan& p, int n_seqs, int nkv, int u) {
   int lo = 0, hi = n_seqs - 1;                     // last b with nkv * sums[b] <= u
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((long long)nkv * sums[mid] <= u) lo = mid;
+    if (nkv * p.sums[mid] <= u) lo = mid;
     else hi = mid - 1;
   }
   Unit c;
   c.b = lo;
-  const int rbs = blocks[lo + 1] - blocks[lo], tiles = (sums[lo + 1] - sums[lo]) / rbs;
-  const int r = (int)(u - (long long)nkv * sums[lo]), pair = r / tiles;
+  const unsigned rbs = p.blocks[lo + 1] - p.blocks[lo], tiles = (unsigned)(p.sums[lo + 1] - p.sums[lo]) / rbs;
+  const unsigned r = u - nkv * p.sums[lo], pair = r / tiles;
   c.t = r - pair * tiles;
   c.kvh = pair / rbs;
   c.rb = pair - c.kvh * rbs;
   return c;
 }
 
-// All threads of a block: sums[], blocks[] and weights[] (what `weight(rows, row blocks, tiles)` gives a head, in the sequences before b) for row
-// blocks of `rows` query rows.
+// All threads of a block: the plan for row blocks of `rows` query rows, and (weights not null) what `weight(rows, row blocks, tiles)` gives a head.
 template <int THREADS, typename Weight>
-__device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, int* sums, int* blocks, int* weights, int3* warp_total, Weight weight) {
+__device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, Plan& p, int* weights, Weight weight) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = a.nh / a.nkv;
   const int per = (a.n_seqs + THREADS - 1) / THREADS;
   const int b0 = tid * per, b1 = min(a.n_seqs, b0 + per);
   int units = 0, rbs = 0, ws = 0;
-  for (int b = b0; b < b1; ++b) {
-    const TreeShape s = tree_shape(a, b);
-    const int r = (s.n * G + rows - 1) / rows;
+  int4 only = make_int4(0, 0, 0, 0);               // of a thread with one sequence
+  auto add = [&](int4 q) {
+    const TreeShape s = shape_of(a, q);
+    const int r = (unsigned)(s.n * G + rows - 1) / (unsigned)rows;
     units += r * s.tiles;
     rbs += r;
     ws += weight(s.n * G, r, s.tiles);
+  };
+  for (int b = b0; b < b1; ++b) {
+    only = fetch_seq(a, b);
+    if (b < STAGED) p.seq[b] = only;
+    add(only);
   }
   int iu = units, ir = rbs, iw = ws;
 #pragma unroll
@@ -144,27 +167,26 @@ __device__ __forceinline__ void plan_units(const TreeArgs& a, int rows, int* sum
       iw += pw;
     }
   }
-  if (lane == 31) warp_total[warp] = make_int3(iu, ir, iw);
+  if (lane == 31) p.warp_total[warp] = make_int3(iu, ir, iw);
   __syncthreads();
-  int su = iu - units, sr = ir - rbs, sw = iw - ws;
+  int before_u = iu - units, before_r = ir - rbs, before_w = iw - ws;
   for (int w = 0; w < warp; ++w) {
-    su += warp_total[w].x;
-    sr += warp_total[w].y;
-    sw += warp_total[w].z;
+    before_u += p.warp_total[w].x;
+    before_r += p.warp_total[w].y;
+    before_w += p.warp_total[w].z;
   }
   if (tid == 0) {
-    sums[0] = blocks[0] = 0;
+    p.sums[0] = p.blocks[0] = 0;
     if (weights) weights[0] = 0;
   }
+  units = before_u;
+  rbs = before_r;
+  ws = before_w;
   for (int b = b0; b < b1; ++b) {
-    const TreeShape s = tree_shape(a, b);
-    const int r = (s.n * G + rows - 1) / rows;
-    su += r * s.tiles;
-    sr += r;
-    sw += weight(s.n * G, r, s.tiles);
-    sums[b + 1] = su;
-    blocks[b + 1] = sr;
-    if (weights) weights[b + 1] = sw;
+    add(per == 1 ? only : fetch_seq(a, b));
+    p.sums[b + 1] = units;
+    p.blocks[b + 1] = rbs;
+    if (weights) weights[b + 1] = ws;
   }
   __syncthreads();
 }
@@ -297,6 +319,9 @@ inline int check_tree(const TreeArgs& a, const char* what) {
   LLG_REQUIRE(a.scale > 0.f, "%s: the softmax scale must be positive", what);
   LLG_REQUIRE(a.part && a.max_len > 0 && a.n_pages > 0, "%s: needs scratch, a bound on the lengths and pages", what);
   LLG_REQUIRE((uintptr_t)a.k_pages % 16 == 0 && (uintptr_t)a.v_pages % 16 == 0 && (uintptr_t)a.q % 16 == 0, "%s: storage must be 16-byte aligned", what);
+  const long long tiles = (a.max_len + TK - 1) / TK, blocks = a.max_nodes * (a.nh / a.nkv) / 16 + 1;
+  LLG_REQUIRE(16 * tiles * blocks * a.nkv * a.n_seqs < 2147483647LL, "%s: %d sequences of %d positions are more work than one launch counts", what, a.n_seqs,
+              a.max_len);
   LLG_REQUIRE((long long)a.n_pages * a.nkv * TK < 2147483647LL, "%s: too many page rows for a tensor map coordinate", what);
   return 0;
 }
