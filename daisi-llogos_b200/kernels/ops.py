@@ -577,6 +577,10 @@ def _load_lib(name: str):
         lib.llg_attn_tree_tc_status.restype = c_int
     elif name == "key_weights":
         lib.llg_key_weights_simt.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
+    elif name == "key_weights_mma":
+        lib.llg_key_weights_mma.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
+        lib.llg_key_weights_mma_supported.argtypes = [c_int]
+        lib.llg_key_weights_mma_status.restype = c_int
     elif name == "cache_rows":
         lib.llg_tree_accept.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p]
@@ -2570,6 +2574,9 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
     _check(lib, lib.llg_tree_accept(_ptr(logits), logits.shape[1], *ptrs, b, n, _ptr(scratch), _ptr(path), _ptr(n_path), _ptr(next_token), _stream()))
 
 
+USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel with bfloat16
+
+
 class KeyWeightPlan:
     """How ``key_weights`` will run for one batch shape.  Made by ``key_weights_plan``; callers read ``scratch_floats`` and ``n_counters``."""
 
@@ -2589,11 +2596,12 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
     if n_seqs <= 0 or last <= 0 or max_len <= 0:
         raise KernelError("key_weights: needs sequences, queries and a bound on the lengths")
     lib = _lib("key_weights")
-    keys = lib.llg_key_weights_keys()
+    mma = USE_MMA_WEIGHTS and dtype == torch.bfloat16 and _lib("key_weights_mma").llg_key_weights_mma_supported(head_dim)
+    keys = _lib("key_weights_mma").llg_key_weights_mma_keys() if mma else lib.llg_key_weights_keys()
     chunks, rows = -(-max_len // keys), n_heads // n_kv_heads * last
     total = n_seqs * n_kv_heads * rows
     scores = total * chunks * keys if rows <= lib.llg_key_weights_store_rows() else 0
-    return KeyWeightPlan("simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, chunks, -(-2 * total * chunks // 4) * 4,
+    return KeyWeightPlan("mma" if mma else "simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, chunks, -(-2 * total * chunks // 4) * 4,
                          -(-2 * total // 4) * 4, scores, n_seqs * n_kv_heads)
 
 
@@ -2638,8 +2646,17 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     a.counters = _ptr(counters)
     a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last, a.chunks = b, n, nh, nkv, hd, last, plan.chunks
     a.scale = float(scale)
-    lib = _lib("key_weights")
-    _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), _stream()), kernels=2)
+    if plan.kind == "mma":
+        lib = _lib("key_weights_mma")
+        _check(lib, lib.llg_key_weights_mma(byref(a), k_pages.shape[0], _stream()), kernels=2)
+    else:
+        lib = _lib("key_weights")
+        _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), _stream()), kernels=2)
+
+
+def key_weights_status() -> int:
+    """Error code that the tensor-core kernel that weighs keys recorded when a wait ran out (0 = none); synchronises."""
+    return _lib("key_weights_mma").llg_key_weights_mma_status()
 
 
 def keep_keys(weights: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, chosen: torch.Tensor, *, first: int,

@@ -431,6 +431,12 @@ def test_weights_of_keys(ops, dtype, nh, nkv, hd, before, brings, last):
     assert torch.equal(once.nan_to_num(9.0), weights.nan_to_num(9.0))    # sums run in one order
 
 
+@pytest.mark.parametrize("hd", [64, 128, 40])
+def test_bfloat16_weights_on_the_cuda_cores(ops, hd, monkeypatch):
+    monkeypatch.setattr(ops, "USE_MMA_WEIGHTS", False)
+    test_weights_of_keys(ops, BF16, 8, 2, hd, [5, 0, 64], [1, 200, 64], 8)
+
+
 def test_weights_of_long_sequences_in_a_graph(ops):
     """Thousands of keys: many blocks' sums are joined; every query's shares add up to one."""
     nh, nkv, hd, before = 8, 2, 128, [3900, 100]
@@ -564,3 +570,8 @@ def test_rows_move_within_a_ring_and_in_a_graph(ops):
         src, dst = base + s, base + j
         want[table[0, dst // 64 % ring], :, dst % 64] = pool[table[0, src // 64 % ring], :, src % 64]
     assert torch.equal(dev.cpu(), want) and torch.equal(values.cpu(), want.neg())
+
+
+def test_no_wait_for_keys_has_run_out(ops):
+    """Behind the tests above."""
+    assert ops.key_weights_status() == 0 and ops.attn_tree_status() == 0
