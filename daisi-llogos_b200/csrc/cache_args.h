@@ -37,11 +37,9 @@ struct KeyWeightArgs {
   const int* len_before;      // [n_seqs]
   float* weights;             // [slots][nkv][weight_width]
   int weight_width;
-  float* stats;               // [n_seqs][nkv][rows][chunks][2], rows = nh / nkv * last
-  float* row_end;             // [n_seqs][nkv][rows][2]
-  float* scores;              // [n_seqs][nkv][rows][chunks * keys per block], or null: the second pass works them out again
-  int* counters;              // [n_seqs * nkv], zero before and after a launch
-  int n_seqs, n_tokens, nh, nkv, hd, last, chunks;
+  float* stats;               // [n_seqs][nkv][splits][rows][2], rows = nh / nkv * last: a split's maximum and sum
+  float* scores;              // [n_seqs][nkv][rows][splits * split_keys], or null: the second pass works them out again
+  int n_seqs, n_tokens, nh, nkv, hd, last, splits, split_keys;
   float scale;
 };
 

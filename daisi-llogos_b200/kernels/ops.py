@@ -382,9 +382,9 @@ class _KeyWeightArgs(Structure):
     _fields_ = [
         ("q", c_void_p), ("k_pages", c_void_p), ("page_table", c_void_p), ("table_width", c_int),
         ("slots", c_void_p), ("cu_tokens", c_void_p), ("len_before", c_void_p), ("weights", c_void_p), ("weight_width", c_int),
-        ("stats", c_void_p), ("row_end", c_void_p), ("scores", c_void_p), ("counters", c_void_p),
-        ("n_seqs", c_int), ("n_tokens", c_int), ("nh", c_int), ("nkv", c_int), ("hd", c_int), ("last", c_int), ("chunks", c_int),
-        ("scale", c_float),
+        ("stats", c_void_p), ("scores", c_void_p),
+        ("n_seqs", c_int), ("n_tokens", c_int), ("nh", c_int), ("nkv", c_int), ("hd", c_int), ("last", c_int), ("splits", c_int),
+        ("split_keys", c_int), ("scale", c_float),
     ]
 
 
@@ -2580,10 +2580,10 @@ USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel
 class KeyWeightPlan:
     """How ``key_weights`` will run for one batch shape.  Made by ``key_weights_plan``; callers read ``scratch_floats`` and ``n_counters``."""
 
-    def __init__(self, kind: str, key, last: int, max_len: int, chunks: int, stats: int, ends: int, scores: int, n_counters: int):
-        self.kind, self.key, self.last, self.max_len, self.chunks = kind, key, last, max_len, chunks
-        self.stats, self.ends, self.scores, self.n_counters = stats, ends, scores, n_counters
-        self.scratch_floats = stats + ends + scores
+    def __init__(self, kind: str, key, last: int, max_len: int, splits: int, split_keys: int, stats: int, scores: int):
+        self.kind, self.key, self.last, self.max_len, self.splits, self.split_keys = kind, key, last, max_len, splits, split_keys
+        self.stats, self.scores, self.n_counters = stats, scores, 0
+        self.scratch_floats = stats + scores
 
 
 def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n_kv_heads: int, head_dim: int, max_len: int) -> KeyWeightPlan:
@@ -2597,12 +2597,15 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
         raise KernelError("key_weights: needs sequences, queries and a bound on the lengths")
     lib = _lib("key_weights")
     mma = USE_MMA_WEIGHTS and dtype == torch.bfloat16 and _lib("key_weights_mma").llg_key_weights_mma_supported(head_dim)
-    keys = _lib("key_weights_mma").llg_key_weights_mma_keys() if mma else lib.llg_key_weights_keys()
-    chunks, rows = -(-max_len // keys), n_heads // n_kv_heads * last
+    tile, rows = lib.llg_key_weights_tile(), n_heads // n_kv_heads * last
+    tiles = -(-max_len // tile)
+    # splits of at least four tiles, as many as give every multiprocessor six blocks
+    per = max(4, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
+    splits = -(-tiles // per)
     total = n_seqs * n_kv_heads * rows
-    scores = total * chunks * keys if rows <= lib.llg_key_weights_store_rows() else 0
-    return KeyWeightPlan("mma" if mma else "simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, chunks, -(-2 * total * chunks // 4) * 4,
-                         -(-2 * total // 4) * 4, scores, n_seqs * n_kv_heads)
+    scores = total * splits * per * tile if rows <= lib.llg_key_weights_store_rows() else 0
+    return KeyWeightPlan("mma" if mma else "simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, splits, per * tile,
+                         -(-2 * total * splits // 4) * 4, scores)
 
 
 def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, cu_tokens: torch.Tensor,
@@ -2641,10 +2644,10 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     a.slots, a.cu_tokens, a.len_before = _ptr(slots), _ptr(cu_tokens), _ptr(len_before)
     a.weights, a.weight_width = _ptr(weights), weights.shape[2]
     base = _ptr(scratch)
-    a.stats, a.row_end = base, base + 4 * plan.stats
-    a.scores = base + 4 * (plan.stats + plan.ends) if plan.scores else None
-    a.counters = _ptr(counters)
-    a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last, a.chunks = b, n, nh, nkv, hd, last, plan.chunks
+    a.stats = base
+    a.scores = base + 4 * plan.stats if plan.scores else None
+    a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last = b, n, nh, nkv, hd, last
+    a.splits, a.split_keys = plan.splits, plan.split_keys
     a.scale = float(scale)
     if plan.kind == "mma":
         lib = _lib("key_weights_mma")

@@ -110,7 +110,7 @@ def test_the_confirmed_path_refuses(change, says):
     (dict(weights=torch.zeros(3, 2, 130, dtype=BF16)), "weights is"), (dict(page_table=torch.zeros(3, 2, dtype=I32)), "2 pages"),
     (dict(scale=-1.0), "scale must be positive"), (dict(scratch=torch.zeros(59)), "scratch of 59"), (dict(counters=torch.zeros(4)), "4 counters")])
 def test_weights_of_keys_refuse(change, says):
-    plan = ops.KeyWeightPlan("simt", (F32, 2, 4, 2, 16), 1, 130, 3, 30, 10, 20, 4)
+    plan = ops.KeyWeightPlan("simt", (F32, 2, 4, 2, 16), 1, 130, 1, 192, 40, 20)
     given = dict(q=torch.zeros(5, 4, 16), k_pages=torch.zeros(6, 2, 64, 16), page_table=torch.zeros(3, 3, dtype=I32), slots=torch.zeros(2, dtype=I32),
                  cu_tokens=torch.zeros(3, dtype=I32), len_before=torch.zeros(2, dtype=I32), weights=torch.zeros(3, 2, 130), scratch=torch.zeros(60),
                  scale=0.25, last=1, plan=plan, counters=torch.zeros(4, dtype=I32))
