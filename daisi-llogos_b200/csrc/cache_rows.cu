@@ -178,22 +178,29 @@ tree_walk_kernel(const int* __restrict__ picked, const int* __restrict__ tokens,
 // Of a sequence's `len` positions in a layer and head, `keep` stay: the first `first`, the newest `recent`, and of those between them the ones of
 // most weight (of equal ones the lower position; NaN counts as less than everything), written in ascending order.
 //
-// A block takes one (layer, sequence, head).  Weights are compared as whole numbers in the floats' order.  The weight at which the count of larger
-// ones reaches what is wanted is found by bisection over the 32 bits, a bit a round: a count over the block's registers, so the weights
-// are read once.  A warp holds a run of neighbouring positions, so that ballots give every chosen position its place in ascending order
-// with one sum over the warps.
+// A block takes one (layer, sequence, head) and keeps its weights in registers, so that they are read once.  They are compared as whole numbers in
+// the floats' order.  The weight of rank `need` is found by counting: the range between the least and the largest is cut into 2,048 bins (of
+// equal width in that order, which is the floats' logarithm, so weights spread over the bins), the counts are added up from the top to the
+// bin that holds the rank, and that bin is the next range; once at most a block's number of weights is left they are ranked directly.  (A
+// bisection over the 32 bits, a bit and a block's count a round, was bound by its instructions: 131 us for eight sequences of 5,000 to
+// 8,190 keys, 32 layers, 8 heads.)  A warp holds a run of neighbouring positions, so that ballots give every chosen position its place in
+// ascending order with one sum over the warps.
 
-constexpr int KEEP_THREADS = 512, KEEP_WARPS = KEEP_THREADS / 32;
+constexpr int KEEP_THREADS = 512, KEEP_WARPS = KEEP_THREADS / 32, KEEP_BINS = 2048;
+static_assert(KEEP_BINS == 4 * KEEP_THREADS, "a thread clears and adds up four bins");
 
 __device__ __forceinline__ unsigned weight_key(float w) { return w != w ? 1u : ordered(w); }      // the least number's is 0x007fffff
 
 // VPL: weights that a lane keeps in registers (0: read again every time)
 template <int VPL>
-__global__ void __launch_bounds__(KEEP_THREADS)
+__global__ void __launch_bounds__(KEEP_THREADS, VPL <= 16 ? 4 : 2)
 keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int width, int nkv, const int* __restrict__ slots,
                  const int* __restrict__ lengths, const int* __restrict__ keeps, int first, int recent, int* __restrict__ chosen, int most,
                  int max_len) {
-  __shared__ int count_of[2][KEEP_WARPS], tie_of[KEEP_WARPS];
+  __shared__ int count_of[KEEP_WARPS], place_of[KEEP_WARPS], tie_of[KEEP_WARPS];
+  __shared__ __align__(16) int bins[KEEP_BINS];
+  __shared__ unsigned least_of[KEEP_WARPS], most_of[KEEP_WARPS], left[KEEP_THREADS], found;
+  __shared__ int bin_at, bin_above, n_left;
   pdl_launch_dependents();
   pdl_wait();
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -217,51 +224,128 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
     for (int i = 0; i < VPL; ++i) v[i] = fetch(i);
   }
   auto value = [&](int i) -> unsigned { return VPL ? v[i] : fetch(i); };
-  // the largest threshold that at least `keep` values reach, bits from the top down; 1 is reached by all that are there
+  // the weight of rank `need` among those between
+  int need = keep - f_end - (len - r_begin);
   unsigned threshold = 0xffffffffu;
-  if (keep > f_end + (len - r_begin)) {
-    threshold = 0u;
-    int turn = 0;
-    for (int bit = 31; bit >= 0; --bit, turn ^= 1) {
-      const unsigned trial = threshold | (1u << bit);
-      int c = 0;
+  if (need > 0) {
+    unsigned lo = 0xffffffffu, hi = 0u;
 #pragma unroll
-      for (int i = 0; i < (VPL ? VPL : per_lane); ++i) c += (int)(value(i) >= trial);
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (lane == 0) count_of[turn][warp] = c;
-      __syncthreads();
-      int all = lane < KEEP_WARPS ? count_of[turn][lane] : 0;
-      all = __reduce_add_sync(0xffffffffu, all);
-      if (all >= keep) threshold = trial;
+    for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
+      const unsigned x = value(i);
+      if (x - 1u < 0xfffffffeu) {                                             // neither "not there" nor one that stays anyway
+        lo = min(lo, x);
+        hi = max(hi, x);
+      }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      least_of[warp] = lo;
+      most_of[warp] = hi;
     }
     __syncthreads();
-  }
-  int larger = 0, ties = 0;
+    lo = __reduce_min_sync(0xffffffffu, lane < KEEP_WARPS ? least_of[lane] : 0xffffffffu);
+    hi = __reduce_max_sync(0xffffffffu, lane < KEEP_WARPS ? most_of[lane] : 0u);
+    for (;;) {
+      const int shift = max(0, 32 - __clz(hi - lo) - 11);                     // (hi - lo) >> shift < KEEP_BINS; lo and hi are the block's
+      reinterpret_cast<int4*>(bins)[tid] = make_int4(0, 0, 0, 0);
+      if (tid == 0) n_left = 0;
+      __syncthreads();
 #pragma unroll
-  for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
-    const unsigned x = value(i);
-    larger += (int)(x > threshold);
-    ties += (int)(x == threshold);
+      for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
+        const unsigned x = value(i) - lo;
+        if (x <= hi - lo) atomicAdd(&bins[x >> shift], 1);
+      }
+      __syncthreads();
+      // a thread's four bins, counted from the top: how many weights lie above them
+      const int4 mine = reinterpret_cast<int4*>(bins)[KEEP_THREADS - 1 - tid];
+      const int here = mine.x + mine.y + mine.z + mine.w;
+      int upto = here;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += below;
+      }
+      if (lane == 31) count_of[warp] = upto;
+      __syncthreads();
+      const int before = lane < warp ? count_of[lane] : 0;
+      int above = upto - here + __reduce_add_sync(0xffffffffu, before);
+      if (above < need && need <= above + here) {                             // one thread
+        const int four[4] = {mine.w, mine.z, mine.y, mine.x};
+        int k = 0;
+        while (above + four[k] < need) above += four[k++];
+        bin_at = (KEEP_THREADS - 1 - tid) * 4 + 3 - k;
+        bin_above = above;
+      }
+      __syncthreads();
+      const int count = bins[bin_at];
+      need -= bin_above;
+      lo += (unsigned)bin_at << shift;
+      hi = shift == 0 ? lo : min(hi, lo + ((1u << shift) - 1u));
+      if (lo == hi) {
+        threshold = lo;
+        break;
+      }
+      if (count <= KEEP_THREADS) {
+#pragma unroll
+        for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
+          const unsigned x = value(i);
+          if (x - lo <= hi - lo) left[atomicAdd(&n_left, 1)] = x;
+        }
+        __syncthreads();
+        if (tid < count) {
+          const unsigned x = left[tid];
+          int more = 0, same = 0;
+          for (int k = 0; k < count; ++k) {
+            more += (int)(left[k] > x);
+            same += (int)(left[k] == x);
+          }
+          if (more < need && need <= more + same) found = x;                  // all that do have this weight
+        }
+        __syncthreads();
+        threshold = found;
+        break;
+      }
+      __syncthreads();                                                        // bins and bin_at have been read
+    }
   }
-  larger = __reduce_add_sync(0xffffffffu, larger);
-  ties = __reduce_add_sync(0xffffffffu, ties);
-  if (lane == 0) {
-    count_of[0][warp] = larger;
-    tie_of[warp] = ties;
-  }
+  // how many reach the threshold: exactly `keep` where all of that very weight stay
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < (VPL ? VPL : per_lane); ++i) reach += (int)(value(i) >= threshold);
+  reach = __reduce_add_sync(0xffffffffu, reach);
+  if (lane == 0) place_of[warp] = reach;
   __syncthreads();
-  int all_larger = lane < KEEP_WARPS ? count_of[0][lane] : 0;
-  all_larger = __reduce_add_sync(0xffffffffu, all_larger);
-  int ties_left = keep - all_larger, at = 0;
-  for (int k = 0; k < warp; ++k) {
-    at += count_of[0][k] + min(tie_of[k], max(0, ties_left));
-    ties_left -= tie_of[k];
-  }
-  ties_left = max(0, ties_left);
+  const int theirs = lane < KEEP_WARPS ? place_of[lane] : 0;
+  int at = __reduce_add_sync(0xffffffffu, lane < warp ? theirs : 0);
+  const unsigned below = (1u << lane) - 1u;
+  if (__reduce_add_sync(0xffffffffu, theirs) == keep) {
 #pragma unroll
-  for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
-    const unsigned x = value(i);
-    const unsigned below = (1u << lane) - 1u;
+    for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
+      const bool mine = value(i) >= threshold;
+      const unsigned taken = __ballot_sync(0xffffffffu, mine);
+      if (mine) out[at + __popc(taken & below)] = p0 + 32 * i;
+      at += __popc(taken);
+    }
+    return;
+  }
+  // of those of that very weight the lowest positions
+  int ties = 0;
+  for (int i = 0; i < per_lane; ++i) ties += (int)(fetch(i) == threshold);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  if (lane == 0) tie_of[warp] = ties;
+  __syncthreads();
+  int all_ties = 0, all = 0, ties_before = 0;
+  for (int k = 0; k < KEEP_WARPS; ++k) {
+    all += place_of[k];
+    all_ties += tie_of[k];
+    if (k < warp) ties_before += tie_of[k];
+  }
+  const int room = keep - (all - all_ties);                                   // for ties
+  at += min(ties_before, room) - ties_before;
+  int ties_left = max(0, room - ties_before);
+  for (int i = 0; i < per_lane; ++i) {
+    const unsigned x = fetch(i);
     const unsigned tie = __ballot_sync(0xffffffffu, x == threshold);
     const bool mine = x > threshold || (x == threshold && __popc(tie & below) < ties_left);
     const unsigned taken = __ballot_sync(0xffffffffu, mine);
@@ -275,48 +359,60 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
 //
 // A block takes the key (or value) rows of one layer, sequence and head, a batch of rows after the other: all of a batch are read before the first
 // is written.  Sources ascend and none lies before its target, so what a batch writes no later batch reads, and the move needs no copy.
+// Such a list cannot be shared by blocks, and its time is the chain of its batches (source, page, row, write), so the launch takes blocks as large
+// as let all lists run at once: a second wave of few blocks would move the last rows at the speed of their latency.  The next batch's sources
+// are asked for before this one is written, and all that a block begins with is asked for at once.
 
-constexpr int MOVE_THREADS = 256, MOVE_DEEP = 8, MOVE_MAX_UNITS = MOVE_THREADS * MOVE_DEEP;
+constexpr int MOVE_DEEP = 4, MOVE_MAX_THREADS = 1024;
 
 template <typename U>
-__device__ __forceinline__ void move_rows(const MoveArgs& a, U* pool, int units, int layer, int b, int h, const int* src, int count, int base) {
-  const int slot = a.slots[b];
-  const int tid = threadIdx.x;
-  const int rows = MOVE_THREADS * MOVE_DEEP / units;                          // of a batch (a row has at most MOVE_MAX_UNITS units)
+__device__ __forceinline__ void move_rows(const MoveArgs& a, U* pool, int units, int b, int h, const int* src) {
+  const int tid = threadIdx.x, side = blockDim.x / units, rows = side * MOVE_DEEP;      // rows that the block reads side by side, and of a batch
+  const int r0 = tid / units, u = tid - r0 * units;                            // this thread's first row of a batch, and its unit of a row
+  const bool works = r0 < side;
+  int s[MOVE_DEEP];
+#pragma unroll
+  for (int k = 0; k < MOVE_DEEP; ++k) s[k] = works && r0 + k * side < a.most ? src[r0 + k * side] : -1;
+  const int slot = a.slots[b], count = min(a.count[b], a.most), base = a.base[b];
+  const int* table = a.page_table + (long long)slot * a.table_width;
+  pool += (long long)h * LLG_PAGE * units + u;
+  const unsigned page_units = (unsigned)a.nkv * LLG_PAGE * units;
+  auto place = [&](int pos) -> U* {
+    unsigned lp = (unsigned)pos / LLG_PAGE;
+    if (lp >= (unsigned)a.ring_pages) lp %= (unsigned)a.ring_pages;
+    return pool + (long long)((unsigned)table[lp] * (unsigned long long)page_units + ((unsigned)pos % LLG_PAGE) * (unsigned)units);
+  };
   for (int j0 = 0; j0 < count; j0 += rows) {
-    const int n = min(rows, count - j0), work = n * units;
     U v[MOVE_DEEP];
-    long long to[MOVE_DEEP];
+    bool goes[MOVE_DEEP];
 #pragma unroll
     for (int k = 0; k < MOVE_DEEP; ++k) {
-      const int c = k * MOVE_THREADS + tid;
-      to[k] = -1;
-      if (c < work) {
-        const int r = c / units, u = c - r * units;
-        const int j = j0 + r, s = src[j];
-        if (s > j) {                                                          // a row that stays where it is costs nothing
-          v[k] = pool[kv_row(a.page_table, a.table_width, a.ring_pages, slot, base + s, h, a.nkv) * units + u];
-          to[k] = kv_row(a.page_table, a.table_width, a.ring_pages, slot, base + j, h, a.nkv) * units + u;
-        }
-      }
+      const int j = j0 + r0 + k * side;
+      goes[k] = works && j < count && s[k] > j;                               // a row that stays where it is costs nothing
+      if (goes[k]) v[k] = *place(base + s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < MOVE_DEEP; ++k) {
+      const int j = j0 + rows + r0 + k * side;
+      s[k] = works && j < count ? src[j] : -1;
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < MOVE_DEEP; ++k)
-      if (to[k] >= 0) pool[to[k]] = v[k];
+      if (goes[k]) *place(base + j0 + r0 + k * side) = v[k];
   }
 }
 
-__global__ void __launch_bounds__(MOVE_THREADS) move_rows_kernel(MoveArgs a) {
+__global__ void __launch_bounds__(MOVE_MAX_THREADS, 2) move_rows_kernel(MoveArgs a) {
   const int h = blockIdx.x, b = blockIdx.y;
   const int per_layer = a.pools_per_layer + (a.weights ? 1 : 0);
   const int layer = blockIdx.z / per_layer, which = blockIdx.z - layer * per_layer;
-  const int count = min(a.count[b], a.most), base = a.base[b];
   const int* src = a.source + layer * a.source_layer + b * a.source_seq + h * a.source_head;
   if (which == a.pools_per_layer) {
     // the weights of the keys that stay, moved along
+    const int count = min(a.count[b], a.most), base = a.base[b], threads = blockDim.x;
     float* w = a.weights + layer * a.weight_layer + ((long long)a.slots[b] * a.nkv + h) * a.weight_width;
-    for (int j0 = 0; j0 < count; j0 += MOVE_THREADS) {
+    for (int j0 = 0; j0 < count; j0 += threads) {
       const int j = j0 + threadIdx.x;
       const int s = j < count ? src[j] : 0;
       const bool goes = j < count && s > j && base + s < a.weight_width;
@@ -327,10 +423,10 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_rows_kernel(MoveArgs a) {
     return;
   }
   void* pool = a.pools[layer * a.pools_per_layer + which];
-  const int bytes = a.row_bytes[which];
-  if (bytes % 16 == 0) move_rows<uint4>(a, (uint4*)pool, bytes / 16, layer, b, h, src, count, base);
-  else if (bytes % 4 == 0) move_rows<unsigned>(a, (unsigned*)pool, bytes / 4, layer, b, h, src, count, base);
-  else move_rows<unsigned short>(a, (unsigned short*)pool, bytes / 2, layer, b, h, src, count, base);
+  const int bytes = which == 0 ? a.row_bytes[0] : a.row_bytes[1];
+  if (bytes % 16 == 0) move_rows<uint4>(a, (uint4*)pool, bytes / 16, b, h, src);
+  else if (bytes % 4 == 0) move_rows<unsigned>(a, (unsigned*)pool, bytes / 4, b, h, src);
+  else move_rows<unsigned short>(a, (unsigned short*)pool, bytes / 2, b, h, src);
 }
 
 }  // namespace
@@ -392,11 +488,20 @@ LLG_API int llg_move_rows(const MoveArgs* args, cudaStream_t stream) {
   const MoveArgs& a = *args;
   LLG_REQUIRE(a.n_layers >= 0 && a.n_seqs >= 0 && a.nkv > 0 && a.pools_per_layer >= 1 && a.pools_per_layer <= 2, "move: bad sizes");
   LLG_REQUIRE(a.ring_pages > 0 && a.table_width >= a.ring_pages, "move: bad cache geometry");
-  for (int i = 0; i < a.pools_per_layer; ++i)
-    LLG_REQUIRE(a.row_bytes[i] > 0 && a.row_bytes[i] % 2 == 0 && a.row_bytes[i] <= 2 * MOVE_MAX_UNITS, "move: rows of %d bytes", a.row_bytes[i]);
+  int units = 1;
+  for (int i = 0; i < a.pools_per_layer; ++i) {
+    LLG_REQUIRE(a.row_bytes[i] > 0 && a.row_bytes[i] % 2 == 0, "move: rows of %d bytes", a.row_bytes[i]);
+    const int u = a.row_bytes[i] / (a.row_bytes[i] % 16 == 0 ? 16 : a.row_bytes[i] % 4 == 0 ? 4 : 2);
+    units = u > units ? u : units;
+  }
+  LLG_REQUIRE(units <= MOVE_MAX_THREADS, "move: rows of %d and %d bytes", a.row_bytes[0], a.row_bytes[1]);
   const long long z = (long long)a.n_layers * (a.pools_per_layer + (a.weights ? 1 : 0));
   LLG_REQUIRE(a.n_seqs <= 65535 && z <= 65535, "move: %d sequences, %d layers: more than a grid takes", a.n_seqs, a.n_layers);
   if (z == 0 || a.n_seqs == 0 || a.most <= 0) return 0;
-  move_rows_kernel<<<dim3(a.nkv, a.n_seqs, (unsigned)z), MOVE_THREADS, 0, stream>>>(a);
+  // as many threads a block as let all lists run at once (2,048 threads a multiprocessor), no more than a list has work for, and a row's at least
+  const long long lists = z * a.n_seqs * a.nkv, fit = 2048LL * llg_sm_count() / lists, work = (long long)a.most * units;
+  int threads = 128;
+  while (threads < MOVE_MAX_THREADS && (threads < units || (2 * threads <= fit && threads * MOVE_DEEP < work))) threads *= 2;
+  move_rows_kernel<<<dim3(a.nkv, a.n_seqs, (unsigned)z), threads, 0, stream>>>(a);
   return llg_check_launch("move");
 }
