@@ -407,7 +407,8 @@ int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 template <int HDP, int WR, int STAGES>
 int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t stream) {
   constexpr int smem = 2 * STAGES * (HDP / 64) * TK * 128;
-  cudaError_t e = cudaFuncSetAttribute(attn_tree_mma_kernel<HDP, WR, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long allowed = 0;
+  cudaError_t e = llg_allow_smem(attn_tree_mma_kernel<HDP, WR, STAGES>, smem, allowed);
   if (e != cudaSuccess) return llg_fail("attn_tree_mma: shared memory %d: %s", smem, cudaGetErrorString(e));
   e = llg_launch(attn_tree_mma_kernel<HDP, WR, STAGES>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_mma: launch: %s", cudaGetErrorString(e));

@@ -712,7 +712,8 @@ int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cons
   constexpr int smem = (HD / 64) * (QT * BQ * 128 + (KST + VST) * TK * 128);
   static_assert(smem > 116 * 1024, "more than half a multiprocessor's: tensor memory is a block's alone");
   const int blocks = grid_blocks(a);
-  cudaError_t e = cudaFuncSetAttribute(attn_tree_tc_kernel<HD, QT, KST, VST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long allowed = 0;
+  cudaError_t e = llg_allow_smem(attn_tree_tc_kernel<HD, QT, KST, VST>, smem, allowed);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: shared memory %d: %s", smem, cudaGetErrorString(e));
   e = llg_launch(attn_tree_tc_kernel<HD, QT, KST, VST>, dim3(blocks), dim3(THREADS), (size_t)smem, stream, mk, mv, mq, a);
   if (e != cudaSuccess) return llg_fail("attn_tree_tc: launch: %s", cudaGetErrorString(e));

@@ -62,3 +62,17 @@ struct MoveArgs {
   int weight_width;
   int n_seqs, nkv, most;      // most: bound of count over the batch
 };
+
+#ifdef __CUDACC__
+// Lets a kernel have `smem` bytes of dynamic shared memory, once per device: asked for at every launch it takes a third of a microsecond of a
+// call that is bound by the host.  `done`: a static word of the caller's, one per kernel.
+template <typename K>
+static inline cudaError_t llg_allow_smem(K kernel, size_t smem, unsigned long long& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 63;
+  if (dev < 63 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+  return e;
+}
+#endif

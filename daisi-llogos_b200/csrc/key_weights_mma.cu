@@ -253,16 +253,17 @@ template <int HDP, int MT, int WR, int STAGES>
 int launch(const KeyWeightArgs& a, const CUtensorMap& mk, cudaStream_t stream) {
   constexpr int smem = STAGES * (HDP / 64) * TK * 128;
   const dim3 grid(a.splits, a.nkv, a.n_seqs);
-  auto go = [&](void (*kernel)(CUtensorMap, KeyWeightArgs)) -> int {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static unsigned long long first_allowed = 0, second_allowed = 0;
+  auto go = [&](void (*kernel)(CUtensorMap, KeyWeightArgs), unsigned long long& allowed) -> int {
+    cudaError_t e = llg_allow_smem(kernel, smem, allowed);
     if (e != cudaSuccess) return llg_fail("key_weights_mma: shared memory %d: %s", smem, cudaGetErrorString(e));
     e = llg_launch(kernel, grid, dim3(THREADS), (size_t)smem, stream, mk, a);
     if (e != cudaSuccess) return llg_fail("key_weights_mma: launch: %s", cudaGetErrorString(e));
     return llg_check_launch("key_weights_mma");
   };
-  if (go(key_weights_mma_kernel<HDP, MT, WR, STAGES, false>)) return 1;
+  if (go(key_weights_mma_kernel<HDP, MT, WR, STAGES, false>, first_allowed)) return 1;
   if constexpr (16 * MT * WR <= STORE_ROWS) return add_stored(a, stream);
-  else return go(key_weights_mma_kernel<HDP, MT, WR, STAGES, true>);
+  else return go(key_weights_mma_kernel<HDP, MT, WR, STAGES, true>, second_allowed);
 }
 
 // Rows of a group's queries: up to 16 and 32 one tile a warp, all warps along the keys or two of them; more: two tiles a warp, four along the rows.

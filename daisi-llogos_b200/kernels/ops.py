@@ -2382,40 +2382,46 @@ _sample_scratch = {}
 
 # ---- drafted trees and shortened caches -----------------------------------------------
 
-def _on_one_device(what: str, *tensors) -> None:
-    """The tensors of a call lie on the current device, whose current stream the launch goes to."""
-    dev = tensors[0].device
-    for t in tensors:
-        if t is not None and t.device != dev:
+def _pointers(what: str, specs) -> list:
+    """Addresses of a call's tensors, each ``(name, tensor, shape, dtype)`` (shape None: any).  They lie on one GPU, the current device, whose
+    current stream the launch goes to, and are contiguous.  (One pass of cheap questions: a call for one short sequence is bound by the host.)"""
+    dev = specs[0][1].get_device()
+    if dev < 0 or dev != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
+        _refuse(what, specs)
+    out = []
+    for name, t, shape, dtype in specs:
+        if (shape is not None and t.shape != shape) or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            _refuse(what, specs)
+        out.append(t.data_ptr())
+    return out
+
+
+def _refuse(what: str, specs) -> None:
+    """Says which of a call's tensors is not what it has to be: shapes and types first, then where they lie."""
+    for name, t, shape, dtype in specs:
+        if shape is not None:
+            _shape(what, name, t, shape)
+        if t.dtype != dtype:
+            raise KernelError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+    dev = specs[0][1].device
+    for name, t, _, _ in specs:
+        if t.device != dev:
             raise KernelError(f"{what}: tensors on {dev} and on {t.device}")
-    if dev.type == "cuda" and dev.index != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
-        raise KernelError(f"{what}: tensors on {dev} while cuda:{torch.cuda.current_device()} is the current device")
+    for name, t, _, _ in specs:
+        _ptr(t)
+    raise KernelError(f"{what}: tensors on {dev} while cuda:{torch.cuda.current_device()} is the current device")
 
 
-def _wide(what: str, *tensors) -> None:
+def _wide(what: str, *pointers) -> None:
     """Storage that the kernels read 16 bytes at a time."""
-    for t in tensors:
-        if t.data_ptr() % 16:
-            raise KernelError(f"{what}: a tensor of shape {tuple(t.shape)} does not start on 16 bytes")
+    for p in pointers:
+        if p & 15:
+            raise KernelError(f"{what}: storage at {p:#x} does not start on 16 bytes")
 
 
-def _shape(what: str, name: str, t: torch.Tensor, shape, dtype: Optional[torch.dtype] = None) -> None:
+def _shape(what: str, name: str, t: torch.Tensor, shape) -> None:
     if tuple(t.shape) != tuple(shape):
         raise KernelError(f"{what}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
-        raise KernelError(f"{what}: {name} is {t.dtype}, expected {dtype}")
-
-
-def _step_layout(what: str, slots, cu_tokens, len_before, page_table) -> int:
-    """Sequences of a step; the layout's tensors are int32 of one length."""
-    b = slots.numel()
-    _shape(what, "slots", slots, (b,), torch.int32)
-    _shape(what, "len_before", len_before, (b,), torch.int32)
-    if cu_tokens is not None:
-        _shape(what, "cu_tokens", cu_tokens, (b + 1,), torch.int32)
-    if page_table.dim() != 2 or page_table.dtype != torch.int32:
-        raise KernelError(f"{what}: the page table is int32 [slots, pages]")
-    return b
 
 
 USE_TC_TREE = True           # tests switch it off to reach the mma.sync kernel with many rows
@@ -2479,38 +2485,39 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
     ``plan`` (``attn_tree_plan`` for this batch shape) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left
     zero) must hold; calls that may run at the same time need their own."""
-    what = "attn_tree"
+    what, dt, i32 = "attn_tree", q.dtype, torch.int32
     n, nh, hd = q.shape
-    nkv, vd = k_pages.shape[1], v_pages.shape[3]
-    b = _step_layout(what, slots, cu_tokens, len_before, page_table)
-    if plan.key != (q.dtype, b, nh, nkv, hd, vd):
-        raise KernelError(f"attn_tree: the plan is for {plan.key}, the call for {(q.dtype, b, nh, nkv, hd, vd)}")
-    _shape(what, "k_pages", k_pages, (k_pages.shape[0], nkv, PAGE, hd), q.dtype)
-    _shape(what, "v_pages", v_pages, (k_pages.shape[0], nkv, PAGE, vd), q.dtype)
-    _shape(what, "ancestors", ancestors, (n,), torch.int64)
-    _shape(what, "out", out, (n, nh * vd), q.dtype)
+    n_pages, nkv = k_pages.shape[:2]
+    b, vd = slots.numel(), v_pages.shape[3]
+    if plan.key != (dt, b, nh, nkv, hd, vd):
+        raise KernelError(f"attn_tree: the plan is for {plan.key}, the call for {(dt, b, nh, nkv, hd, vd)}")
     if not scale > 0:
         raise KernelError("attn_tree: the softmax scale must be positive")
-    if window < 0 or not 0 < ring_pages <= page_table.shape[1]:
-        raise KernelError(f"attn_tree: window {window}, {ring_pages} ring pages in a table of {page_table.shape[1]}")
-    if window > 0 and ring_pages * PAGE < min(window + PAGE, plan.max_len):
-        raise KernelError(f"attn_tree: a ring of {ring_pages} pages does not hold a window of {window} keys and a tree")
-    if window == 0 and ring_pages * PAGE < plan.max_len:
+    if page_table.dim() != 2:
+        raise KernelError("attn_tree: the page table is int32 [slots, pages]")
+    width = page_table.shape[1]
+    if window < 0 or not 0 < ring_pages <= width:
+        raise KernelError(f"attn_tree: window {window}, {ring_pages} ring pages in a table of {width}")
+    if ring_pages * PAGE < (min(window + PAGE, plan.max_len) if window > 0 else plan.max_len):
+        if window > 0:
+            raise KernelError(f"attn_tree: a ring of {ring_pages} pages does not hold a window of {window} keys and a tree")
         raise KernelError(f"attn_tree: {ring_pages} pages do not hold {plan.max_len} positions")
-    if scratch.dtype != torch.float32 or scratch.numel() < plan.scratch_floats:
+    if scratch.dtype is not torch.float32 or scratch.numel() < plan.scratch_floats:
         raise KernelError(f"attn_tree: scratch of {scratch.numel()} {scratch.dtype}, {plan.scratch_floats} float32 needed")
-    if counters.dtype != torch.int32 or counters.numel() < plan.n_counters:
+    if counters.dtype is not i32 or counters.numel() < plan.n_counters:
         raise KernelError(f"attn_tree: {counters.numel()} counters of {counters.dtype}, {plan.n_counters} zeroed int32 needed")
-    _on_one_device(what, q, k_pages, v_pages, page_table, slots, cu_tokens, len_before, ancestors, out, scratch, counters)
     a = _TreeArgs()
-    a.q, a.k_pages, a.v_pages = _ptr(q), _ptr(k_pages), _ptr(v_pages)
-    _wide(what, q, k_pages, v_pages, out, scratch)
-    a.page_table, a.table_width, a.ring_pages = _ptr(page_table), page_table.shape[1], ring_pages
-    a.slots, a.cu_tokens, a.len_before, a.ancestors = _ptr(slots), _ptr(cu_tokens), _ptr(len_before), _ptr(ancestors)
-    a.out, a.part, a.counters = _ptr(out), _ptr(scratch), _ptr(counters)
-    a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages = b, n, plan.max_nodes, k_pages.shape[0]
+    (a.q, a.k_pages, a.v_pages, a.page_table, a.slots, a.cu_tokens, a.len_before, a.ancestors, a.out, a.part, a.counters) = p = _pointers(what, (
+        ("q", q, None, dt), ("k_pages", k_pages, (n_pages, nkv, PAGE, hd), dt), ("v_pages", v_pages, (n_pages, nkv, PAGE, vd), dt),
+        ("page_table", page_table, None, i32), ("slots", slots, (b,), i32), ("cu_tokens", cu_tokens, (b + 1,), i32),
+        ("len_before", len_before, (b,), i32), ("ancestors", ancestors, (n,), torch.int64), ("out", out, (n, nh * vd), dt),
+        ("scratch", scratch, None, torch.float32), ("counters", counters, None, i32)))
+    if (p[0] | p[1] | p[2] | p[8] | p[9]) & 15:
+        _wide(what, p[0], p[1], p[2], p[8], p[9])
+    a.table_width, a.ring_pages = width, ring_pages
+    a.n_seqs, a.n_tokens, a.max_nodes, a.n_pages = b, n, plan.max_nodes, n_pages
     a.nh, a.nkv, a.hd, a.vd, a.n_splits, a.max_len = nh, nkv, hd, vd, plan.n_splits, plan.max_len
-    a.scale, a.window = float(scale), int(window)
+    a.scale, a.window = scale, window
     if plan.kind == "tc":
         lib = _lib("attention_tree_tc")
         _check(lib, lib.llg_attn_tree_tc(byref(a), _stream()), kernels=2)
@@ -2544,34 +2551,28 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
     nodes, filled up with -1, ``n_path`` their number, and ``next_token`` what follows the last (of a tree without nodes: 0 and -1).
 
     ``scratch`` (with ``logits``): int64, ``tree_accept_scratch`` numbers, zero when first used, left zero; one call at a time."""
-    what = "tree_accept"
+    what, i32 = "tree_accept", torch.int32
     n, b = tokens.numel(), n_path.numel()
     if (logits is None) == (picked is None):
         raise KernelError("tree_accept: either logits or picked tokens")
-    _shape(what, "tokens", tokens, (n,), torch.int32)
-    _shape(what, "parents", parents, (n,), torch.int32)
-    _shape(what, "cu_tokens", cu_tokens, (b + 1,), torch.int32)
-    _shape(what, "path", path, (b, TREE_MAX_NODES), torch.int32)
-    _shape(what, "n_path", n_path, (b,), torch.int32)
-    _shape(what, "next_token", next_token, (b,), torch.int32)
     if n == 0 or b == 0:
         raise KernelError("tree_accept: no trees, or none with a node")
+    specs = (("tokens", tokens, (n,), i32), ("parents", parents, (n,), i32), ("cu_tokens", cu_tokens, (b + 1,), i32),
+             ("path", path, (b, TREE_MAX_NODES), i32), ("n_path", n_path, (b,), i32), ("next_token", next_token, (b,), i32))
     if picked is not None:
-        _shape(what, "picked", picked, (n,), torch.int32)
-        _on_one_device(what, tokens, parents, cu_tokens, path, n_path, next_token, picked)
-        ptrs = [_ptr(t) for t in (picked, tokens, parents, cu_tokens)]
+        tok, par, cu, to, count, nxt, given = _pointers(what, specs + (("picked", picked, (n,), i32),))
         lib = _lib("cache_rows")
-        _check(lib, lib.llg_tree_walk(*ptrs, b, _ptr(path), _ptr(n_path), _ptr(next_token), _stream()))
+        _check(lib, lib.llg_tree_walk(given, tok, par, cu, b, to, count, nxt, _stream()))
         return
     if logits.dim() != 2:
         raise KernelError(f"tree_accept: logits of shape {tuple(logits.shape)}, expected [nodes, vocabulary]")
-    _shape(what, "logits", logits, (n, logits.shape[1]), torch.float32)
-    if scratch is None or scratch.dtype != torch.int64 or scratch.numel() < n + b:
+    vocab = logits.shape[1]
+    if scratch is None or scratch.dtype is not torch.int64 or scratch.numel() < n + b:
         raise KernelError(f"tree_accept: needs {n + b} zeroed int64 of scratch")
-    _on_one_device(what, tokens, parents, cu_tokens, path, n_path, next_token, logits, scratch)
-    ptrs = [_ptr(t) for t in (tokens, parents, cu_tokens)]
+    tok, par, cu, to, count, nxt, rows, maxima = _pointers(what, specs + (("logits", logits, (n, vocab), torch.float32),
+                                                                          ("scratch", scratch, None, torch.int64)))
     lib = _lib("cache_rows")
-    _check(lib, lib.llg_tree_accept(_ptr(logits), logits.shape[1], *ptrs, b, n, _ptr(scratch), _ptr(path), _ptr(n_path), _ptr(next_token), _stream()))
+    _check(lib, lib.llg_tree_accept(rows, vocab, tok, par, cu, b, n, maxima, to, count, nxt, _stream()))
 
 
 USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel with bfloat16
@@ -2618,40 +2619,40 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
 
     ``plan`` (``key_weights_plan``) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left zero) must hold; calls
     that may run at the same time need their own.  A slot may be in a step once."""
-    what = "key_weights"
+    what, dt, i32 = "key_weights", q.dtype, torch.int32
     n, nh, hd = q.shape
-    nkv = k_pages.shape[1]
-    b = _step_layout(what, slots, cu_tokens, len_before, page_table)
-    if plan.key != (q.dtype, b, nh, nkv, hd) or plan.last != last:
-        raise KernelError(f"key_weights: the plan is for {plan.key} and {plan.last} queries, the call for {(q.dtype, b, nh, nkv, hd)} and {last}")
-    _shape(what, "k_pages", k_pages, (k_pages.shape[0], nkv, PAGE, hd), q.dtype)
-    if weights.dim() != 3:
+    n_pages, nkv = k_pages.shape[:2]
+    b = slots.numel()
+    if plan.key != (dt, b, nh, nkv, hd) or plan.last != last:
+        raise KernelError(f"key_weights: the plan is for {plan.key} and {plan.last} queries, the call for {(dt, b, nh, nkv, hd)} and {last}")
+    if weights.dim() != 3 or page_table.dim() != 2:
         raise KernelError(f"key_weights: weights of shape {tuple(weights.shape)}, expected [slots, heads, positions]")
-    _shape(what, "weights", weights, (page_table.shape[0], nkv, weights.shape[2]), torch.float32)
-    if plan.max_len > weights.shape[2] or plan.max_len > page_table.shape[1] * PAGE:
-        raise KernelError(f"key_weights: {plan.max_len} keys, {weights.shape[2]} weights a row and {page_table.shape[1]} pages")
+    n_slots, width = page_table.shape
+    positions = weights.shape[2]
+    if plan.max_len > positions or plan.max_len > width * PAGE:
+        raise KernelError(f"key_weights: {plan.max_len} keys, {positions} weights a row and {width} pages")
     if not scale > 0:
         raise KernelError("key_weights: the softmax scale must be positive")
-    if scratch.dtype != torch.float32 or scratch.numel() < plan.scratch_floats:
+    if scratch.dtype is not torch.float32 or scratch.numel() < plan.scratch_floats:
         raise KernelError(f"key_weights: scratch of {scratch.numel()} {scratch.dtype}, {plan.scratch_floats} float32 needed")
-    if counters.dtype != torch.int32 or counters.numel() < plan.n_counters:
+    if counters.dtype is not i32 or counters.numel() < plan.n_counters:
         raise KernelError(f"key_weights: {counters.numel()} counters of {counters.dtype}, {plan.n_counters} zeroed int32 needed")
-    _on_one_device(what, q, k_pages, page_table, slots, cu_tokens, len_before, weights, scratch, counters)
     a = _KeyWeightArgs()
-    a.q, a.k_pages = _ptr(q), _ptr(k_pages)
-    _wide(what, q, k_pages, scratch)
-    a.page_table, a.table_width = _ptr(page_table), page_table.shape[1]
-    a.slots, a.cu_tokens, a.len_before = _ptr(slots), _ptr(cu_tokens), _ptr(len_before)
-    a.weights, a.weight_width = _ptr(weights), weights.shape[2]
-    base = _ptr(scratch)
+    a.q, a.k_pages, a.page_table, a.slots, a.cu_tokens, a.len_before, a.weights, base, _ = p = _pointers(what, (
+        ("q", q, None, dt), ("k_pages", k_pages, (n_pages, nkv, PAGE, hd), dt), ("page_table", page_table, None, i32), ("slots", slots, (b,), i32),
+        ("cu_tokens", cu_tokens, (b + 1,), i32), ("len_before", len_before, (b,), i32),
+        ("weights", weights, (n_slots, nkv, positions), torch.float32), ("scratch", scratch, None, torch.float32), ("counters", counters, None, i32)))
+    if (p[0] | p[1] | base) & 15:
+        _wide(what, p[0], p[1], base)
+    a.table_width, a.weight_width = width, positions
     a.stats = base
     a.scores = base + 4 * plan.stats if plan.scores else None
     a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last = b, n, nh, nkv, hd, last
     a.splits, a.split_keys = plan.splits, plan.split_keys
-    a.scale = float(scale)
+    a.scale = scale
     if plan.kind == "mma":
         lib = _lib("key_weights_mma")
-        _check(lib, lib.llg_key_weights_mma(byref(a), k_pages.shape[0], _stream()), kernels=2)
+        _check(lib, lib.llg_key_weights_mma(byref(a), n_pages, _stream()), kernels=2)
     else:
         lib = _lib("key_weights")
         _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), _stream()), kernels=2)
@@ -2669,25 +2670,20 @@ def keep_keys(weights: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor,
     width]``; of equal ones the lower position, NaN last).  Where the first and the newest are more than ``keep`` already, the lowest of them.
     ``chosen`` (int32 ``[layers, B, nkv, most]``, most >= every ``keep``) gets the positions in ascending order; places behind ``keep[b]`` are
     left as they were.  ``max_len``: a bound on the lengths (default: the weights' width), which fewer registers serve."""
-    what = "keep_keys"
+    what, i32 = "keep_keys", torch.int32
     if weights.dim() != 4 or chosen.dim() != 4:
         raise KernelError("keep_keys: weights are [layers, slots, heads, positions], the chosen [layers, sequences, heads, most]")
     layers, n_slots, nkv, width = weights.shape
     b, most = slots.numel(), chosen.shape[3]
-    _shape(what, "weights", weights, weights.shape, torch.float32)
-    for name, t in (("slots", slots), ("lengths", lengths), ("keep", keep)):
-        _shape(what, name, t, (b,), torch.int32)
-    _shape(what, "chosen", chosen, (layers, b, nkv, most), torch.int32)
     bound = width if max_len is None else int(max_len)
     if not 0 < bound <= width:
         raise KernelError(f"keep_keys: lengths up to {bound} in rows of {width} weights")
     if first < 0 or recent < 0:
         raise KernelError(f"keep_keys: first {first} and recent {recent} must not be negative")
-    _on_one_device(what, weights, slots, lengths, keep, chosen)
-    w, s = _ptr(weights), _ptr(slots)
+    w, s, n, k, c = _pointers(what, (("weights", weights, None, torch.float32), ("slots", slots, (b,), i32), ("lengths", lengths, (b,), i32),
+                                     ("keep", keep, (b,), i32), ("chosen", chosen, (layers, b, nkv, most), i32)))
     lib = _lib("cache_rows")
-    _check(lib, lib.llg_keep_keys(w, n_slots * nkv * width, width, nkv, layers, b, s, _ptr(lengths), _ptr(keep), int(first), int(recent),
-                                  _ptr(chosen), most, bound, _stream()))
+    _check(lib, lib.llg_keep_keys(w, n_slots * nkv * width, width, nkv, layers, b, s, n, k, first, recent, c, most, bound, _stream()))
 
 
 class CacheRows:
@@ -2705,17 +2701,16 @@ class CacheRows:
             raise KernelError(f"CacheRows: pages of shape {tuple(first.shape)}, expected [pages, heads, {PAGE}, head size]")
         _dt(first)
         self.n_pages, self.nkv = first.shape[:2]
-        for t in self.k:
-            _shape(what, "a layer's key pages", t, first.shape, first.dtype)
-        for t in self.v or ():
-            _shape(what, "a layer's value pages", t, (self.n_pages, self.nkv, PAGE, self.v[0].shape[3]), first.dtype)
-        self.weights = weights
         if weights is not None:
             if weights.dim() != 4 or weights.shape[0] != len(self.k) or weights.shape[2] != self.nkv or weights.dtype != torch.float32:
                 raise KernelError(f"CacheRows: weights of shape {tuple(weights.shape)}, expected float32 [{len(self.k)}, slots, {self.nkv}, positions]")
-        _on_one_device(what, *self.k, *(self.v or ()), weights)
-        pools = [p for i in range(len(self.k)) for p in ([_ptr(self.k[i])] + ([_ptr(self.v[i])] if self.v is not None else []))]
-        _wide(what, *self.k, *(self.v or ()))
+        specs = [("a layer's key pages", t, first.shape, first.dtype) for t in self.k]
+        specs += [("a layer's value pages", t, (self.n_pages, self.nkv, PAGE, self.v[0].shape[3]), first.dtype) for t in self.v or ()]
+        addresses = _pointers(what, specs + ([("weights", weights, None, torch.float32)] if weights is not None else []))
+        _wide(what, *addresses)
+        self.weights = weights
+        n = len(self.k)
+        pools = addresses[:n] if self.v is None else [x for pair in zip(addresses[:n], addresses[n:2 * n]) for x in pair]
         self.pools = torch.tensor(pools, dtype=torch.int64, device=first.device)
         a = self.args = _MoveArgs()
         a.pools, a.n_layers, a.pools_per_layer = self.pools.data_ptr(), len(self.k), 1 if self.v is None else 2
@@ -2731,22 +2726,21 @@ class CacheRows:
         of position ``base[b] + j``, for ``j < count[b]`` (int32 ``[B]``, at most the width of ``source``).  ``source`` is int32 ``[layers or 1,
         B, heads or 1, width]``: one list for all layers or heads where that is 1.  A list ascends (each place once), so that nothing is
         needed after it was overwritten; a slot may be in a call once.  Other rows are left as they were."""
-        what = "CacheRows.move"
-        b = _step_layout(what, slots, None, base, page_table)
-        _shape(what, "count", count, (b,), torch.int32)
-        if source.dim() != 4 or source.dtype != torch.int32 or source.shape[0] not in (1, len(self.k)) or source.shape[1] != b \
-                or source.shape[2] not in (1, self.nkv):
-            raise KernelError(f"CacheRows.move: sources of shape {tuple(source.shape)} and {source.dtype}, expected int32 [1 or {len(self.k)}, {b}, "
-                              f"1 or {self.nkv}, places]")
-        if not 0 < ring_pages <= page_table.shape[1]:
-            raise KernelError(f"CacheRows.move: {ring_pages} ring pages in a table of {page_table.shape[1]}")
+        what, i32 = "CacheRows.move", torch.int32
+        b, n = slots.numel(), len(self.k)
+        shape = source.shape
+        if len(shape) != 4 or shape[0] not in (1, n) or shape[1] != b or shape[2] not in (1, self.nkv):
+            raise KernelError(f"CacheRows.move: sources of shape {tuple(shape)}, expected int32 [1 or {n}, {b}, 1 or {self.nkv}, places]")
+        if page_table.dim() != 2 or not 0 < ring_pages <= page_table.shape[1]:
+            raise KernelError(f"CacheRows.move: {ring_pages} ring pages in a page table of shape {tuple(page_table.shape)}")
         if self.weights is not None and self.weights.shape[1] != page_table.shape[0]:
             raise KernelError(f"CacheRows.move: weights of {self.weights.shape[1]} slots, a page table of {page_table.shape[0]}")
-        _on_one_device(what, self.k[0], page_table, slots, base, source, count)
         a = _MoveArgs()
         ctypes.pointer(a)[0] = self.args
-        a.page_table, a.table_width, a.ring_pages = _ptr(page_table), page_table.shape[1], ring_pages
-        a.slots, a.base, a.source, a.count = _ptr(slots), _ptr(base), _ptr(source), _ptr(count)
+        a.page_table, a.slots, a.base, a.source, a.count, _ = _pointers(what, (
+            ("page_table", page_table, None, i32), ("slots", slots, (b,), i32), ("base", base, (b,), i32), ("source", source, None, i32),
+            ("count", count, (b,), i32), ("pools", self.pools, None, torch.int64)))
+        a.table_width, a.ring_pages = page_table.shape[1], ring_pages
         width = source.shape[3]
         a.source_seq = source.shape[2] * width
         a.source_layer = b * a.source_seq if source.shape[0] > 1 else 0

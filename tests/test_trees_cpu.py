@@ -69,7 +69,7 @@ def tree_call(**change):
     (dict(scratch=torch.zeros(99)), "scratch of 99"),
     (dict(scratch=torch.zeros(100, dtype=BF16)), "scratch of 100"),
     (dict(counters=torch.zeros(3, dtype=I32)), "3 counters"),
-    (dict(page_table=torch.zeros(3, 3, dtype=I64)), "page table is int32"),
+    (dict(page_table=torch.zeros(3, 3, dtype=I64)), "page_table is"),
     (dict(slots=torch.zeros(2, device="meta", dtype=I32)), "tensors on cpu and on meta"),
 ])
 def test_attention_of_trees_refuses(change, says):
@@ -151,11 +151,12 @@ def test_cache_rows_refuse(args, says):
 
 @pytest.mark.parametrize("change,says", [
     (dict(count=torch.zeros(3, dtype=I32)), "count has shape"), (dict(source=torch.zeros(2, 2, 1, 4, dtype=I32)), "sources of shape"),
-    (dict(source=torch.zeros(1, 2, 3, 4, dtype=I32)), "sources of shape"), (dict(source=torch.zeros(1, 2, 1, 4, dtype=I64)), "sources of shape"),
-    (dict(ring_pages=0), "0 ring pages"), (dict(ring_pages=4), "4 ring pages"), (dict(base=torch.zeros(2)), "len_before is")])
+    (dict(source=torch.zeros(1, 2, 3, 4, dtype=I32)), "sources of shape"), (dict(source=torch.zeros(1, 2, 1, 4, dtype=I64)), "source is"),
+    (dict(ring_pages=0), "0 ring pages"), (dict(ring_pages=4), "4 ring pages"), (dict(base=torch.zeros(2)), "base is")])
 def test_moves_refuse(change, says):
     rows = object.__new__(ops.CacheRows)
-    rows.k, rows.v, rows.nkv, rows.weights = [torch.zeros(3, 2, 64, 8)], None, 2, None
+    rows.k, rows.v, rows.nkv, rows.weights, rows.args = [torch.zeros(3, 2, 64, 8)], None, 2, None, ops._MoveArgs()
+    rows.pools = torch.zeros(1, dtype=I64)
     given = dict(page_table=torch.zeros(3, 3, dtype=I32), ring_pages=3, slots=torch.zeros(2, dtype=I32), base=torch.zeros(2, dtype=I32),
                  source=torch.zeros(1, 2, 1, 4, dtype=I32), count=torch.zeros(2, dtype=I32))
     given.update(change)
