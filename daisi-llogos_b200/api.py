@@ -61,13 +61,13 @@ class LlogosModel:
     """A loaded model with its cache, step function, sampler and generation loop."""
 
     def __init__(self, model, *, max_context: int = 2048, max_batch: int = 8, max_tokens: Optional[int] = None,
-                 use_graphs: bool = True):
+                 use_graphs: bool = True, weigh_keys: int = 0):
         self.model = model
         self.max_batch = max_batch
         if max_tokens is None:
             max_tokens = max_batch * ((max_context + 63) // 64) * 64
         self.engine = Engine(model, max_tokens=max_tokens, max_seq_len=max_context, n_slots=max(max_batch, 1),
-                             use_graphs=use_graphs)
+                             use_graphs=use_graphs, weigh_keys=weigh_keys)
         self.sampler = DeviceSampler(model.env.ops, model.device, model.spec.vocab_size)
 
     # ---- construction --------------------------------------------------------------------
@@ -146,3 +146,15 @@ class LlogosModel:
     def step(self, entries, want=None) -> torch.Tensor:
         """See ``Engine.step``."""
         return self.engine.step(entries, want)
+
+    def step_tree(self, entries) -> torch.Tensor:
+        """Logits of every node of drafted trees; see ``Engine.step_tree``."""
+        return self.engine.step_tree(entries)
+
+    def accept_tree(self, picked: Optional[torch.Tensor] = None):
+        """Which path of each tree stays, and the token behind it; see ``Engine.accept_tree``."""
+        return self.engine.accept_tree(picked)
+
+    def evict(self, entries, **kw) -> None:
+        """Cuts sequences down to the keys of most weight (``weigh_keys`` at construction); see ``Engine.evict``."""
+        self.engine.evict(entries, **kw)

@@ -44,6 +44,7 @@ class KvView:
     unit: int
     owner: bool = True               # False: this entry reads the unit, another entry writes it
     keep_step_kv: bool = False       # the unit is read by later entries: keep this step's packed k/v
+    weights: Optional[torch.Tensor] = None       # [n_slots + 1, n_kv, positions] float32: what queries gave each key (``SequenceCache.weigh_keys``)
     shared: Dict = field(default_factory=dict)   # owner leaves {"k_new", "v_new"} here for readers
 
 
@@ -116,6 +117,14 @@ class KvGroup:
             self.v = self.k                      # one set of pages is read as keys and as values
         else:
             self.v = {u: torch.zeros(v_shape, dtype=dtype, device=device) for u in units}
+        self.weights: Optional[torch.Tensor] = None      # [units, n_slots + 1, n_kv, positions]
+        self._rows = None
+
+    def rows(self, ops):
+        """The pages of all units as rows that are moved together (``ops.CacheRows``)."""
+        if self._rows is None:
+            self._rows = ops.CacheRows([self.k[u] for u in self.units], None if self.v is self.k else [self.v[u] for u in self.units], self.weights)
+        return self._rows
 
     def pages_needed(self, length: int) -> int:
         return min(pages_for(length), self.ring_pages)
@@ -162,7 +171,7 @@ class KvGroup:
 
     def bytes(self) -> int:
         sets = list(self.k.values()) + ([] if self.v is self.k else list(self.v.values()))
-        return sum(t.numel() * t.element_size() for t in sets)
+        return sum(t.numel() * t.element_size() for t in sets) + (0 if self.weights is None else 4 * self.weights.numel())
 
 
 class SequenceCache:
@@ -254,6 +263,38 @@ class SequenceCache:
         self._longest[slot] = written
         self.slots.length[slot] = new_len
 
+    # ---- drafted tokens, and keys that are taken out -------------------------------------
+    def weigh_keys(self) -> None:
+        """Gives every key a number, what queries have given it so far (kept by the mixers, ``KvView.weights``)."""
+        for g in self.kv_groups:
+            if g.window > 0 or g.need.values_in_keys:
+                raise ValueError("key weights go with caches that keep every key, and values of their own")
+            g.weights = torch.zeros((len(g.units), self.slots.n_slots + 1, g.need.num_kv_heads, self.max_seq_len), dtype=torch.float32,
+                                    device=self.device)
+
+    def settle(self, slot: int, new_len: int, written: int) -> None:
+        """Behind a step that wrote ``written`` tokens of ``slot`` (``grow`` reserved them, ``commit`` was not called): the first ``new_len``
+        stay, the pages of the rest go back.  Unlike ``truncate`` this is always possible: at most a page's worth of tokens beyond
+        ``new_len`` was written, and a ring holds a page more than its window."""
+        self.slots.check_live(slot)
+        if not self.slots.length[slot] <= new_len <= written <= self.slots.length[slot] + PAGE:
+            raise CacheError(f"slot {slot}: {written} tokens written behind {self.slots.length[slot]}, {new_len} kept")
+        written = max(written, self._longest.get(slot, 0))
+        for g in self.kv_groups:
+            g.shrink(slot, written, new_len)
+        self._longest[slot] = written
+        self.slots.length[slot] = new_len
+
+    def shorten(self, slot: int, new_len: int) -> None:
+        """Behind the move of the keys that stay to a sequence's front (``KvGroup.rows``): it holds ``new_len`` keys, the other pages go back."""
+        self.slots.check_live(slot)
+        old = self.slots.length[slot]
+        if not 0 < new_len <= old or self.state or any(g.window > 0 for g in self.kv_groups):
+            raise CacheError(f"slot {slot}: cannot shorten {old} keys to {new_len}")
+        for g in self.kv_groups:
+            g.shrink(slot, old, new_len)
+        self.slots.length[slot] = new_len
+
     def check_room(self, growth: Sequence[Tuple[int, int]]) -> None:
         """``growth`` = (slot, tokens to add) for a whole step; raises before anything changes."""
         seen = set()
@@ -296,7 +337,7 @@ class SequenceCache:
         g = self._group_of_unit.get(unit)
         if g is not None:
             return KvView(g.k[unit], g.v[unit], g.page_table, g.ring_pages, g.window, unit, owner,
-                          keep_step_kv, shared if shared is not None else {})
+                          keep_step_kv, None if g.weights is None else g.weights[g.units.index(unit)], shared if shared is not None else {})
         if unit in self.state:
             return StateView(self.state[unit], unit, owner)
         return None

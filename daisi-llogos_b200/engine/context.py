@@ -74,6 +74,12 @@ class StepContext:
                                                   # the launches are recorded once and replayed)
     upload: Optional[Callable[[np.ndarray, torch.Tensor], None]] = None   # host int32 array -> device buffer
     extras: Dict[str, Any] = field(default_factory=dict)
+    # [N] where a token's key lies among its sequence's, in steps in which that is not its position: nodes of drafted trees (a node's
+    # position is its depth behind the cached tokens), and caches that keys were taken out of.  Only engines whose mixers all take such
+    # steps (``Mixer.placed_steps_refused``) make them.
+    cache_positions: Optional[torch.Tensor] = None
+    tree_ancestors: Optional[torch.Tensor] = None     # [N] int64: the step's tokens are nodes of trees; the bits of the nodes that each sees
+    weigh_last: int = 0                               # > 0: the last so many queries of every sequence are to be added to the cache's key weights
 
     def buffer(self, name: str, shape, dtype=None, zero: bool = False) -> torch.Tensor:
         return self.workspace.get(name, tuple(shape), dtype or self.dtype, zero)

@@ -24,6 +24,7 @@ from ..cache.slots import CacheError
 from ..cache.store import PAGE, SequenceCache
 from .context import StepContext, Workspace
 from .model import DecoderModel
+from .trees import TreeSteps
 
 
 class StepError(ValueError):
@@ -101,11 +102,13 @@ class Engine:
 
     ``max_tokens``: tokens that live sequences may hold together, each rounded up to whole pages
     of 64.  ``max_seq_len``: longest single sequence (default: the smaller of the model's
-    position limit and ``max_tokens``).  ``n_slots``: most sequences alive at once.
+    position limit and ``max_tokens``).  ``n_slots``: most sequences alive at once.  ``weigh_keys`` W > 0: the cache keeps what
+    the last W queries of every step gave each key, by which ``evict`` chooses (float32, ``max_seq_len`` numbers per layer, key/value
+    head and slot).
     """
 
     def __init__(self, model: DecoderModel, *, max_tokens: int, max_seq_len: Optional[int] = None,
-                 n_slots: Optional[int] = None, use_graphs: bool = True):
+                 n_slots: Optional[int] = None, use_graphs: bool = True, weigh_keys: int = 0):
         self.model = model
         self.device = model.device
         self.dtype = model.dtype
@@ -122,10 +125,21 @@ class Engine:
             n_slots = max(1, min(n_pages, 1024))
         self.cache = SequenceCache(model.cache_needs(), max_tokens=max_tokens, max_seq_len=max_seq_len,
                                    n_slots=n_slots, dtype=self.dtype, device=self.device)
-        model.prepare(self.cache.max_seq_len)
+        self.trees = TreeSteps(self)
+        self.weigh_keys = int(weigh_keys)
+        self._taken: Dict[int, int] = {}        # slot -> keys that ``evict`` took out of it: its tokens' positions are that much ahead of their keys' places
+        self._kept: Dict[int, int] = {}         # slot -> keys it held when that last happened
+        if self.weigh_keys < 0:
+            raise ValueError(f"weigh_keys must not be negative, got {weigh_keys}")
+        if self.weigh_keys:
+            why = self.trees.refused(shorten=True)
+            if why is not None:
+                raise ValueError(f"weigh_keys: keys cannot be taken out of this model's cache: {why}")
+            self.cache.weigh_keys()
+        model.prepare(self.cache.max_seq_len if not self.weigh_keys or model.spec.max_positions is None else model.spec.max_positions)
         # the stock blocks' launch chain in native code, where the model is made of nothing else
         self._runner = None
-        if self.device.type == "cuda":
+        if self.device.type == "cuda" and not self.weigh_keys:
             from .runner import BlockRunner
             self._runner = BlockRunner.build(model, self.cache)
             if self._runner is not None and self.cache.max_seq_len > 0:
@@ -170,27 +184,62 @@ class Engine:
     # ---- sequences -----------------------------------------------------------------------
     def open(self) -> int:
         """Starts a sequence: returns its slot (length 0)."""
-        return self.cache.acquire()
+        slot = self.cache.acquire()
+        self._taken.pop(slot, None)
+        self._kept.pop(slot, None)
+        return slot
 
     def close(self, slot: int) -> None:
         """Ends a sequence: its slot and pages go back to the free lists."""
+        self.trees.drop()
         self.cache.release(slot)
 
     def truncate(self, slot: int, length: int) -> None:
-        """Forgets a sequence's tokens from position ``length`` on; the next step continues there."""
+        """Forgets a sequence's keys from place ``length`` on; the next step continues there.  Of a sequence that keys were taken out of, only
+        tokens that came later can be forgotten."""
+        self.trees.drop()
+        if length < self._kept.get(slot, 0):
+            raise StepError(f"slot {slot}: {self._kept[slot]} keys were left by an eviction, cannot truncate to {length}")
         try:
             self.cache.truncate(slot, length)
         except CacheError as e:
             raise StepError(str(e)) from None
 
     def length(self, slot: int) -> int:
+        """Keys that the sequence holds."""
         return self.cache.length(slot)
+
+    def position(self, slot: int) -> int:
+        """The position of the sequence's next token: its length, and the keys that were taken out of it."""
+        return self.cache.length(slot) + self._taken.get(slot, 0)
+
+    # ---- drafted trees, and keys that are taken out ----------------------------------------
+    def step_tree(self, entries: Sequence[Tuple[int, Sequence[int], Sequence[int]]]) -> torch.Tensor:
+        """Runs a tree of drafted tokens for every ``(slot, tokens, parents)`` entry; returns float32 logits of all nodes, ``[nodes, vocab]``, in
+        the entries' order.  ``tokens[0]`` is the sequence's last certain token (what a decode step would be given), ``parents[0]`` -1;
+        ``parents[i] < i`` is the node that node i follows.  Up to 64 nodes a tree.  No length changes: ``accept_tree`` says which path
+        stays; another step, ``truncate`` or ``close`` forgets the trees.  The logits are valid until the next step."""
+        return self.trees.step(entries)
+
+    def accept_tree(self, picked: Optional[torch.Tensor] = None):
+        """Ends the ``step_tree`` before it: of every tree the path stays whose nodes' tokens are the ones of largest logits behind their
+        parents (of equal ones the lowest id), or ``picked[node]`` (int32 on the device, what a sampler drew for every node).  Returns per
+        entry ``(path, next)``: the nodes that stay, the first always, and the token that follows the last of them, with which the next
+        step begins."""
+        return self.trees.accept(picked)
+
+    def evict(self, entries: Sequence[Tuple[int, int]], *, first: int = 4, recent: int = 32) -> None:
+        """Cuts sequences down to ``keep`` keys each, ``(slot, keep)``: in every layer and key/value head the ``first`` and the newest
+        ``recent`` ones and those that queries gave most weight so far.  Their tokens keep their positions, and the next token takes
+        ``position(slot)``; ``length(slot)`` is ``keep``.  Needs an engine with ``weigh_keys``."""
+        self.trees.evict(entries, first, recent)
 
     def assume(self, slot: int, n_tokens: int) -> None:
         """Declares ``n_tokens`` more tokens of ``slot`` as present without running them: pages are
         reserved and the length advances, the keys and values are whatever the pages hold.  For
         measurements of a step at a given context length; results after it mean nothing."""
         growth = [(int(slot), int(n_tokens))]
+        self.trees.drop()
         try:
             self.cache.check_room(growth)
         except CacheError as e:
@@ -263,13 +312,14 @@ class Engine:
 
     def _run(self, slots, toks, counts, want, fed) -> torch.Tensor:
         growth = list(zip(slots, counts))
+        self.trees.drop()
         try:
             self.cache.check_room(growth)
         except CacheError as e:
             raise StepError(str(e)) from None
 
         len_before = [self.cache.length(s) for s in slots]
-        longest = max(lb + c for lb, c in zip(len_before, counts))
+        longest = max(lb + c + self._taken.get(s, 0) for s, lb, c in zip(slots, len_before, counts))
         limit = self.model.position_limit()
         if limit is not None and longest > limit:
             raise StepError(f"a sequence would reach {longest} tokens, the position tables hold {limit}")
@@ -310,11 +360,14 @@ class Engine:
         cu = np.zeros(b + 1, dtype=np.int32)
         np.cumsum(counts, out=cu[1:])
         token_ids = np.concatenate(toks).astype(np.int32)
-        positions = np.concatenate([np.arange(lb, lb + c, dtype=np.int32) for lb, c in zip(len_before, counts)])
+        taken = [self._taken.get(s, 0) for s in slots] if self.weigh_keys else [0] * b
+        positions = np.concatenate([np.arange(lb + t, lb + t + c, dtype=np.int32) for lb, t, c in zip(len_before, taken, counts)])
         seq_of = np.repeat(np.arange(b, dtype=np.int32), counts)
         rows = np.array([cu[i] + int(w) for i in range(b) for w in want[i]], dtype=np.int32)
         host = [token_ids, positions, seq_of, np.asarray(slots, dtype=np.int32), cu,
                 np.asarray(len_before, dtype=np.int32), rows]
+        if self.weigh_keys:
+            host.append(positions - np.repeat(np.asarray(taken, dtype=np.int32), counts))
         plan = self._apply_updates(updates, host)
         block = np.concatenate(host)
         meta = self._ensure_meta(block.size)
@@ -335,6 +388,8 @@ class Engine:
             max_len_after=max(lb + c for lb, c in zip(len_before, counts)),
             len_before_host=list(len_before), upload=self._staging.upload)
         rows_dev = take(rows.size)
+        if self.weigh_keys:
+            ctx.cache_positions, ctx.weigh_last = take(n), self.weigh_keys
         for g, off, k in plan:
             self.ops.scatter_i32(g.page_table, meta[off:off + k], meta[off + k:off + 2 * k])
         return self.model.forward(ctx, self.cache, rows_dev, self._runner)
@@ -355,7 +410,8 @@ class Engine:
         lb = np.asarray(list(len_before) + [0] * pad, dtype=np.int32)
         all_slots = np.asarray(list(slots) + [self.cache.pad_slot] * pad, dtype=np.int32)
         # layout: token_ids | positions | seq_of_token | slots | cu_tokens (b + 1) | len_before
-        host = [token_ids, lb, ar, all_slots, np.arange(b + 1, dtype=np.int32), lb]
+        at = lb + np.asarray([self._taken.get(s, 0) for s in slots] + [0] * pad, dtype=np.int32) if self.weigh_keys else lb
+        host = [token_ids, at, ar, all_slots, np.arange(b + 1, dtype=np.int32), lb]
         fixed = 6 * b + 1
         if fed is not None:
             host.append(np.asarray(fed[1], dtype=np.int32))      # source rows, right after the fixed part
@@ -384,6 +440,8 @@ class Engine:
                 cu_tokens=m[4 * b:5 * b + 1], len_before=m[5 * b + 1:6 * b + 1],
                 dtype=self.dtype, device=self.device, ops=self.ops, workspace=st.workspace,
                 max_len_after=bound)
+            if self.weigh_keys:
+                ctx.cache_positions, ctx.weigh_last = ctx.len_before, self.weigh_keys
             if self.use_graphs and st.eager_runs >= 1:
                 # the buffers exist since the eager run; record the same launches and replay them
                 graph = torch.cuda.CUDAGraph()

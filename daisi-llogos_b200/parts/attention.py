@@ -240,7 +240,59 @@ class Attention(Mixer):
             raise ValueError(f"the owner keeps (key/value heads, head size, window, value head size) = "
                              f"{theirs}, this reader expects {mine}")
 
+    def placed_steps_refused(self):
+        for there, what in ((self.conv_taps, "convolutions behind its projections"), (self.maps, "two maps"), (self.head_gate, "gates per head"),
+                            (self.softcap or self.head_mix, "capped or mixed scores"), (self.sink_kind, "sinks"),
+                            (self.mask != "window", "a mask by chunks")):
+            if there:
+                return f"its attention has {what}"
+        return None
+
     # ---- one step ------------------------------------------------------------------------
+    def _attend_placed(self, ctx, cache, prep, qkv, common, q, out) -> None:
+        """Keys and values go to ``ctx.cache_positions``, which are not the tokens' positions; then the step's attention, by its kind, and
+        where the cache weighs its keys what the newest queries gave them."""
+        ops, n = ctx.ops, q.shape[0]
+        if self.own_kv:
+            suffix = f".{cache.unit}" if cache.keep_step_kv else ""
+            k_new = ctx.buffer("attn.k_new" + suffix, (n, self.nkv, self.hd))
+            v_new = ctx.buffer("attn.v_new" + suffix, (n, self.nkv, self.vd))
+            prep(qkv, **common, k_new=k_new, v_new=v_new)
+            ops.kv_write(k_new, v_new, cache.k_pages, cache.v_pages, cache.page_table, cache.ring_pages, ctx.cache_positions, ctx.seq_of_token,
+                         ctx.slots, ctx.cu_tokens, ctx.len_before)
+            cache.shared["k_new"], cache.shared["v_new"] = k_new, v_new
+        else:
+            prep(qkv, **common)
+            k_new, v_new = cache.shared["k_new"], cache.shared["v_new"]
+        form_kw = {"form": self.form} if self.form is not None else {}
+
+        def planned(make, name, *sizes, **kw):
+            # (the same for all layers of the same sizes: worked out once a step)
+            plan = ctx.extras.get((name, *sizes))
+            if plan is None:
+                plan = ctx.extras[(name, *sizes)] = make(ctx.dtype, *sizes, **kw)
+            return (plan, ctx.buffer(f"attn.{name}", (max(1, plan.scratch_floats),), torch.float32),
+                    ctx.buffer(f"attn.{name}.counters", (max(1, plan.n_counters),), torch.int32, zero=True))
+
+        if ctx.tree_ancestors is not None:
+            plan, scratch, counters = planned(ops.attn_tree_plan, "tree", ctx.n_seqs, ctx.max_count, self.nh, self.nkv, self.hd, ctx.max_len_after,
+                                              self.vd)
+            ops.attn_tree(q, cache.k_pages, cache.v_pages, cache.page_table, cache.ring_pages, ctx.slots, ctx.cu_tokens, ctx.len_before,
+                          ctx.tree_ancestors, out, scratch, scale=self.scale, window=self.window, plan=plan, counters=counters)
+        elif ctx.decode:
+            plan, scratch, counters = planned(ops.attn_decode_plan, "decode", ctx.n_seqs, self.nh, self.nkv, self.hd, ctx.max_len_after, **form_kw)
+            ops.attn_decode(q, cache.k_pages, cache.v_pages, cache.page_table, cache.ring_pages, ctx.slots, ctx.len_before, out, scratch,
+                            scale=self.scale, window=self.window, plan=plan, counters=counters if plan.n_counters else None, **form_kw)
+        else:
+            tq = ops.prefill_tile_queries(q.dtype, self.hd, **form_kw)
+            ops.attn_prefill(q, k_new, v_new, cache.k_pages, cache.v_pages, cache.page_table, cache.ring_pages, ctx.query_tiles(tq), ctx.cu_tokens,
+                             ctx.len_before, ctx.slots, out, scale=self.scale, window=self.window, tile_queries=tq, **form_kw)
+        if ctx.weigh_last and cache.weights is not None:
+            last = min(ctx.weigh_last, ctx.max_count)
+            plan, scratch, counters = planned(ops.key_weights_plan, "weigh", ctx.n_seqs, last, self.nh, self.nkv, self.hd, ctx.max_len_after)
+            ops.key_weights(q, cache.k_pages, cache.page_table, ctx.slots, ctx.cu_tokens, ctx.len_before, cache.weights, scratch, scale=self.scale,
+                            last=last, plan=plan, counters=counters)
+
     def forward(self, x, ctx, cache, row_scale=None) -> Branch:
         ops = ctx.ops
         n = x.shape[0]
@@ -311,7 +363,9 @@ class Attention(Mixer):
                       bias=self.b_qkv, cos=rot.cos if rot else None, sin=rot.sin if rot else None,
                       rotary_dim=rot.rotary_dim if rot else 0, pairing=rot.pairing if rot else 0,
                       positions=ctx.positions, q_out=q)
-        if ctx.decode:
+        if ctx.cache_positions is not None:
+            self._attend_placed(ctx, cache, prep, qkv, common, q, out)
+        elif ctx.decode:
             if self.own_kv:
                 prep(qkv, **common, k_pages=cache.k_pages, v_pages=cache.v_pages,
                      page_table=cache.page_table, ring_pages=cache.ring_pages,

@@ -204,6 +204,11 @@ class Mixer(Part):
         """Called when the model is built for a mixer whose schedule entry reads another entry's cache
         (``cache_of``): ``need`` is what the owner keeps.  Raise ``ValueError`` if this mixer cannot read it."""
 
+    def placed_steps_refused(self) -> Optional[str]:
+        """Why this mixer cannot take a step whose tokens' keys lie elsewhere in the cache than their positions say
+        (``StepContext.cache_positions``): drafted trees, and caches that keys were taken out of.  ``None``: it can."""
+        return "it has no form for drafted trees and shortened caches"
+
 
 class FeedForward(Part):
     TAKES_ROW_SCALE = False     # as for ``Mixer``
