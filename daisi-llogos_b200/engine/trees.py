@@ -10,6 +10,7 @@ layers; lengths advance by the path, and nothing was committed before.  Tree ste
 """
 from __future__ import annotations
 
+import weakref
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -52,11 +53,17 @@ class TreeSteps:
     """The engine's tree steps and evictions."""
 
     def __init__(self, engine):
-        self.engine = engine
+        # (not a reference: an engine in a cycle is freed whenever the collector runs, and graphs that are freed while another is recorded
+        # end that recording)
+        self._engine = weakref.ref(engine)
         self.pending: Optional[_Pending] = None
         self._seen: Dict[tuple, int] = {}
         self._recorded: Dict[tuple, _Recorded] = {}
         self._accept: Dict[int, Tuple[torch.Tensor, ...]] = {}
+
+    @property
+    def engine(self):
+        return self._engine()
 
     # ---- which models take them ------------------------------------------------------------
     def refused(self, shorten: bool = False) -> Optional[str]:
@@ -68,8 +75,9 @@ class TreeSteps:
             return "it keeps no keys and values"
         for block in model.blocks:
             for part in block.parts.values():
-                if isinstance(part, Mixer):
-                    why = part.placed_steps_refused()
+                if isinstance(part, Mixer) or part.cache_need() is not None:
+                    # (a part that keeps a cache and is no Mixer says nothing: it takes none)
+                    why = getattr(part, "placed_steps_refused", lambda part=part: Mixer.placed_steps_refused(part))()
                     if why is not None:
                         return why
         if shorten:

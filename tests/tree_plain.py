@@ -122,3 +122,69 @@ def walk(tokens, parents, best):
         if not nxt:
             return path, best[path[-1]]
         path.append(nxt[0])
+
+
+class KeptModel:
+    """The dense decoder token by token in float64, with a list of keys and values per layer and key/value head that keys can be taken out of,
+    and what queries gave each key so far.  The formulas are ``plain_model``'s."""
+
+    def __init__(self, weights, cfg):
+        import plain_model as P
+        self.P, self.w, self.cfg = P, weights, cfg
+        self.nh, self.nkv = cfg["num_attention_heads"], cfg["num_key_value_heads"]
+        self.hd = cfg.get("head_dim") or cfg["hidden_size"] // self.nh
+        self.layers = cfg["num_hidden_layers"]
+        arch = cfg["architectures"][0]
+        self.qk_norm = arch == "Qwen3ForCausalLM"
+        self.bias = cfg.get("attention_bias", arch == "Qwen2ForCausalLM")
+        self.freq = P.rope_inverse_frequencies(int(self.hd * cfg.get("partial_rotary_factor", 1.0)), cfg["rope_theta"], cfg.get("rope_scaling"))
+        assert not any(P.layer_windows(cfg))
+        self.k = [[[] for _ in range(self.nkv)] for _ in range(self.layers)]
+        self.v = [[[] for _ in range(self.nkv)] for _ in range(self.layers)]
+        self.given = [[[] for _ in range(self.nkv)] for _ in range(self.layers)]
+        self.position = 0
+
+    def step(self, tokens, last):
+        """Logits of the step's tokens; its last ``last`` queries count."""
+        return torch.stack([self._token(t, i >= len(tokens) - last) for i, t in enumerate(tokens)])
+
+    def _token(self, token, counts):
+        P, cfg, w = self.P, self.cfg, self.w
+        eps = cfg["rms_norm_eps"]
+        h = P.embedding(w["model.embed_tokens.weight"], [token])
+        for i in range(self.layers):
+            p = f"model.layers.{i}."
+            x = P.rms_norm(h, w[p + "input_layernorm.weight"], eps)
+            a = p + "self_attn."
+            q, k, v = (P.linear(x, w[a + f"{n}_proj.weight"]).view(1, -1, self.hd) for n in "qkv")
+            if self.qk_norm:
+                q, k = P.per_head_rms_norm(q, w[a + "q_norm.weight"], eps), P.per_head_rms_norm(k, w[a + "k_norm.weight"], eps)
+            if self.bias:
+                q, k, v = (t + w[a + f"{n}_proj.bias"].to(F64).view(-1, self.hd) for t, n in ((q, "q"), (k, "k"), (v, "v")))
+            q, k = (P.rope_rotate(t, [self.position], self.freq, "half") for t in (q, k))
+            o = torch.empty(self.nh, self.hd, dtype=F64)
+            for kvh in range(self.nkv):
+                self.k[i][kvh].append(k[0, kvh])
+                self.v[i][kvh].append(v[0, kvh])
+                self.given[i][kvh].append(0.0)
+                keys, values = torch.stack(self.k[i][kvh]), torch.stack(self.v[i][kvh])
+                for g in range(self.nh // self.nkv):
+                    head = kvh * (self.nh // self.nkv) + g
+                    share = torch.softmax(keys @ q[0, head] / math.sqrt(self.hd), 0)
+                    o[head] = share @ values
+                    if counts:
+                        self.given[i][kvh] = [x + y for x, y in zip(self.given[i][kvh], share.tolist())]
+            h = h + P.linear(o.view(1, -1), w[a + "o_proj.weight"])
+            x = P.rms_norm(h, w[p + "post_attention_layernorm.weight"], eps)
+            m = p + "mlp."
+            h = h + P.swiglu(x, w[m + "gate_proj.weight"], w[m + "up_proj.weight"], w[m + "down_proj.weight"])
+        self.position += 1
+        x = P.rms_norm(h, w["model.norm.weight"], eps)
+        return P.linear(x, w["model.embed_tokens.weight"] if cfg.get("tie_word_embeddings") else w["lm_head.weight"])[0]
+
+    def keep(self, stays):
+        """``stays[layer][head]``: the places of the keys that stay."""
+        for lists in (self.k, self.v, self.given):
+            for i in range(self.layers):
+                for h in range(self.nkv):
+                    lists[i][h] = [lists[i][h][j] for j in stays[i][h]]
