@@ -136,6 +136,46 @@ __device__ __forceinline__ int unit_at(const Plan& p, const int* weigh, int n_se
   return nkv * p.sums[lo] + kvh * s.tiles * s.rbs + rb * s.tiles + min((unsigned)s.tiles, at);
 }
 
+// O = (first ? 0 : O corr) + P V for a tile with values that are not finite: a thread adds up its row from the row's weights in tensor memory, and
+// leaves out the keys of no weight.  (A function of its own: its registers are not the main loop's.)
+template <int HD>
+__device__ __noinline__ void add_by_hand(uint32_t p_at, uint32_t o_at, const unsigned char* values, bool first, float corr) {
+  for (int c0 = 0; c0 < HD; c0 += 16) {                                        // uniform
+    uint32_t rr[16];
+    warp_whole();
+    tmem_ld16(o_at + c0, rr);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int x = 0; x < 16; ++x) rr[x] = first ? 0u : __float_as_uint(__uint_as_float(rr[x]) * corr);
+    const unsigned char* vb = values + (c0 >> 6) * (TK * 128);
+    const int ch = (c0 & 63) >> 3;
+    for (int h = 0; h < 2; ++h) {                                              // uniform
+      uint32_t pr[16];                                                         // the weights of half of the tile's keys
+      warp_whole();
+      tmem_ld16(p_at + h * 16, pr);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const float w = __uint_as_float(e & 1 ? pr[e >> 1] & 0xffff0000u : pr[e >> 1] << 16);
+        if (w == 0.f) continue;
+        const int key = h * 32 + e;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint4 y = *reinterpret_cast<const uint4*>(vb + swz(key, ch + q));
+          const uint32_t yy[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            rr[q * 8 + 2 * z] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] << 16), __uint_as_float(rr[q * 8 + 2 * z])));
+            rr[q * 8 + 2 * z + 1] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] & 0xffff0000u), __uint_as_float(rr[q * 8 + 2 * z + 1])));
+          }
+        }
+      }
+    }
+    warp_whole();
+    tmem_st16(o_at + c0, rr);
+  }
+}
+
 // QT: tiles of queries that a row block may have (1: SPLIT alone).  KST, VST: stages of keys and of values.
 template <int HD, int QT, int KST, int VST>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -529,12 +569,10 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (pass == 1 || warp_all(fits)) break;        // uniform
         }
         l_run = l_run * corr + psum;
-        if (!by_hand) {                                  // uniform
-          warp_whole();
+        warp_whole();
 #pragma unroll
-          for (int c16 = 0; c16 < TK / 32; ++c16)        // uniform
-            tmem_st16(lane_base + (uint32_t)(c & 1) * TK + c16 * 16, reinterpret_cast<const uint32_t(&)[16]>(pk[c16 * 16]));
-        }
+        for (int c16 = 0; c16 < TK / 32; ++c16)          // uniform
+          tmem_st16(lane_base + (uint32_t)(c & 1) * TK + c16 * 16, reinterpret_cast<const uint32_t(&)[16]>(pk[c16 * 16]));
         // O += P(c-1) V(c-1) has finished: before O is touched, and at the segment's last tile (a wait by parity sees one phase back)
         const bool touch = !first && (rescale || by_hand);
         if (touch || (!first && last)) {
@@ -544,46 +582,18 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           if (!ok) break;                                // uniform
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        if (touch || by_hand) {                          // uniform
-          const unsigned char* vt = Vs + (i % VST) * KV_BYTES;
+        if (by_hand) {                                   // uniform
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          add_by_hand<HD>(lane_base + (uint32_t)(c & 1) * TK, lane_base + O_COL, Vs + (i % VST) * KV_BYTES, first, corr);
+        } else if (touch) {                              // uniform
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 16) {          // uniform
             uint32_t rr[16];
             warp_whole();
-            if (!first) {                                // uniform
-              tmem_ld16(lane_base + O_COL + c0, rr);
-              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            }
+            tmem_ld16(lane_base + O_COL + c0, rr);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int x = 0; x < 16; ++x) rr[x] = first ? 0u : __float_as_uint(__uint_as_float(rr[x]) * corr);
-            if (by_hand) {                               // uniform
-              const unsigned char* vb = vt + (c0 >> 6) * (TK * 128);
-              const int ch = (c0 & 63) >> 3;
-#pragma unroll 1
-              for (int k2 = 0; k2 < TK / 2; ++k2) {
-                uint32_t w2 = 0;
-#pragma unroll
-                for (int e = 0; e < TK / 2; ++e) w2 = e == k2 ? pk[e] : w2;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float w = __uint_as_float(e ? w2 & 0xffff0000u : w2 << 16);
-                  const int k = 2 * k2 + e;
-                  if (w != 0.f) {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                      const uint4 y = *reinterpret_cast<const uint4*>(vb + swz(k, ch + q));
-                      const uint32_t yy[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                      for (int z = 0; z < 4; ++z) {
-                        rr[q * 8 + 2 * z] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] << 16), __uint_as_float(rr[q * 8 + 2 * z])));
-                        rr[q * 8 + 2 * z + 1] = __float_as_uint(fmaf(w, __uint_as_float(yy[z] & 0xffff0000u), __uint_as_float(rr[q * 8 + 2 * z + 1])));
-                      }
-                    }
-                  }
-                }
-              }
-            }
-            warp_whole();
+            for (int x = 0; x < 16; ++x) rr[x] = __float_as_uint(__uint_as_float(rr[x]) * corr);
             tmem_st16(lane_base + O_COL + c0, rr);
           }
         }
