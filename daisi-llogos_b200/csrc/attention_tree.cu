@@ -7,12 +7,15 @@
 // (positions behind the tree are never read, a node's value that another node does not see is not multiplied by zero).
 //
 // A block takes ROWS query rows of a (sequence, key/value head) and one of n_splits equal runs of its 32-key tiles; all heads of a group and
-// all nodes share a tile's keys and values through shared memory.  Products are 4 rows x 2 keys (scores) and 4 rows x 4 elements (values) a
-// thread, so that a float read from shared memory is used two to four times; the keys' rows are padded by 16 bytes, which spreads the
-// sixteen rows that a half warp reads over all banks.  Runs that share a row block leave partial results (sums, maximum, sum of weights); the
-// block that takes the last ticket joins them in their order, so results do not depend on who comes last.
+// all nodes share a tile's keys and values through shared memory, where the next tile's arrive (cp.async) while this one's are used.  Products are 4
+// rows x 2 keys (scores) and 4 rows x 4 elements x 4 keys (values) a thread at a time, so that a float read from shared memory is used two to
+// eight times; the keys' rows are padded by 16 bytes, which spreads the sixteen rows that a half warp reads over all banks.  Runs that share
+// a row block leave partial results (sums, maximum, sum of weights); the block that takes the last ticket joins them in their order, four
+// columns of a row a thread and eight runs asked for at once, so results do not depend on who comes last.  (Without the copies ahead, a division
+// and a page look-up per 16 bytes, and a warp that joined a row run by run: three trees behind 301 to 1,999 keys, heads of 64, 149 us.)
 #include "common.cuh"
 #include "cache_args.h"
+#include "simt_tiles.cuh"
 
 LLG_API const char* llg_last_error() { return g_llg_error; }
 
@@ -21,41 +24,11 @@ namespace {
 constexpr int TK = 32;            // keys per tile (half a page)
 constexpr int THREADS = 128;
 constexpr int MAX_HD = 384;
-constexpr int PART_EXTRA = 2;     // a partial row is [vd] sums, the maximum, the sum of weights
-
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
-// Copies rows of `width` elements into shared memory as float32, zeros behind `width` up to `padded` and for rows that are not there.
-template <typename T, typename Row>
-__device__ __forceinline__ void stage(float* dst, int rows, int width, int padded, int stride, Row row) {
-  if ((width & 3) == 0) {
-    const int w4 = padded / 4;
-    for (int c = threadIdx.x; c < rows * w4; c += THREADS) {
-      const int r = c / w4, d = (c - r * w4) * 4;
-      const T* src = row(r);
-      *reinterpret_cast<float4*>(dst + r * stride + d) = (src && d < width) ? load4<T>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  } else {
-    for (int c = threadIdx.x; c < rows * padded; c += THREADS) {
-      const int r = c / padded, d = c - r * padded;
-      const T* src = row(r);
-      dst[r * stride + d] = (src && d < width) ? to_f32(src[d]) : 0.f;
-    }
-  }
-}
+constexpr int PART_EXTRA = 4;     // a partial row is [vd, filled up to 4] sums, the maximum, the sum of weights, and 2 unused
 
 // RY: rows per thread; a block's 8 rows of threads take 8 RY query rows.  VD: sums per row and thread, in steps of 64 value elements.
-template <typename T, int RY, int VD>
+// STAGES: tiles in shared memory, 2 where they fit.
+template <typename T, int RY, int VD, int STAGES>
 __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   constexpr int ROWS = 8 * RY;
   extern __shared__ __align__(16) float smem[];
@@ -67,9 +40,9 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   const int kp = (a.hd + 3) / 4 * 4, vp = (a.vd + 3) / 4 * 4;       // padded row sizes
   const int ks = kp + 4, vs = vp + 4;
   float* Qs = smem;                       // [ROWS][ks]
-  float* Ks = Qs + ROWS * ks;             // [TK][ks]
-  float* Vs = Ks + TK * ks;               // [TK][vs]
-  float* Ps = Vs + TK * vs;               // [ROWS][TK + 4]
+  float* Ks = Qs + ROWS * ks;             // [STAGES][TK][ks]
+  float* Vs = Ks + STAGES * TK * ks;      // [STAGES][TK][vs]
+  float* Ps = Vs + STAGES * TK * vs;      // [ROWS][TK + 4]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int G = a.nh / a.nkv;
   const int b = blockIdx.z, split = blockIdx.x;
@@ -90,9 +63,8 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     bits[r] = mine;
     depth[r] = __popcll(mine) - 1;
   }
-  stage<T>(Qs, ROWS, a.hd, kp, ks, [&](int r) -> const T* {
-    return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
-  });
+  for (int r = ty; r < ROWS; r += 8)
+    copy_row<T>(Qs + r * ks, r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr, a.hd, kp, tx, 16);
 
   const int lo = a.window > 0 ? max(0, lb - a.window) : 0;          // no row sees less than this (a row without any bit has depth -1)
   const int t0 = lo / TK, t_end = (total + TK - 1) / TK;
@@ -107,22 +79,31 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int e = 0; e < VD * 4; ++e) o[r][e] = 0.f;
   }
+  const TileCopy<THREADS> copy_k(kp), copy_v(vp);
+  auto request = [&](int t) {              // tile t into its stage: its keys lie in one page, one behind the other
+    if (t < t_to) {
+      const int p0 = t * TK, st = (t - t_from) % STAGES;
+      const long long row = kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0, kvh, a.nkv);
+      copy_k(Ks + st * TK * ks, ks, kg + row * a.hd, TK, total - p0, a.hd);
+      copy_v(Vs + st * TK * vs, vs, vg + row * a.vd, TK, total - p0, a.vd);
+    }
+    tile_commit();
+  };
+  if (STAGES == 2) request(t_from);
   for (int t = t_from; t < t_to; ++t) {
     const int p0 = t * TK;
+    __syncthreads();                       // the stage that is filled now has been read
+    request(STAGES == 2 ? t + 1 : t);
+    tile_wait<STAGES - 1>();
     __syncthreads();
-    stage<T>(Ks, TK, a.hd, kp, ks, [&](int r) -> const T* {
-      return p0 + r < total ? kg + kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0 + r, kvh, a.nkv) * a.hd : nullptr;
-    });
-    stage<T>(Vs, TK, a.vd, vp, vs, [&](int r) -> const T* {
-      return p0 + r < total ? vg + kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0 + r, kvh, a.nkv) * a.vd : nullptr;
-    });
-    __syncthreads();
+    const float* Kt = Ks + (t - t_from) % STAGES * TK * ks;
+    const float* Vt = Vs + (t - t_from) % STAGES * TK * vs;
     float s[RY][2];
 #pragma unroll
     for (int r = 0; r < RY; ++r) s[r][0] = s[r][1] = 0.f;
     for (int d = 0; d < kp; d += 4) {
-      const float4 k0 = *reinterpret_cast<const float4*>(Ks + tx * ks + d);
-      const float4 k1 = *reinterpret_cast<const float4*>(Ks + (tx + 16) * ks + d);
+      const float4 k0 = *reinterpret_cast<const float4*>(Kt + tx * ks + d);
+      const float4 k1 = *reinterpret_cast<const float4*>(Kt + (tx + 16) * ks + d);
 #pragma unroll
       for (int r = 0; r < RY; ++r) {
         const float4 q = *reinterpret_cast<const float4*>(Qs + (ty * RY + r) * ks + d);
@@ -163,22 +144,25 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       }
     }
     __syncwarp();                          // a row's weights come from and go to the lanes of one warp
-    for (int j = 0; j < TK; ++j) {
-      float p[RY];
+    for (int j = 0; j < TK; j += 4) {
+      float p[RY][4];
 #pragma unroll
-      for (int r = 0; r < RY; ++r) p[r] = Ps[(ty * RY + r) * (TK + 4) + j];
+      for (int r = 0; r < RY; ++r) *reinterpret_cast<float4*>(p[r]) = *reinterpret_cast<const float4*>(Ps + (ty * RY + r) * (TK + 4) + j);
 #pragma unroll
       for (int c = 0; c < VD; ++c) {
         const int d = c * 64 + tx * 4;
         if (d < vp) {
-          const float4 v = *reinterpret_cast<const float4*>(Vs + j * vs + d);
 #pragma unroll
-          for (int r = 0; r < RY; ++r) {
-            if (!mixed || p[r] != 0.f) {
-              o[r][c * 4 + 0] += p[r] * v.x;
-              o[r][c * 4 + 1] += p[r] * v.y;
-              o[r][c * 4 + 2] += p[r] * v.z;
-              o[r][c * 4 + 3] += p[r] * v.w;
+          for (int k = 0; k < 4; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(Vt + (j + k) * vs + d);
+#pragma unroll
+            for (int r = 0; r < RY; ++r) {
+              if (!mixed || p[r][k] != 0.f) {
+                o[r][c * 4 + 0] += p[r][k] * v.x;
+                o[r][c * 4 + 1] += p[r][k] * v.y;
+                o[r][c * 4 + 2] += p[r][k] * v.z;
+                o[r][c * 4 + 3] += p[r][k] * v.w;
+              }
             }
           }
         }
@@ -194,7 +178,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   T* out = (T*)a.out;
   const int slots_per_row = a.n_splits;
   const long long first_row = ((long long)b * a.nkv + kvh) * a.max_nodes * G + row0;
-  const int pw = a.vd + PART_EXTRA;
+  const int pw = vp + PART_EXTRA;
 #pragma unroll
   for (int r = 0; r < RY; ++r) {
     const int row = ty * RY + r;
@@ -210,14 +194,14 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     } else {
       float* dst = a.part + ((first_row + row) * slots_per_row + split) * pw;
       if (tx == 0) {
-        dst[a.vd] = m[r];
-        dst[a.vd + 1] = l[r];
+        dst[vp] = m[r];
+        dst[vp + 1] = l[r];
       }
       if (m[r] == -INFINITY) continue;                              // nothing seen: nobody reads the sums
 #pragma unroll
-      for (int e = 0; e < VD * 4; ++e) {
-        const int d = (e >> 2) * 64 + tx * 4 + (e & 3);
-        if (d < a.vd) dst[d] = o[r][e];
+      for (int c = 0; c < VD; ++c) {
+        const int d = c * 64 + tx * 4;
+        if (d < vp) *reinterpret_cast<float4*>(dst + d) = make_float4(o[r][4 * c], o[r][4 * c + 1], o[r][4 * c + 2], o[r][4 * c + 3]);
       }
     }
   }
@@ -233,43 +217,58 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  const int warp = tid >> 5, lane = tid & 31;
-  for (int row = warp; row < n_rows; row += THREADS / 32) {
+  const int v4 = vp / 4;
+  for (int x = tid; x < n_rows * v4; x += THREADS) {
+    const int row = x / v4, d = (x - row * v4) * 4;
     const float* src = a.part + (first_row + row) * slots_per_row * pw;
-    float M = -INFINITY;
-    for (int s = 0; s < a.n_splits; ++s) M = fmaxf(M, __ldcg(src + (long long)s * pw + a.vd));
-    float L = 0.f, acc[MAX_HD / 32];
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < a.n_splits; s0 += 8) {
+      float2 ml[8];
+      float4 v[8];
 #pragma unroll
-    for (int k = 0; k < MAX_HD / 32; ++k) acc[k] = 0.f;
-    for (int s = 0; s < a.n_splits; ++s) {
-      const float* p = src + (long long)s * pw;
-      const float ms = __ldcg(p + a.vd);
-      if (ms == -INFINITY) continue;
-      const float w = expf(ms - M);
-      L += w * __ldcg(p + a.vd + 1);
+      for (int k = 0; k < 8; ++k) {
+        const float* p = src + (long long)(s0 + k < a.n_splits ? s0 + k : 0) * pw;
+        ml[k] = s0 + k < a.n_splits ? __ldcg(reinterpret_cast<const float2*>(p + vp)) : make_float2(-INFINITY, 0.f);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p + d));
+      }
+      float top = M;
 #pragma unroll
-      for (int k = 0; k < MAX_HD / 32; ++k) {
-        const int d = lane + 32 * k;
-        if (d < a.vd) acc[k] += w * __ldcg(p + d);
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+      const float f = M == -INFINITY ? 0.f : expf(M - top);
+      M = top;
+      L *= f;
+      acc.x *= f;
+      acc.y *= f;
+      acc.z *= f;
+      acc.w *= f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (ml[k].x == -INFINITY) continue;                          // a run in which the row sees nothing has left no sums
+        const float w = expf(ml[k].x - M);
+        L += w * ml[k].y;
+        acc.x += w * v[k].x;
+        acc.y += w * v[k].y;
+        acc.z += w * v[k].z;
+        acc.w += w * v[k].w;
       }
     }
     const float inv = L != 0.f ? 1.f / L : 0.f;
-    T* dst = out + ((long long)(tok0 + (row0 + row) / G) * a.nh + kvh * G + (row0 + row) % G) * a.vd;
+    T* dst = out + ((long long)(tok0 + (row0 + row) / G) * a.nh + kvh * G + (row0 + row) % G) * a.vd + d;
+    const float four[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
-    for (int k = 0; k < MAX_HD / 32; ++k) {
-      const int d = lane + 32 * k;
-      if (d < a.vd) dst[d] = from_f32<T>(acc[k] * inv);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (d + e < a.vd) dst[e] = from_f32<T>(four[e]);
   }
 }
 
 int rows_per_block(int rows) { return rows <= 8 ? 8 : 32; }
 
-template <typename T, int RY, int VD>
+template <typename T, int RY, int VD, int STAGES>
 int launch(const TreeArgs& a, cudaStream_t stream) {
   const int kp = (a.hd + 3) / 4 * 4 + 4, vp = (a.vd + 3) / 4 * 4 + 4;
-  const size_t smem = sizeof(float) * ((size_t)(8 * RY + TK) * kp + (size_t)TK * vp + 8 * RY * (TK + 4));
-  auto kernel = attn_tree_kernel<T, RY, VD>;
+  const size_t smem = sizeof(float) * ((size_t)(8 * RY + STAGES * TK) * kp + (size_t)STAGES * TK * vp + 8 * RY * (TK + 4));
+  auto kernel = attn_tree_kernel<T, RY, VD, STAGES>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return llg_fail("attn_tree: shared memory %zu: %s", smem, cudaGetErrorString(e));
   const int G = a.nh / a.nkv, blocks = (a.max_nodes * G + 8 * RY - 1) / (8 * RY);
@@ -283,9 +282,9 @@ int launch(const TreeArgs& a, cudaStream_t stream) {
 template <typename T>
 int dispatch(const TreeArgs& a, cudaStream_t stream) {
   const bool few = rows_per_block(a.max_nodes * (a.nh / a.nkv)) == 8;
-  if (a.vd <= 64) return few ? launch<T, 1, 1>(a, stream) : launch<T, 4, 1>(a, stream);
-  if (a.vd <= 128) return few ? launch<T, 1, 2>(a, stream) : launch<T, 4, 2>(a, stream);
-  return few ? launch<T, 1, 6>(a, stream) : launch<T, 4, 6>(a, stream);
+  if (a.vd <= 64 && a.hd <= 128) return few ? launch<T, 1, 1, 2>(a, stream) : launch<T, 4, 1, 2>(a, stream);
+  if (a.vd <= 128 && a.hd <= 128) return few ? launch<T, 1, 2, 2>(a, stream) : launch<T, 4, 2, 2>(a, stream);
+  return few ? launch<T, 1, 6, 1>(a, stream) : launch<T, 4, 6, 1>(a, stream);
 }
 
 }  // namespace
@@ -295,7 +294,7 @@ LLG_API int llg_tree_max_nodes() { return LLG_TREE_NODES; }
 // Query rows that a block takes where a tree has up to `rows` of them per key/value head: there are n_seqs * nkv * ceil(rows / this) counters.
 LLG_API int llg_attn_tree_rows(int rows) { return rows_per_block(rows); }
 
-// part: [n_seqs * nkv * max_nodes * group][n_splits][vd + 2] floats where n_splits > 1.
+// part: [n_seqs * nkv * max_nodes * group][n_splits][vd filled up to 4, + 4] floats where n_splits > 1.
 LLG_API int llg_attn_tree_simt(const TreeArgs* args, int dtype, cudaStream_t stream) {
   const TreeArgs& a = *args;
   LLG_REQUIRE(a.nh > 0 && a.nkv > 0 && a.nh % a.nkv == 0, "attn_tree: %d heads are no multiple of %d key/value heads", a.nh, a.nkv);

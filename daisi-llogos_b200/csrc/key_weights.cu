@@ -14,6 +14,7 @@
 #include "common.cuh"
 #include "cache_args.h"
 #include "key_weights.cuh"
+#include "simt_tiles.cuh"
 
 LLG_API const char* llg_last_error() { return g_llg_error; }
 
@@ -21,38 +22,9 @@ namespace {
 
 constexpr int THREADS = 128, ROWS = 32, MAX_HD = 384;
 
-template <typename T>
-__device__ __forceinline__ float4 load4(const T* p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* p) {
-  const uint2 r = *reinterpret_cast<const uint2*>(p);
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
-template <typename T, typename Row>
-__device__ __forceinline__ void stage(float* dst, int rows, int width, int padded, int stride, Row row) {
-  if ((width & 3) == 0) {
-    const int w4 = padded / 4;
-    for (int c = threadIdx.x; c < rows * w4; c += THREADS) {
-      const int r = c / w4, d = (c - r * w4) * 4;
-      const T* src = row(r);
-      *reinterpret_cast<float4*>(dst + r * stride + d) = (src && d < width) ? load4<T>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  } else {
-    for (int c = threadIdx.x; c < rows * padded; c += THREADS) {
-      const int r = c / padded, d = c - r * padded;
-      const T* src = row(r);
-      dst[r * stride + d] = (src && d < width) ? to_f32(src[d]) : 0.f;
-    }
-  }
-}
-
 // A block: a split's keys of a (sequence, head), 64 at a time, ROWS rows at a time; a thread: 4 rows x 4 keys.  SECOND: the rows' ends are known.
-template <typename T, bool SECOND>
+// STAGES: tiles in shared memory, 2 where they fit: the next one's keys arrive while this one's are used.
+template <typename T, bool SECOND, int STAGES>
 __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
   constexpr int KEYS = WEIGHT_TILE, KPT = KEYS / 16;
   extern __shared__ __align__(16) float smem[];
@@ -65,18 +37,19 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
   const int first = split * a.split_keys, last = min(s.total, first + a.split_keys);
   if (first >= last || s.rows <= 0) return;
   const int kp = (a.hd + 3) / 4 * 4, ks = kp + 4;
-  float* Ks = smem;                        // [KEYS][ks]
-  float* Qs = Ks + KEYS * ks;              // [ROWS][ks]
+  float* Ks = smem;                        // [STAGES][KEYS][ks]
+  float* Qs = Ks + STAGES * KEYS * ks;     // [ROWS][ks]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const T* qg = (const T*)a.q;
   const T* kg = (const T*)a.k_pages;
   const int slot = a.slots[b], most = s.group * a.last;
   const long long pair = (long long)b * a.nkv + h;
+  const TileCopy<THREADS> copy(kp);
   for (int r0 = 0; r0 < s.rows; r0 += ROWS) {
     __syncthreads();
-    stage<T>(Qs, ROWS, a.hd, kp, ks, [&](int r) -> const T* {
-      return r0 + r < s.rows ? qg + ((long long)(s.tok0 + (r0 + r) / s.group) * a.nh + h * s.group + (r0 + r) % s.group) * a.hd : nullptr;
-    });
+    for (int r = ty; r < ROWS; r += 8)
+      copy_row<T>(Qs + r * ks, r0 + r < s.rows ? qg + ((long long)(s.tok0 + (r0 + r) / s.group) * a.nh + h * s.group + (r0 + r) % s.group) * a.hd : nullptr,
+                  a.hd, kp, tx, 16);
     if (SECOND && tid < ROWS && r0 + tid < s.rows) ends[tid] = row_end(a, pair, s, r0 + tid);
     const float sc = a.scale * WEIGHT_LOG2E;
     float m[4], l[4];                      // this thread's keys alone
@@ -87,12 +60,19 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
       l[r] = 0.f;
       pos[r] = s.pos0 + (r0 + ty * 4 + r) / s.group;
     }
+    auto request = [&](int p0) {           // a tile of keys into its stage: a page's, one behind the other
+      if (p0 < last)
+        copy(Ks + (p0 - first) / KEYS % STAGES * KEYS * ks, ks, kg + kv_row(a.page_table, a.table_width, a.table_width, slot, p0, h, a.nkv) * a.hd, KEYS,
+             s.total - p0, a.hd);
+      tile_commit();
+    };
+    if (STAGES == 2) request(first);
     for (int p0 = first; p0 < last; p0 += KEYS) {
+      __syncthreads();                     // the stage that is filled now has been read
+      request(STAGES == 2 ? p0 + KEYS : p0);
+      tile_wait<STAGES - 1>();
       __syncthreads();
-      stage<T>(Ks, KEYS, a.hd, kp, ks, [&](int r) -> const T* {
-        return p0 + r < s.total ? kg + kv_row(a.page_table, a.table_width, a.table_width, slot, p0 + r, h, a.nkv) * a.hd : nullptr;
-      });
-      __syncthreads();
+      const float* Kt = Ks + (p0 - first) / KEYS % STAGES * KEYS * ks;
       float x[4][KPT];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -104,7 +84,7 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
         for (int r = 0; r < 4; ++r) q[r] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + r) * ks + d);
 #pragma unroll
         for (int c = 0; c < KPT; ++c) {
-          const float4 k = *reinterpret_cast<const float4*>(Ks + (tx + 16 * c) * ks + d);
+          const float4 k = *reinterpret_cast<const float4*>(Kt + (tx + 16 * c) * ks + d);
 #pragma unroll
           for (int r = 0; r < 4; ++r) x[r][c] += q[r].x * k.x + q[r].y * k.y + q[r].z * k.z + q[r].w * k.w;
         }
@@ -163,20 +143,20 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
   }
 }
 
-template <typename T>
+template <typename T, int STAGES>
 int run(const KeyWeightArgs& a, cudaStream_t stream) {
   const int ks = (a.hd + 3) / 4 * 4 + 4;
-  const size_t smem = sizeof(float) * (size_t)(WEIGHT_TILE + ROWS) * ks;
+  const size_t smem = sizeof(float) * (size_t)(STAGES * WEIGHT_TILE + ROWS) * ks;
   const dim3 grid(a.splits, a.nkv, a.n_seqs);
   auto go = [&](void (*kernel)(KeyWeightArgs)) -> int {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llg_fail("key_weights: shared memory %zu: %s", smem, cudaGetErrorString(e));
     e = llg_launch(kernel, grid, dim3(THREADS), smem, stream, a);
     if (e != cudaSuccess) return llg_fail("key_weights: launch: %s", cudaGetErrorString(e));
-    return 0;
+    return llg_check_launch("key_weights");
   };
-  if (go(key_weights_kernel<T, false>)) return 1;
-  return a.scores ? add_stored(a, stream) : go(key_weights_kernel<T, true>);
+  if (go(key_weights_kernel<T, false, STAGES>)) return 1;
+  return a.scores ? add_stored(a, stream) : go(key_weights_kernel<T, true, STAGES>);
 }
 
 }  // namespace
@@ -189,7 +169,7 @@ LLG_API int llg_key_weights_simt(const KeyWeightArgs* args, int dtype, cudaStrea
   if (check(a)) return 1;
   LLG_REQUIRE(a.hd <= MAX_HD, "key_weights: heads of %d elements (1 to %d)", a.hd, MAX_HD);
   if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
-  if (dtype == LLG_F32) return run<float>(a, stream);
-  if (dtype == LLG_BF16) return run<__nv_bfloat16>(a, stream);
+  if (dtype == LLG_F32) return a.hd <= 128 ? run<float, 2>(a, stream) : run<float, 1>(a, stream);
+  if (dtype == LLG_BF16) return a.hd <= 128 ? run<__nv_bfloat16, 2>(a, stream) : run<__nv_bfloat16, 1>(a, stream);
   return llg_fail("key_weights: unknown dtype %d", dtype);
 }

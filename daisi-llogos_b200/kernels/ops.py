@@ -2468,7 +2468,8 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
     blocks = n_seqs * n_kv_heads * -(-rows // per)
     tiles = -(-max_len // 32)
     splits = max(1, min(-(-4 * sm_count() // blocks), -(-tiles // 4), 64))       # four blocks a multiprocessor, four tiles a block at least
-    return TreePlan("simt", key, splits, max_nodes, max_len, n_seqs * n_kv_heads * rows * splits * (vd + 2) if splits > 1 else 0, blocks)
+    return TreePlan("simt", key, splits, max_nodes, max_len, n_seqs * n_kv_heads * rows * splits * (-(-vd // 4) * 4 + 4) if splits > 1 else 0,
+                    blocks)
 
 
 def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, ring_pages: int, slots: torch.Tensor,
