@@ -209,14 +209,13 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
   const float* w = weights + layer * layer_stride + ((long long)slots[b] * nkv + h) * width;
   int* out = chosen + (((long long)layer * gridDim.y + b) * nkv + h) * most;
   const int f_end = min(first, len), r_begin = max(f_end, len - recent);      // [0, f_end) and [r_begin, len) stay
+  const unsigned between = r_begin - f_end;
   const int per_lane = VPL ? VPL : (len + KEEP_THREADS - 1) / KEEP_THREADS, run = per_lane * 32;
   const int p0 = warp * run + lane;                                           // this lane's positions: p0, p0 + 32, ...
   // 0: not there; positions that stay anyway are above every weight
   auto fetch = [&](int i) -> unsigned {
     const int p = p0 + 32 * i;
-    if (p >= len) return 0u;
-    if (p < f_end || p >= r_begin) return 0xffffffffu;
-    return weight_key(w[p]);
+    return (unsigned)(p - f_end) < between ? weight_key(w[p]) : p < len ? 0xffffffffu : 0u;
   };
   unsigned v[VPL ? VPL : 1];
   if (VPL) {
