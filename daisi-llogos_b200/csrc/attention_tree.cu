@@ -6,13 +6,16 @@
 // with a running maximum m and sum; a key's weight is exactly nothing where the row does not see it, whatever the key or value holds there
 // (positions behind the tree are never read, a node's value that another node does not see is not multiplied by zero).
 //
-// A block takes ROWS query rows of a (sequence, key/value head) and one of n_splits equal runs of its 32-key tiles; all heads of a group and
-// all nodes share a tile's keys and values through shared memory, where the next tile's arrive (cp.async) while this one's are used.  Products are 4
-// rows x 2 keys (scores) and 4 rows x 4 elements x 4 keys (values) a thread at a time, so that a float read from shared memory is used two to
-// eight times; the keys' rows are padded by 16 bytes, which spreads the sixteen rows that a half warp reads over all banks.  Runs that share
-// a row block leave partial results (sums, maximum, sum of weights); the block that takes the last ticket joins them in their order, four
-// columns of a row a thread and eight runs asked for at once, so results do not depend on who comes last.  (Without the copies ahead, a division
-// and a page look-up per 16 bytes, and a warp that joined a row run by run: three trees behind 301 to 1,999 keys, heads of 64, 149 us.)
+// A block takes ROWS query rows of a (sequence, key/value head) and one of up to n_splits runs of its 32-key tiles, runs of one length for all
+// sequences; all heads of a group and all nodes share a tile's keys and values through shared memory, where the next tile's arrive (cp.async)
+// while this one's are used.  Products are 4 rows x 2 keys (scores) and 4 rows x 4 elements x 4 keys (values) a thread at a time, two of them an
+// instruction, so that a float read from shared memory is used two to eight times; the keys' rows are padded by 16 bytes, which spreads the
+// sixteen rows that a half warp reads over all banks.  Runs that share a row block leave partial results (sums, maximum, sum of weights); the
+// block that takes the last ticket joins them in their order, four columns of a row a thread and sixteen runs asked for at once, so results do
+// not depend on who comes last.  What bounds it: reads of shared memory, about 500 a warp and tile, and two warps a scheduler that wait for
+// them; the join is 7 of 41 us.  Three trees of 8 to 12 nodes behind 735 to 1,878 keys, 32 heads of 64 in groups of four: 41 us (13 splits
+// of five tiles: 47; 21 of three: 40; 32 of two: 45.  One product an instruction, 13 splits: 54.  Without the copies ahead, a division and a page
+// look-up per 16 bytes, and a warp that joined a row run by run: 149).
 #include "common.cuh"
 #include "cache_args.h"
 #include "simt_tiles.cuh"
@@ -57,33 +60,43 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   const T* kg = (const T*)a.k_pages;
   const T* vg = (const T*)a.v_pages;
 
+  const int lo = a.window > 0 ? max(0, lb - a.window) : 0;          // no row sees less than this (a row without any bit has depth -1)
+  const int t0 = lo / TK, t_end = (total + TK - 1) / TK;
+  // runs of equal length for all sequences, so that short ones have fewer (the second size: of a sequence that is longer than it may be)
+  const int per = max(((a.max_len + TK - 1) / TK + a.n_splits - 1) / a.n_splits, (t_end - t0 + a.n_splits - 1) / a.n_splits);
+  const int runs = (t_end - t0 + per - 1) / per;
+  if (split >= runs) return;
+  const int t_from = t0 + split * per, t_to = min(t_end, t_from + per);
+
   for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
   for (int r = tid; r < ROWS; r += THREADS) {
     const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
     bits[r] = mine;
     depth[r] = __popcll(mine) - 1;
   }
-  for (int r = ty; r < ROWS; r += 8)
-    copy_row<T>(Qs + r * ks, r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr, a.hd, kp, tx, 16);
+  copy_rows<THREADS, T>(Qs, ks, ROWS, a.hd, kp, [&](int r) {
+    return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
+  });
 
-  const int lo = a.window > 0 ? max(0, lb - a.window) : 0;          // no row sees less than this (a row without any bit has depth -1)
-  const int t0 = lo / TK, t_end = (total + TK - 1) / TK;
-  const int per = (t_end - t0 + a.n_splits - 1) / a.n_splits;
-  const int t_from = t0 + split * per, t_to = min(t_end, t_from + per);
-
-  float m[RY], l[RY], o[RY][VD * 4];
+  float m[RY], l[RY];
+  float2 o[RY][VD * 2];
 #pragma unroll
   for (int r = 0; r < RY; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int e = 0; e < VD * 4; ++e) o[r][e] = 0.f;
+    for (int e = 0; e < VD * 2; ++e) o[r][e] = make_float2(0.f, 0.f);
   }
   const TileCopy<THREADS> copy_k(kp), copy_v(vp);
+  // the page of the tile that is asked for next is looked up a tile ahead
+  const int* table = a.page_table + (long long)slot * a.table_width;
+  auto page_of = [&](int t) { return t < t_to ? table[t / 2 % a.ring_pages] : 0; };
+  int page = page_of(t_from);
   auto request = [&](int t) {              // tile t into its stage: its keys lie in one page, one behind the other
     if (t < t_to) {
       const int p0 = t * TK, st = (t - t_from) % STAGES;
-      const long long row = kv_row(a.page_table, a.table_width, a.ring_pages, slot, p0, kvh, a.nkv);
+      const long long row = ((long long)page * a.nkv + kvh) * (2 * TK) + p0 % (2 * TK);
+      page = page_of(t + 1);
       copy_k(Ks + st * TK * ks, ks, kg + row * a.hd, TK, total - p0, a.hd);
       copy_v(Vs + st * TK * vs, vs, vg + row * a.vd, TK, total - p0, a.vd);
     }
@@ -98,18 +111,27 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     __syncthreads();
     const float* Kt = Ks + (t - t_from) % STAGES * TK * ks;
     const float* Vt = Vs + (t - t_from) % STAGES * TK * vs;
-    float s[RY][2];
+    float2 s2[RY][2];                      // elements 0, 2, ... and 1, 3, ...
 #pragma unroll
-    for (int r = 0; r < RY; ++r) s[r][0] = s[r][1] = 0.f;
+    for (int r = 0; r < RY; ++r) s2[r][0] = s2[r][1] = make_float2(0.f, 0.f);
+#pragma unroll 4
     for (int d = 0; d < kp; d += 4) {
       const float4 k0 = *reinterpret_cast<const float4*>(Kt + tx * ks + d);
       const float4 k1 = *reinterpret_cast<const float4*>(Kt + (tx + 16) * ks + d);
 #pragma unroll
       for (int r = 0; r < RY; ++r) {
         const float4 q = *reinterpret_cast<const float4*>(Qs + (ty * RY + r) * ks + d);
-        s[r][0] += q.x * k0.x + q.y * k0.y + q.z * k0.z + q.w * k0.w;
-        s[r][1] += q.x * k1.x + q.y * k1.y + q.z * k1.z + q.w * k1.w;
+        s2[r][0] = __ffma2_rn(make_float2(q.x, q.y), make_float2(k0.x, k0.y), s2[r][0]);
+        s2[r][1] = __ffma2_rn(make_float2(q.x, q.y), make_float2(k1.x, k1.y), s2[r][1]);
+        s2[r][0] = __ffma2_rn(make_float2(q.z, q.w), make_float2(k0.z, k0.w), s2[r][0]);
+        s2[r][1] = __ffma2_rn(make_float2(q.z, q.w), make_float2(k1.z, k1.w), s2[r][1]);
       }
+    }
+    float s[RY][2];
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      s[r][0] = s2[r][0].x + s2[r][0].y;
+      s[r][1] = s2[r][1].x + s2[r][1].y;
     }
     // positions that some row may not see: the tree's, those behind it, the window's edge
     const bool mixed = p0 + TK > lb || (a.window > 0 && p0 <= lb + n - a.window);
@@ -135,7 +157,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       m[r] = m_new;
       l[r] *= corr;
 #pragma unroll
-      for (int e = 0; e < VD * 4; ++e) o[r][e] *= corr;
+      for (int e = 0; e < VD * 2; ++e) o[r][e] = __fmul2_rn(o[r][e], make_float2(corr, corr));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float p = s[r][e] == -INFINITY ? 0.f : expf(s[r][e] - m_new);
@@ -144,6 +166,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       }
     }
     __syncwarp();                          // a row's weights come from and go to the lanes of one warp
+#pragma unroll 2
     for (int j = 0; j < TK; j += 4) {
       float p[RY][4];
 #pragma unroll
@@ -158,10 +181,9 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
 #pragma unroll
             for (int r = 0; r < RY; ++r) {
               if (!mixed || p[r][k] != 0.f) {
-                o[r][c * 4 + 0] += p[r][k] * v.x;
-                o[r][c * 4 + 1] += p[r][k] * v.y;
-                o[r][c * 4 + 2] += p[r][k] * v.z;
-                o[r][c * 4 + 3] += p[r][k] * v.w;
+                const float2 w = make_float2(p[r][k], p[r][k]);
+                o[r][c * 2] = __ffma2_rn(w, make_float2(v.x, v.y), o[r][c * 2]);
+                o[r][c * 2 + 1] = __ffma2_rn(w, make_float2(v.z, v.w), o[r][c * 2 + 1]);
               }
             }
           }
@@ -183,13 +205,13 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   for (int r = 0; r < RY; ++r) {
     const int row = ty * RY + r;
     if (row >= n_rows) continue;
-    if (a.n_splits == 1) {
+    if (runs == 1) {
       T* dst = out + ((long long)(tok0 + (row0 + row) / G) * a.nh + kvh * G + (row0 + row) % G) * a.vd;
       const float inv = l[r] != 0.f ? 1.f / l[r] : 0.f;
 #pragma unroll
       for (int e = 0; e < VD * 4; ++e) {
         const int d = (e >> 2) * 64 + tx * 4 + (e & 3);
-        if (d < a.vd) dst[d] = from_f32<T>(o[r][e] * inv);
+        if (d < a.vd) dst[d] = from_f32<T>((e & 1 ? o[r][e >> 1].y : o[r][e >> 1].x) * inv);
       }
     } else {
       float* dst = a.part + ((first_row + row) * slots_per_row + split) * pw;
@@ -201,40 +223,41 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
 #pragma unroll
       for (int c = 0; c < VD; ++c) {
         const int d = c * 64 + tx * 4;
-        if (d < vp) *reinterpret_cast<float4*>(dst + d) = make_float4(o[r][4 * c], o[r][4 * c + 1], o[r][4 * c + 2], o[r][4 * c + 3]);
+        if (d < vp) *reinterpret_cast<float4*>(dst + d) = make_float4(o[r][2 * c].x, o[r][2 * c].y, o[r][2 * c + 1].x, o[r][2 * c + 1].y);
       }
     }
   }
-  if (a.n_splits == 1) return;
+  if (runs == 1) return;
   __threadfence();
   __syncthreads();
   if (tid == 0) {
     int* counter = a.counters + (b * a.nkv + kvh) * row_blocks + rb;
     const int ticket = atomicAdd(counter, 1);
-    is_last = ticket == a.n_splits - 1;
+    is_last = ticket == runs - 1;
     if (is_last) *counter = 0;
   }
   __syncthreads();
   if (!is_last) return;
   __threadfence();
   const int v4 = vp / 4;
+  constexpr int DEEP = 16;                 // runs asked for at once
   for (int x = tid; x < n_rows * v4; x += THREADS) {
     const int row = x / v4, d = (x - row * v4) * 4;
     const float* src = a.part + (first_row + row) * slots_per_row * pw;
     float M = -INFINITY, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < a.n_splits; s0 += 8) {
-      float2 ml[8];
-      float4 v[8];
+    for (int s0 = 0; s0 < runs; s0 += DEEP) {
+      float2 ml[DEEP];
+      float4 v[DEEP];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float* p = src + (long long)(s0 + k < a.n_splits ? s0 + k : 0) * pw;
-        ml[k] = s0 + k < a.n_splits ? __ldcg(reinterpret_cast<const float2*>(p + vp)) : make_float2(-INFINITY, 0.f);
+      for (int k = 0; k < DEEP; ++k) {
+        const float* p = src + (long long)(s0 + k < runs ? s0 + k : 0) * pw;
+        ml[k] = s0 + k < runs ? __ldcg(reinterpret_cast<const float2*>(p + vp)) : make_float2(-INFINITY, 0.f);
         v[k] = __ldcg(reinterpret_cast<const float4*>(p + d));
       }
       float top = M;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+      for (int k = 0; k < DEEP; ++k) top = fmaxf(top, ml[k].x);
       const float f = M == -INFINITY ? 0.f : expf(M - top);
       M = top;
       L *= f;
@@ -243,7 +266,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       acc.z *= f;
       acc.w *= f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < DEEP; ++k) {
         if (ml[k].x == -INFINITY) continue;                          // a run in which the row sees nothing has left no sums
         const float w = expf(ml[k].x - M);
         L += w * ml[k].y;

@@ -47,9 +47,9 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
   const TileCopy<THREADS> copy(kp);
   for (int r0 = 0; r0 < s.rows; r0 += ROWS) {
     __syncthreads();
-    for (int r = ty; r < ROWS; r += 8)
-      copy_row<T>(Qs + r * ks, r0 + r < s.rows ? qg + ((long long)(s.tok0 + (r0 + r) / s.group) * a.nh + h * s.group + (r0 + r) % s.group) * a.hd : nullptr,
-                  a.hd, kp, tx, 16);
+    copy_rows<THREADS, T>(Qs, ks, ROWS, a.hd, kp, [&](int r) {
+      return r0 + r < s.rows ? qg + ((long long)(s.tok0 + (r0 + r) / s.group) * a.nh + h * s.group + (r0 + r) % s.group) * a.hd : nullptr;
+    });
     if (SECOND && tid < ROWS && r0 + tid < s.rows) ends[tid] = row_end(a, pair, s, r0 + tid);
     const float sc = a.scale * WEIGHT_LOG2E;
     float m[4], l[4];                      // this thread's keys alone

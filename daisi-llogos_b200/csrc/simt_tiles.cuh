@@ -53,10 +53,28 @@ __device__ __forceinline__ void tile_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void tile_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// A query row: its elements into a padded row of shared memory (a half warp per row would do; rows are few).
-template <typename T>
-__device__ __forceinline__ void copy_row(float* dst, const T* src, int width, int padded, int lane, int lanes) {
-  for (int d = lane; d < padded; d += lanes) dst[d] = src && d < width ? to_f32(src[d]) : 0.f;
+// A thread's share of `rows` query rows (`row(r)`: where row r's elements lie, null for a row of zeros): rows of whole 16 bytes go asynchronously, as above.
+template <int THREADS, typename T, typename Row>
+__device__ __forceinline__ void copy_rows(float* dst, int stride, int rows, int width, int padded, Row row) {
+  const int padded4 = padded / 4;
+  const bool wide = (width & 3) == 0;
+  for (int x = threadIdx.x; x < rows * padded4; x += THREADS) {
+    const int r = x / padded4, d = (x - r * padded4) * 4;
+    const T* src = row(r);
+    float* to = dst + r * stride + d;
+    if (wide && sizeof(T) == 4 && src) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(src + d) : "memory");
+    } else {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (src) {
+        v.x = d < width ? to_f32(src[d]) : 0.f;
+        v.y = d + 1 < width ? to_f32(src[d + 1]) : 0.f;
+        v.z = d + 2 < width ? to_f32(src[d + 2]) : 0.f;
+        v.w = d + 3 < width ? to_f32(src[d + 3]) : 0.f;
+      }
+      *reinterpret_cast<float4*>(to) = v;
+    }
+  }
 }
 
 }  // namespace

@@ -2467,7 +2467,9 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
     per = lib.llg_attn_tree_rows(rows)
     blocks = n_seqs * n_kv_heads * -(-rows // per)
     tiles = -(-max_len // 32)
-    splits = max(1, min(-(-4 * sm_count() // blocks), -(-tiles // 4), 64))       # four blocks a multiprocessor, four tiles a block at least
+    # six blocks a multiprocessor if every sequence were as long as it may be (shorter ones have fewer), three tiles a block at least
+    splits = max(1, min(-(-6 * sm_count() // blocks), -(-tiles // 3), 64))
+    splits = -(-tiles // -(-tiles // splits))
     return TreePlan("simt", key, splits, max_nodes, max_len, n_seqs * n_kv_heads * rows * splits * (-(-vd // 4) * 4 + 4) if splits > 1 else 0,
                     blocks)
 
