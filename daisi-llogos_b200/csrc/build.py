@@ -49,9 +49,10 @@ SOURCES: Dict[str, List[str]] = {
     "moe": ["moe.cu", "common.cuh", "kernel_args.h"],
     "attention_tree": ["attention_tree.cu", "simt_tiles.cuh", "common.cuh", "cache_args.h"],
     "attention_tree_mma": ["attention_tree_mma.cu", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
-    "attention_tree_tc": ["attention_tree_tc.cu", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
+    "attention_tree_tc": ["attention_tree_tc.cu", "umma_tiles.cuh", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "key_weights": ["key_weights.cu", "key_weights.cuh", "simt_tiles.cuh", "common.cuh", "cache_args.h"],
     "key_weights_mma": ["key_weights_mma.cu", "key_weights.cuh", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
+    "key_weights_tc": ["key_weights_tc.cu", "key_weights.cuh", "umma_tiles.cuh", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "cache_rows": ["cache_rows.cu", "common.cuh", "cache_args.h"],
 }
 

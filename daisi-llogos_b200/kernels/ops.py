@@ -581,6 +581,10 @@ def _load_lib(name: str):
         lib.llg_key_weights_mma.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
         lib.llg_key_weights_mma_supported.argtypes = [c_int]
         lib.llg_key_weights_mma_status.restype = c_int
+    elif name == "key_weights_tc":
+        lib.llg_key_weights_tc.argtypes = [POINTER(_KeyWeightArgs), c_int, c_void_p]
+        lib.llg_key_weights_tc_supported.argtypes = [c_int, c_int, c_int]
+        lib.llg_key_weights_tc_status.restype = c_int
     elif name == "cache_rows":
         lib.llg_tree_accept.argtypes = [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
                                         c_void_p]
@@ -2579,6 +2583,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
 
 
 USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel with bfloat16
+USE_TC_WEIGHTS = True        # and this, to reach the mma.sync kernel with more rows than have their scores stored
 
 
 class KeyWeightPlan:
@@ -2603,12 +2608,18 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
     mma = USE_MMA_WEIGHTS and dtype == torch.bfloat16 and _lib("key_weights_mma").llg_key_weights_mma_supported(head_dim)
     tile, rows = lib.llg_key_weights_tile(), n_heads // n_kv_heads * last
     tiles = -(-max_len // tile)
-    # splits of at least four tiles, as many as give every multiprocessor six blocks
-    per = max(4, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
+    kind = "mma" if mma else "simt"
+    if mma and USE_TC_WEIGHTS and _lib("key_weights_tc").llg_key_weights_tc_supported(head_dim, n_heads // n_kv_heads, last):
+        kind = "tc"
+        # pairs of tiles, at least two a split
+        per = 2 * max(2, -(-tiles * n_seqs * n_kv_heads // (2 * 3 * sm_count())))
+    else:
+        # splits of at least four tiles, as many as give every multiprocessor six blocks
+        per = max(4, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
     splits = -(-tiles // per)
     total = n_seqs * n_kv_heads * rows
     scores = total * splits * per * tile if rows <= lib.llg_key_weights_store_rows() else 0
-    return KeyWeightPlan("mma" if mma else "simt", (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, splits, per * tile,
+    return KeyWeightPlan(kind, (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, splits, per * tile,
                          -(-2 * total * splits // 4) * 4, scores)
 
 
@@ -2653,7 +2664,10 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last = b, n, nh, nkv, hd, last
     a.splits, a.split_keys = plan.splits, plan.split_keys
     a.scale = scale
-    if plan.kind == "mma":
+    if plan.kind == "tc":
+        lib = _lib("key_weights_tc")
+        _check(lib, lib.llg_key_weights_tc(byref(a), n_pages, _stream()), kernels=2)
+    elif plan.kind == "mma":
         lib = _lib("key_weights_mma")
         _check(lib, lib.llg_key_weights_mma(byref(a), n_pages, _stream()), kernels=2)
     else:
@@ -2662,8 +2676,8 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
 
 
 def key_weights_status() -> int:
-    """Error code that the tensor-core kernel that weighs keys recorded when a wait ran out (0 = none); synchronises."""
-    return _lib("key_weights_mma").llg_key_weights_mma_status()
+    """Error code that the tensor-core kernels that weigh keys recorded when a wait ran out (0 = none); synchronises."""
+    return _lib("key_weights_tc").llg_key_weights_tc_status() or _lib("key_weights_mma").llg_key_weights_mma_status()
 
 
 def keep_keys(weights: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor, keep: torch.Tensor, chosen: torch.Tensor, *, first: int,

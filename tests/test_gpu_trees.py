@@ -437,6 +437,18 @@ def test_bfloat16_weights_on_the_cuda_cores(ops, hd, monkeypatch):
     test_weights_of_keys(ops, BF16, 8, 2, hd, [5, 0, 64], [1, 200, 64], 8)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_weights_of_many_queries_on_mma_sync(ops, hd, monkeypatch):
+    monkeypatch.setattr(ops, "USE_TC_WEIGHTS", False)
+    test_weights_of_keys(ops, BF16, 8, 2, hd, [5, 0, 64], [1, 200, 64], 20)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,last", [(8, 2, 128, 64), (5, 1, 64, 40), (40, 8, 128, 9), (33, 1, 64, 1), (128, 1, 128, 2)], ids=str)
+def test_weights_of_many_queries(ops, nh, nkv, hd, last):
+    """More rows than one row block of 128, splits of several pairs of pages that end in a page, in one key and in a whole pair."""
+    test_weights_of_keys(ops, BF16, nh, nkv, hd, [700, 0, 1023, 320], [1, 1153, 1, 64], last)
+
+
 def test_weights_of_long_sequences_in_a_graph(ops):
     """Thousands of keys: many blocks' sums are joined; every query's shares add up to one."""
     nh, nkv, hd, before = 8, 2, 128, [3900, 100]

@@ -28,10 +28,11 @@ def _fields(text, name):
     return P._c_struct(text.replace("void* const* pools", "void* pools"), name, {})
 
 
-def test_the_warp_is_whole_where_tensor_memory_wants_it():
-    with open(os.path.join(P.CSRC, "attention_tree_tc.cu")) as f:
+@pytest.mark.parametrize("source,least", [("attention_tree_tc.cu", 8), ("key_weights_tc.cu", 4)])
+def test_the_warp_is_whole_where_tensor_memory_wants_it(source, least):
+    with open(os.path.join(P.CSRC, source)) as f:
         found = W.lines_that_want_the_warp(f.read())
-    assert len(found) >= 8, found
+    assert len(found) >= least, found
     assert not [x for x in found if not x[2]]
 
 
