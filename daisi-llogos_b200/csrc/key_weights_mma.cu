@@ -6,8 +6,8 @@
 // elements); several blocks share a multiprocessor, so that one's copies run beside another's products.  A thread keeps the maximum and sum
 // of its own keys only, and lanes and warps meet at the split's end: no exchange per tile.  The second pass over many rows adds a key's
 // shares up over the rows: in a thread, over the eight lanes that hold the key's other rows by halves (7 exchanges for 8 keys), over
-// the warps in shared memory.  (With the keys as rows and every row's maximum and sum exchanged per 32 keys, and the splits joined by the last block: a decode step of
-// eight sequences of 8,190 keys 51 us; now 33.)  Heads of 64 and 128 with more than 32 rows go to key_weights_tc.cu.
+// the warps in shared memory.  (With the keys as rows and every row's maximum and sum exchanged per 32 keys, and the splits joined by the last
+// block: a decode step of eight sequences of 8,190 keys 51 us; now 33.)  Heads of 64 and 128 with more than 32 rows go to key_weights_tc.cu.
 //
 // Waits are bounded (llg_key_weights_mma_status).  No load uses cluster multicast.
 #include "tree_tiles.cuh"

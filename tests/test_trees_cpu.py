@@ -28,7 +28,7 @@ def _fields(text, name):
     return P._c_struct(text.replace("void* const* pools", "void* pools"), name, {})
 
 
-@pytest.mark.parametrize("source,least", [("attention_tree_tc.cu", 8), ("key_weights_tc.cu", 4)])
+@pytest.mark.parametrize("source,least", [("attention_tree_tc.cu", 8), ("key_weights_tc.cu", 3)])
 def test_the_warp_is_whole_where_tensor_memory_wants_it(source, least):
     with open(os.path.join(P.CSRC, source)) as f:
         found = W.lines_that_want_the_warp(f.read())
