@@ -206,35 +206,34 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
   const int h = blockIdx.x, b = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int len = min(lengths[b], max_len), keep = min(min(keeps[b], len), most);
   if (keep <= 0) return;
-  const float* w = weights + layer * layer_stride + ((long long)slots[b] * nkv + h) * width;
   int* out = chosen + (((long long)layer * gridDim.y + b) * nkv + h) * most;
   const int f_end = min(first, len), r_begin = max(f_end, len - recent);      // [0, f_end) and [r_begin, len) stay
-  const unsigned between = r_begin - f_end;
-  const int per_lane = VPL ? VPL : (len + KEEP_THREADS - 1) / KEEP_THREADS, run = per_lane * 32;
-  const int p0 = warp * run + lane;                                           // this lane's positions: p0, p0 + 32, ...
-  // 0: not there; positions that stay anyway are above every weight
-  auto fetch = [&](int i) -> unsigned {
-    const int p = p0 + 32 * i;
-    return (unsigned)(p - f_end) < between ? weight_key(w[p]) : p < len ? 0xffffffffu : 0u;
-  };
+  const int between = r_begin - f_end;
+  int need = keep - f_end - (len - r_begin);                                  // of those between
+  for (int j = tid; j < min(f_end, keep); j += KEEP_THREADS) out[j] = j;
+  for (int j = max(0, need) + f_end + tid; j < keep; j += KEEP_THREADS) out[j] = r_begin + j - f_end - max(0, need);
+  if (need <= 0) return;
+  const float* w = weights + layer * layer_stride + ((long long)slots[b] * nkv + h) * width + f_end;
+  out += f_end;
+  const int per_lane = VPL ? VPL : (between + KEEP_THREADS - 1) / KEEP_THREADS, run = per_lane * 32;
+  const int p0 = warp * run + lane;                                           // this lane's positions between: p0, p0 + 32, ...
+  auto fetch = [&](int i) -> unsigned { return p0 + 32 * i < between ? weight_key(w[p0 + 32 * i]) : 0u; };      // 0: not there
   unsigned v[VPL ? VPL : 1];
   if (VPL) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) v[i] = fetch(i);
   }
   auto value = [&](int i) -> unsigned { return VPL ? v[i] : fetch(i); };
-  // the weight of rank `need` among those between
-  int need = keep - f_end - (len - r_begin);
-  unsigned threshold = 0xffffffffu;
-  if (need > 0) {
-    unsigned lo = 0xffffffffu, hi = 0u;
+  const int all_needed = need;
+  // the weight of rank `need`
+  unsigned threshold = 1u;
+  if (need < between) {
+    unsigned lo = 0xffffffffu, hi = 0u;                                       // (the least less one)
 #pragma unroll
     for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
       const unsigned x = value(i);
-      if (x - 1u < 0xfffffffeu) {                                             // neither "not there" nor one that stays anyway
-        lo = min(lo, x);
-        hi = max(hi, x);
-      }
+      lo = min(lo, x - 1u);                                                   // (what is not there: the largest number)
+      hi = max(hi, x);
     }
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
@@ -243,7 +242,7 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
       most_of[warp] = hi;
     }
     __syncthreads();
-    lo = __reduce_min_sync(0xffffffffu, lane < KEEP_WARPS ? least_of[lane] : 0xffffffffu);
+    lo = __reduce_min_sync(0xffffffffu, lane < KEEP_WARPS ? least_of[lane] : 0xffffffffu) + 1u;
     hi = __reduce_max_sync(0xffffffffu, lane < KEEP_WARPS ? most_of[lane] : 0u);
     for (;;) {
       const int shift = max(0, 32 - __clz(hi - lo) - 11);                     // (hi - lo) >> shift < KEEP_BINS; lo and hi are the block's
@@ -308,7 +307,7 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
       __syncthreads();                                                        // bins and bin_at have been read
     }
   }
-  // how many reach the threshold: exactly `keep` where all of that very weight stay
+  // how many reach the threshold: exactly as many as are needed where all of that very weight stay
   int reach = 0;
 #pragma unroll
   for (int i = 0; i < (VPL ? VPL : per_lane); ++i) reach += (int)(value(i) >= threshold);
@@ -318,12 +317,12 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
   const int theirs = lane < KEEP_WARPS ? place_of[lane] : 0;
   int at = __reduce_add_sync(0xffffffffu, lane < warp ? theirs : 0);
   const unsigned below = (1u << lane) - 1u;
-  if (__reduce_add_sync(0xffffffffu, theirs) == keep) {
+  if (__reduce_add_sync(0xffffffffu, theirs) == all_needed) {
 #pragma unroll
     for (int i = 0; i < (VPL ? VPL : per_lane); ++i) {
       const bool mine = value(i) >= threshold;
       const unsigned taken = __ballot_sync(0xffffffffu, mine);
-      if (mine) out[at + __popc(taken & below)] = p0 + 32 * i;
+      if (mine) out[at + __popc(taken & below)] = f_end + p0 + 32 * i;
       at += __popc(taken);
     }
     return;
@@ -340,7 +339,7 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
     all_ties += tie_of[k];
     if (k < warp) ties_before += tie_of[k];
   }
-  const int room = keep - (all - all_ties);                                   // for ties
+  const int room = all_needed - (all - all_ties);                             // for ties
   at += min(ties_before, room) - ties_before;
   int ties_left = max(0, room - ties_before);
   for (int i = 0; i < per_lane; ++i) {
@@ -348,7 +347,7 @@ keep_keys_kernel(const float* __restrict__ weights, long long layer_stride, int 
     const unsigned tie = __ballot_sync(0xffffffffu, x == threshold);
     const bool mine = x > threshold || (x == threshold && __popc(tie & below) < ties_left);
     const unsigned taken = __ballot_sync(0xffffffffu, mine);
-    if (mine) out[at + __popc(taken & below)] = p0 + 32 * i;
+    if (mine) out[at + __popc(taken & below)] = f_end + p0 + 32 * i;
     at += __popc(taken);
     ties_left = max(0, ties_left - __popc(tie));
   }
