@@ -10,9 +10,10 @@
 // memory each), so that one's first copies run beside another's exponentials.
 //
 // What bounds it: a pair of pages is 2,500 to 2,700 cycles of a warp's reads of tensor memory, exponentials and sums, two warps a scheduler, and a
-// pass 3 us until its first scores are there.  Four prompts of 2,199 to 6,454 tokens, 32 queries, 32 heads of 128 in groups of four: 27 us (on
-// mma.sync 55); splits of 4, 6, 8, 10 and 12 pages: 33, 32, 27, 29, 32; scores in registers 64 at a time: 39; a quarter or half of the
-// exponentials as polynomials on the pipe of the products: 30 and 31, where without it were 30.
+// pass 3 us until its first scores are there, of which the second hides the most: its blocks copy and multiply while the first pass ends.  Four
+// prompts of 2,199 to 6,454 tokens, 32 queries, 32 heads of 128 in groups of four: 25 us (on mma.sync 55; the second pass waiting for the
+// first with all it does 27, and with splits of 4, 6, 8, 10 and 12 pages then 33, 32, 27, 29, 32).  Scores in registers 64 at a time, where 32
+// took 30: 39; a quarter or half of the exponentials as polynomials on the pipe of the products, the same: 30 and 31.
 //
 // Every wait is bounded (llg_key_weights_tc_status); a role that gives up tells the others, and the warps of exponentials go on without waiting, so that
 // all come to the end, where tensor memory is freed.  No load uses cluster multicast.
@@ -58,12 +59,14 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (tid == 0) atomicCAS(&g_error, 0, 3);
     return;
   }
-  pdl_wait();
+  // The first pass's blocks let the second's start when they have waited for all that was launched before and have their tensor memory, so what the
+  // second reads of the step's tensors is there without a wait; it waits for the first pass's sums alone.
+  if (!SECOND) pdl_wait();
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const Rows s = rows_of(a, b);
   const int first = split * a.split_keys, last = min(s.total, first + a.split_keys);
   if (first >= last || s.rows <= 0) return;  // uniform over the block
-  if (warp == ISSUE_WARP) {                  // (behind pdl_wait: a block must not take tensor memory ahead of the kernel before and then wait for it)
+  if (warp == ISSUE_WARP) {                  // (not ahead of blocks of a kernel before that have yet to take theirs, and then wait for them)
     warp_whole();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
                  "r"((uint32_t)TMEM_COLS)
@@ -202,6 +205,7 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
       const int pos = s.pos0 + row / s.group;
       float m = -INFINITY, l = 0.f;
       if (SECOND) {
+        if (rb == 0) pdl_wait();
         asm volatile("bar.sync 1, 128;" ::: "memory");      // the row block before has been read
         if (tid < LANES) {
           float2 end = live ? row_end(a, pair_at, s, row) : make_float2(0.f, 0.f);
