@@ -1,8 +1,10 @@
 // Attention of trees of drafted tokens over the paged cache, bfloat16, head sizes in steps of 8 up to 128 for keys and values, on mma.sync
 // (m16n8k16, float32 accumulation).  What a node sees is said in cache_args.h, the formula in attention_tree.cu.
 //
-// The kernel streams the cache: with R query rows (nodes x heads of a group) a key's and a value's 4 hd bytes take 4 R hd flops, so up to 64
-// rows the memory system decides the time and mma.sync keeps up beside it; more rows of head size 64 or 128 go to attention_tree_tc.cu.
+// The kernel streams the cache: with R query rows (nodes x heads of a group) a key's and a value's 4 hd bytes take 4 R hd flops, so up to 16 rows
+// of heads of 128, 32 of heads of 64, the memory system decides the time and mma.sync keeps up beside it (eight sequences of 8,190 keys, heads of
+// 128, 16 rows: 59 us, 69 % of the copy bandwidth); more go to attention_tree_tc.cu, heads of other sizes stay.  One tree of 8 nodes behind
+// 611 keys, 32 heads of 64 in groups of four: 11 us, the latency of two kernels.
 //
 //   copies     A fifth warp brings every key and value tile (one cache page of one key/value head) with TMA boxes of 64 x 64 elements into a
 //              ring of stages handed over by mbarriers; head sizes that are no multiple of 64 are filled up with zeros by the boxes.

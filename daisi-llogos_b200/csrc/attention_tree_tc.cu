@@ -1,14 +1,16 @@
 // Attention of large trees of drafted tokens over the paged cache on the 5th-generation tensor cores (tcgen05), bfloat16, head sizes 64 and 128.
 // What a node sees is said in cache_args.h, the formula in attention_tree.cu.
 //
-// With more than 64 query rows (nodes x heads of a group) mma.sync is what takes the time, not the cache.  Here 128 rows are the lanes of tensor
-// memory, and a block's two groups of four softmax warps each have scores S[128 x 64] (two buffers) and an accumulator O[128 x head] of their own
-// there, a lane that issues their products, and two copying warps for both.  Thread r of a group owns row r, so a row's softmax needs no
-// exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile (attention_tc.cu says what of).  A tile of queries is as
-// many whole nodes as 128 rows hold, so that one TMA box of [nodes][heads of the group] brings it; a row block is one or two of them.  Two (PLAIN):
-// each group takes one, and all key tiles: 2,000 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one
-// every 1,000 cycles, where the memory system brings one every 1,400.  (Row blocks of 128 alone, all of them SPLIT: every 128 rows read
-// the keys again, sixteen full trees behind up to 8,192 keys 277 us.)
+// With more than 16 query rows (nodes x heads of a group) of 128 elements, 32 of 64, mma.sync is what takes the time, not the cache.  Here 128 rows are
+// the lanes of tensor memory, and a block's two groups of four softmax warps each have scores S[128 x 64] (two buffers) and an accumulator
+// O[128 x head] of their own there, a lane that issues their products, and two copying warps for both.  Thread r of a group owns row r, so a row's
+// softmax needs no exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile, half of them exponentials (attention_tc.cu
+// says what of; with two threads a row, which meet once a tile, it took longer).  A tile of queries is as many whole nodes as 128 rows hold, so
+// that one TMA box of [nodes][heads of the group] brings it; a row block is one or two of them.  Two (PLAIN): each group takes one, and all key
+// tiles: 2,700 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one every 1,660 cycles, where the memory
+// system brings one every 1,400.  (Row blocks of 128 alone, all of them SPLIT: every 128 rows read the keys again, sixteen full trees behind up
+// to 8,000 keys 277 us.)  Eight trees of 13 to 32 nodes behind 8,190 keys, 32 heads of 128 in groups of four: 60 us, of which 7 lie before the first
+// scores; sixteen trees of 64 nodes behind 350 to 7,990 keys, 40 heads in groups of five: 198 us, bound by the groups' chains.
 //
 //   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
 //              of equal weight, a PLAIN tile 3, a SPLIT tile 2 and a row block's end SEGMENT_WEIGHT; keys, values and queries of a run's next segment are

@@ -2429,7 +2429,10 @@ def _shape(what: str, name: str, t: torch.Tensor, shape) -> None:
 
 
 USE_TC_TREE = True           # tests switch it off to reach the mma.sync kernel with many rows
-TREE_MMA_ROWS = 64           # query rows (nodes x heads of a group) up to which drafted trees' attention runs on mma.sync
+# Query rows (nodes x heads of a group) by head size up to which drafted trees' attention runs on mma.sync.  us on mma.sync / tcgen05 with 16, 24, 32 and
+# 48 rows: heads of 128, 8 x 8,190 keys 59/57, 68/58, 69/58, 90/59, one of 611 12.2/12.2, 15.5/12.3, 16/12, 18/12; heads of 64, 8 x 4,000 keys 20/30,
+# 26/30, 26/30, 30/31, one of 611 9.4/10.8, 10.6/10.9, 11.0/10.9, 11.8/10.9.
+TREE_MMA_ROWS = {64: 32, 128: 16}
 USE_MMA_TREE = True          # tests switch it off to reach the CUDA-core kernel with bfloat16
 
 
@@ -2457,7 +2460,7 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
         raise KernelError("attn_tree: needs sequences and a bound on their lengths")
     key = (dtype, n_seqs, n_heads, n_kv_heads, head_dim, vd)
     rows = max_nodes * (n_heads // n_kv_heads)
-    if USE_TC_TREE and dtype == torch.bfloat16 and rows > TREE_MMA_ROWS:
+    if USE_TC_TREE and dtype == torch.bfloat16 and rows > TREE_MMA_ROWS.get(head_dim, rows):
         lib = _lib("attention_tree_tc")
         if lib.llg_attn_tree_tc_supported(head_dim, vd, n_seqs, n_heads // n_kv_heads):
             return TreePlan("tc", key, 1, max_nodes, max_len,

@@ -229,6 +229,16 @@ def test_many_rows(ops, hd, before, nodes, nh, nkv, monkeypatch):
     c.check(ops)
 
 
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("before,nodes", [([0, 63, 64, 300], [5, 9, 16, 12]), ([1000, 2], [9, 5])], ids=str)
+def test_a_few_rows_on_both_matrix_paths(ops, hd, before, nodes, window, monkeypatch):
+    c = Case(BF16, 8, 2, hd, before, nodes, window=window, seed=hd)
+    for rows in ({}, {64: 0, 128: 0}):
+        monkeypatch.setattr(ops, "TREE_MMA_ROWS", rows)
+        c.check(ops)
+
+
 @pytest.mark.parametrize("tc", [True, False], ids=["tc", "mma"])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_what_many_rows_do_not_see_has_no_part(ops, hd, tc, monkeypatch):
