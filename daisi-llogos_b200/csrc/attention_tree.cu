@@ -12,10 +12,12 @@
 // instruction, so that a float read from shared memory is used two to eight times; the keys' rows are padded by 16 bytes, which spreads the
 // sixteen rows that a half warp reads over all banks.  Runs that share a row block leave partial results (sums, maximum, sum of weights); the
 // block that takes the last ticket joins them in their order, four columns of a row a thread and sixteen runs asked for at once, so results do
-// not depend on who comes last.  What bounds it: reads of shared memory, about 500 a warp and tile, and two warps a scheduler that wait for
-// them; the join is 7 of 41 us.  Three trees of 8 to 12 nodes behind 735 to 1,878 keys, 32 heads of 64 in groups of four: 41 us (13 splits
-// of five tiles: 47; 21 of three: 40; 32 of two: 45.  One product an instruction, 13 splits: 54.  Without the copies ahead, a division and a page
-// look-up per 16 bytes, and a warp that joined a row run by run: 149).
+// not depend on who comes last.  The running maxima are raised, with the exchange that this takes, only when a weight would be more than 2^12 (with
+// an exchange per tile the softmax took 2,800 cycles of a tile's 9,300, now 600 of 7,500).  What bounds it: reads of shared memory for the
+// products, 2,500 cycles each, with two to three blocks a multiprocessor; 12 us lie before the first tile and in the join.  Three trees of 8 to 12
+// nodes behind 735 to 1,878 keys, 32 heads of 64 in groups of four: 38 us (13 splits of five tiles: 43; 21 of three: 37; 32 of two: 40.  One product
+// an instruction and an exchange per tile, 13 splits: 54.  Without the copies ahead, a division and a page look-up per 16 bytes, and a warp that
+// joined a row run by run: 149).
 #include "common.cuh"
 #include "cache_args.h"
 #include "simt_tiles.cuh"
@@ -78,6 +80,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
   });
 
+  const float sc = a.scale * 1.4426950408889634f;      // maxima and exponents are in binary orders
   float m[RY], l[RY];
   float2 o[RY][VD * 2];
 #pragma unroll
@@ -135,36 +138,51 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     }
     // positions that some row may not see: the tree's, those behind it, the window's edge
     const bool mixed = p0 + TK > lb || (a.window > 0 && p0 <= lb + n - a.window);
+    if (mixed) {
 #pragma unroll
-    for (int r = 0; r < RY; ++r) {
-      const int row = ty * RY + r;
-      float mx = -INFINITY;
+      for (int r = 0; r < RY; ++r)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int p = p0 + tx + 16 * e, j = p - lb;
-        bool sees = true;
-        if (mixed) {
-          if (j < 0) sees = a.window <= 0 || depth[row] - j < a.window;
-          else sees = j < n && ((bits[row] >> j) & 1) && (a.window <= 0 || depth[row] - node_depth[j] < a.window);
+        for (int e = 0; e < 2; ++e) {
+          const int row = ty * RY + r, j = p0 + tx + 16 * e - lb;
+          const bool sees = j < 0 ? a.window <= 0 || depth[row] - j < a.window
+                                  : j < n && ((bits[row] >> j) & 1) && (a.window <= 0 || depth[row] - node_depth[j] < a.window);
+          s[r][e] = sees ? s[r][e] : -INFINITY;
         }
-        s[r][e] = sees ? s[r][e] * a.scale : -INFINITY;
-        mx = fmaxf(mx, s[r][e]);
-      }
+    }
+    // the maxima are raised, by all lanes of a row, only when a weight would be more than 2^12
+    bool raise = false;
 #pragma unroll
-      for (int k = 8; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-      const float m_new = fmaxf(m[r], mx);
-      const float corr = m_new == -INFINITY ? 1.f : expf(m[r] - m_new);
-      m[r] = m_new;
-      l[r] *= corr;
+    for (int r = 0; r < RY; ++r) raise |= fmaxf(s[r][0], s[r][1]) * sc > m[r] + 12.f;
+    if (__any_sync(0xffffffffu, raise)) {
+      float mx[RY];
 #pragma unroll
-      for (int e = 0; e < VD * 2; ++e) o[r][e] = __fmul2_rn(o[r][e], make_float2(corr, corr));
+      for (int r = 0; r < RY; ++r) mx[r] = fmaxf(s[r][0], s[r][1]) * sc;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float p = s[r][e] == -INFINITY ? 0.f : expf(s[r][e] - m_new);
-        l[r] += p;
-        Ps[row * (TK + 4) + tx + 16 * e] = p;
+      for (int k = 8; k > 0; k >>= 1)
+#pragma unroll
+        for (int r = 0; r < RY; ++r) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], k));
+#pragma unroll
+      for (int r = 0; r < RY; ++r) {
+        const float m_new = fmaxf(m[r], mx[r]), corr = m_new == -INFINITY ? 1.f : exp2f(m[r] - m_new);
+        m[r] = m_new;
+        l[r] *= corr;
+#pragma unroll
+        for (int e = 0; e < VD * 2; ++e) o[r][e] = __fmul2_rn(o[r][e], make_float2(corr, corr));
       }
     }
+#pragma unroll
+    for (int r = 0; r < RY; ++r) {
+      const float ms = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[r][e] = exp2f(fmaf(s[r][e], sc, -ms));       // (of -inf exactly nothing)
+        l[r] += s[r][e];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RY; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) Ps[(ty * RY + r) * (TK + 4) + tx + 16 * e] = s[r][e];
     __syncwarp();                          // a row's weights come from and go to the lanes of one warp
 #pragma unroll 2
     for (int j = 0; j < TK; j += 4) {
@@ -258,7 +276,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       float top = M;
 #pragma unroll
       for (int k = 0; k < DEEP; ++k) top = fmaxf(top, ml[k].x);
-      const float f = M == -INFINITY ? 0.f : expf(M - top);
+      const float f = M == -INFINITY ? 0.f : exp2f(M - top);
       M = top;
       L *= f;
       acc.x *= f;
@@ -268,7 +286,7 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
 #pragma unroll
       for (int k = 0; k < DEEP; ++k) {
         if (ml[k].x == -INFINITY) continue;                          // a run in which the row sees nothing has left no sums
-        const float w = expf(ml[k].x - M);
+        const float w = exp2f(ml[k].x - M);
         L += w * ml[k].y;
         acc.x += w * v[k].x;
         acc.y += w * v[k].y;

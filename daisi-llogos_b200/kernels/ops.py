@@ -2617,8 +2617,8 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
         # pairs of tiles, at least two a split
         per = 2 * max(2, -(-tiles * n_seqs * n_kv_heads // (2 * 3 * sm_count())))
     else:
-        # splits of at least four tiles, as many as give every multiprocessor six blocks
-        per = max(4, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
+        # splits of at least four tiles (two on the CUDA cores, whose tiles take several times as long), as many as give every multiprocessor six blocks
+        per = max(4 if mma else 2, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
     splits = -(-tiles // per)
     total = n_seqs * n_kv_heads * rows
     scores = total * splits * per * tile if rows <= lib.llg_key_weights_store_rows() else 0
