@@ -8,31 +8,39 @@
 //
 // A weight needs its row's whole sum, so there are two passes over a (sequence, head)'s keys, cut into splits: the first leaves every split's
 // maximum and sum per row; the blocks of the second join those for their rows and divide.  Few rows (a decode step: the heads of a group) leave
-// their scores on the way, 4 bytes a row beside a key's 2 hd bytes, and the second pass reads those; with more rows than STORE_ROWS the
-// second pass works the scores out again from the keys, which then lie in L2, because storing them would be the larger traffic.
+// their scores on the way, 4 bytes a row beside a key's 2 hd bytes, and the second pass reads those; on the matrix instructions with more rows than
+// STORE_ROWS, and here where the scores would be more than a workspace should be, the second pass works them out again from the keys.
 // Sums run in a fixed order everywhere.
+//
+// What bounds it: reads of shared memory for the products, and for small calls the two passes' latency.  float32, us with scores kept / worked out
+// twice: a decode step of 8 x 4,000 keys, 32 heads of 128 in groups of four, 60 / 120 (the keys alone 21); 13 x 1,106, 38 / 73; 32 queries of two
+// prompts of 2,000 to 4,000, 105 / 205; 17 queries of five of 748, 9 heads of 48, 23 / 34.  (With 32 rows to a block whatever their number, row blocks
+// one after the other, one product an instruction and splits of four tiles: 130, 75, 283 and 59.)
 #include "common.cuh"
 #include "cache_args.h"
 #include "key_weights.cuh"
 #include "simt_tiles.cuh"
 
+#include <algorithm>
+
 LLG_API const char* llg_last_error() { return g_llg_error; }
 
 namespace {
 
-constexpr int THREADS = 128, ROWS = 32, MAX_HD = 384;
+constexpr int THREADS = 128, MAX_HD = 384;
 
-// A block: a split's keys of a (sequence, head), 64 at a time, ROWS rows at a time; a thread: 4 rows x 4 keys.  SECOND: the rows' ends are known.
-// STAGES: tiles in shared memory, 2 where they fit: the next one's keys arrive while this one's are used.
-template <typename T, bool SECOND, int STAGES>
+// A block: a split's keys of a (sequence, head), 64 at a time, and 8 RY rows, or in the second pass all rows, 8 RY at a time; a thread: RY rows x 4
+// keys, two products an instruction.  SECOND: the rows' ends are known.  STAGES: tiles in shared memory, 2 where they fit: the next one's keys
+// arrive while this one's are used.
+template <typename T, int RY, bool SECOND, int STAGES>
 __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
-  constexpr int KEYS = WEIGHT_TILE, KPT = KEYS / 16;
+  constexpr int KEYS = WEIGHT_TILE, KPT = KEYS / 16, ROWS = 8 * RY;
   extern __shared__ __align__(16) float smem[];
   __shared__ float column[8][KEYS];
   __shared__ float2 ends[ROWS];
   pdl_launch_dependents();
   pdl_wait();
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int row_blocks = gridDim.y / a.nkv, split = blockIdx.x, h = blockIdx.y / row_blocks, b = blockIdx.z;
   const Rows s = rows_of(a, b);
   const int first = split * a.split_keys, last = min(s.total, first + a.split_keys);
   if (first >= last || s.rows <= 0) return;
@@ -45,20 +53,20 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
   const int slot = a.slots[b], most = s.group * a.last;
   const long long pair = (long long)b * a.nkv + h;
   const TileCopy<THREADS> copy(kp);
-  for (int r0 = 0; r0 < s.rows; r0 += ROWS) {
+  for (int r0 = ((int)blockIdx.y - h * row_blocks) * ROWS; r0 < s.rows; r0 += row_blocks * ROWS) {
     __syncthreads();
     copy_rows<THREADS, T>(Qs, ks, ROWS, a.hd, kp, [&](int r) {
       return r0 + r < s.rows ? qg + ((long long)(s.tok0 + (r0 + r) / s.group) * a.nh + h * s.group + (r0 + r) % s.group) * a.hd : nullptr;
     });
     if (SECOND && tid < ROWS && r0 + tid < s.rows) ends[tid] = row_end(a, pair, s, r0 + tid);
     const float sc = a.scale * WEIGHT_LOG2E;
-    float m[4], l[4];                      // this thread's keys alone
-    int pos[4];                            // the query's own position: it sees the keys up to there
+    float m[RY], l[RY];                    // this thread's keys alone
+    int pos[RY];                           // the query's own position: it sees the keys up to there
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < RY; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
-      pos[r] = s.pos0 + (r0 + ty * 4 + r) / s.group;
+      pos[r] = s.pos0 + (r0 + ty * RY + r) / s.group;
     }
     auto request = [&](int p0) {           // a tile of keys into its stage: a page's, one behind the other
       if (p0 < last)
@@ -73,28 +81,37 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
       tile_wait<STAGES - 1>();
       __syncthreads();
       const float* Kt = Ks + (p0 - first) / KEYS % STAGES * KEYS * ks;
-      float x[4][KPT];
+      float2 x2[RY][KPT];                  // elements 0, 2, ... and 1, 3, ...
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int r = 0; r < RY; ++r)
 #pragma unroll
-        for (int c = 0; c < KPT; ++c) x[r][c] = 0.f;
+        for (int c = 0; c < KPT; ++c) x2[r][c] = make_float2(0.f, 0.f);
+#pragma unroll 2
       for (int d = 0; d < kp; d += 4) {
-        float4 q[4];
+        float4 q[RY];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) q[r] = *reinterpret_cast<const float4*>(Qs + (ty * 4 + r) * ks + d);
+        for (int r = 0; r < RY; ++r) q[r] = *reinterpret_cast<const float4*>(Qs + (ty * RY + r) * ks + d);
 #pragma unroll
         for (int c = 0; c < KPT; ++c) {
           const float4 k = *reinterpret_cast<const float4*>(Kt + (tx + 16 * c) * ks + d);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r][c] += q[r].x * k.x + q[r].y * k.y + q[r].z * k.z + q[r].w * k.w;
+          for (int r = 0; r < RY; ++r) {
+            x2[r][c] = __ffma2_rn(make_float2(q[r].x, q[r].y), make_float2(k.x, k.y), x2[r][c]);
+            x2[r][c] = __ffma2_rn(make_float2(q[r].z, q[r].w), make_float2(k.z, k.w), x2[r][c]);
+          }
         }
       }
+      float x[RY][KPT];
+#pragma unroll
+      for (int r = 0; r < RY; ++r)
+#pragma unroll
+        for (int c = 0; c < KPT; ++c) x[r][c] = x2[r][c].x + x2[r][c].y;
       float sum[KPT];
 #pragma unroll
       for (int c = 0; c < KPT; ++c) sum[c] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = r0 + ty * 4 + r;
+      for (int r = 0; r < RY; ++r) {
+        const int row = r0 + ty * RY + r;
         if (row >= s.rows) continue;
         float top = m[r];
 #pragma unroll
@@ -102,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
           const int p = p0 + tx + 16 * c;
           if (p > pos[r]) x[r][c] = -INFINITY;
           if (SECOND) {
-            if (p <= pos[r]) sum[c] += share(x[r][c], sc, ends[ty * 4 + r]);
+            if (p <= pos[r]) sum[c] += share(x[r][c], sc, ends[ty * RY + r]);
           } else {
             top = fmaxf(top, ceilf(x[r][c] * sc));
             if (a.scores && p < s.total) a.scores[score_at(a, pair * most + row, p)] = x[r][c];
@@ -129,34 +146,41 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
     }
     if (!SECOND) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
+      for (int r = 0; r < RY; ++r) {
         float top = m[r];
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         float sum = m[r] == -INFINITY ? 0.f : l[r] * whole2(m[r] - top);
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-        const int row = r0 + ty * 4 + r;
+        const int row = r0 + ty * RY + r;
         if (row < s.rows && tx == 0) stats_of(a, pair, split)[row] = make_float2(top, sum);
       }
     }
   }
 }
 
-template <typename T, int STAGES>
+template <typename T, int RY, int STAGES>
 int run(const KeyWeightArgs& a, cudaStream_t stream) {
   const int ks = (a.hd + 3) / 4 * 4 + 4;
-  const size_t smem = sizeof(float) * (size_t)(STAGES * WEIGHT_TILE + ROWS) * ks;
-  const dim3 grid(a.splits, a.nkv, a.n_seqs);
-  auto go = [&](void (*kernel)(KeyWeightArgs)) -> int {
+  const size_t smem = sizeof(float) * (size_t)(STAGES * WEIGHT_TILE + 8 * RY) * ks;
+  const int rows = a.nh / a.nkv * a.last, row_blocks = std::min((rows + 8 * RY - 1) / (8 * RY), 65535 / a.nkv);
+  auto go = [&](void (*kernel)(KeyWeightArgs), int rbs) -> int {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return llg_fail("key_weights: shared memory %zu: %s", smem, cudaGetErrorString(e));
-    e = llg_launch(kernel, grid, dim3(THREADS), smem, stream, a);
+    e = llg_launch(kernel, dim3(a.splits, a.nkv * rbs, a.n_seqs), dim3(THREADS), smem, stream, a);
     if (e != cudaSuccess) return llg_fail("key_weights: launch: %s", cudaGetErrorString(e));
     return llg_check_launch("key_weights");
   };
-  if (go(key_weights_kernel<T, false, STAGES>)) return 1;
-  return a.scores ? add_stored(a, stream) : go(key_weights_kernel<T, true, STAGES>);
+  if (go(key_weights_kernel<T, RY, false, STAGES>, row_blocks)) return 1;
+  return a.scores ? add_stored(a, stream) : go(key_weights_kernel<T, RY, true, STAGES>, 1);      // (a key's shares are added up by one block)
+}
+
+template <typename T>
+int dispatch(const KeyWeightArgs& a, cudaStream_t stream) {
+  const bool few = a.nh / a.nkv * a.last <= 8;
+  if (a.hd <= 128) return few ? run<T, 1, 2>(a, stream) : run<T, 4, 2>(a, stream);
+  return few ? run<T, 1, 1>(a, stream) : run<T, 4, 1>(a, stream);
 }
 
 }  // namespace
@@ -169,7 +193,7 @@ LLG_API int llg_key_weights_simt(const KeyWeightArgs* args, int dtype, cudaStrea
   if (check(a)) return 1;
   LLG_REQUIRE(a.hd <= MAX_HD, "key_weights: heads of %d elements (1 to %d)", a.hd, MAX_HD);
   if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
-  if (dtype == LLG_F32) return a.hd <= 128 ? run<float, 2>(a, stream) : run<float, 1>(a, stream);
-  if (dtype == LLG_BF16) return a.hd <= 128 ? run<__nv_bfloat16, 2>(a, stream) : run<__nv_bfloat16, 1>(a, stream);
+  if (dtype == LLG_F32) return dispatch<float>(a, stream);
+  if (dtype == LLG_BF16) return dispatch<__nv_bfloat16>(a, stream);
   return llg_fail("key_weights: unknown dtype %d", dtype);
 }

@@ -7,7 +7,7 @@
 namespace {
 
 constexpr int WEIGHT_TILE = 64;     // keys of a tile (a page); a split is a whole number of them
-constexpr int STORE_ROWS = 32;      // most rows of a (sequence, head) whose scores are kept between the passes
+constexpr int STORE_ROWS = 32;      // most rows of a (sequence, head) whose scores the matrix instructions' kernels keep between the passes
 
 // The rows of sequence b: its last queries' heads of one group.
 struct Rows {
@@ -20,7 +20,7 @@ __device__ __forceinline__ Rows rows_of(const KeyWeightArgs& a, int b) {
   s.tok0 = end - n;
   s.rows = n * s.group;
   s.before = a.len_before[b];
-  s.total = min(min(s.before + count, a.weight_width), a.splits * a.split_keys);
+  s.total = min(min(s.before + count, a.weight_width), min(a.splits * a.split_keys, a.table_width * WEIGHT_TILE));      // (no key behind what holds it)
   s.pos0 = s.before + count - n;
   return s;
 }
@@ -65,12 +65,14 @@ __device__ __forceinline__ void add_weight(const KeyWeightArgs& a, int slot, int
   *w = (again || p < before ? *w : 0.f) + t;
 }
 
-// The second pass over stored scores: a thread takes four keys, a block's width apart, and four rows of them at a time; the first rows' scores and the
-// keys' entries are under way while the rows' ends are worked out.  (A thread per key: twice as many blocks as run at once, each a chain of
-// four reads; eight sequences of 8,190 keys, 4 rows, 13 us.)
-constexpr int ADD_THREADS = 256, ADD_KEYS = 4, ADD_ROWS = 4;
+// The second pass over stored scores: a thread takes four keys, a block's width apart, and DEEP rows of them at a time, four where there are no more;
+// the first rows' scores and the keys' entries are under way while the rows' ends are worked out.  (A thread per key: twice as many blocks as run
+// at once, each a chain of reads; eight sequences of 8,190 keys, 4 rows, 13 us of a call's 40, now 6 of 33.)
+constexpr int ADD_THREADS = 256, ADD_KEYS = 4;
+template <int DEEP>
 __global__ void __launch_bounds__(ADD_THREADS) add_stored_kernel(KeyWeightArgs a) {
-  __shared__ float2 ends[STORE_ROWS];
+  constexpr int AT_ONCE = 32;                           // rows whose ends are worked out at once
+  __shared__ float2 ends[AT_ONCE];
   pdl_launch_dependents();
   pdl_wait();
   const int h = blockIdx.y, b = blockIdx.z, p0 = blockIdx.x * (ADD_THREADS * ADD_KEYS) + threadIdx.x;
@@ -79,10 +81,11 @@ __global__ void __launch_bounds__(ADD_THREADS) add_stored_kernel(KeyWeightArgs a
   if (p0 - (int)threadIdx.x >= s.total || s.rows <= 0) return;
   const long long pair = (long long)b * a.nkv + h, first = pair * s.group * a.last;
   float* w = a.weights + ((long long)slot * a.nkv + h) * a.weight_width;
-  float x[ADD_ROWS][ADD_KEYS], sum[ADD_KEYS], held[ADD_KEYS];
+  const float sc = a.scale * WEIGHT_LOG2E;
+  float x[DEEP][ADD_KEYS], sum[ADD_KEYS], held[ADD_KEYS];
   auto fetch = [&](int r0) {
 #pragma unroll
-    for (int r = 0; r < ADD_ROWS; ++r)
+    for (int r = 0; r < DEEP; ++r)
 #pragma unroll
       for (int k = 0; k < ADD_KEYS; ++k) {
         const int p = p0 + k * ADD_THREADS;
@@ -96,17 +99,19 @@ __global__ void __launch_bounds__(ADD_THREADS) add_stored_kernel(KeyWeightArgs a
     held[k] = p < s.before && p < s.total ? w[p] : 0.f;
     sum[k] = 0.f;
   }
-  if (threadIdx.x < s.rows) ends[threadIdx.x] = row_end(a, pair, s, threadIdx.x);
-  __syncthreads();
-  const float sc = a.scale * WEIGHT_LOG2E;
-  for (int r0 = 0; r0 < s.rows; r0 += ADD_ROWS) {
-    if (r0 > 0) fetch(r0);
+  for (int r0 = 0; r0 < s.rows; r0 += DEEP) {
+    if (r0 % AT_ONCE == 0) {
+      __syncthreads();                                  // the rows before have been read
+      if (threadIdx.x < AT_ONCE && r0 + (int)threadIdx.x < s.rows) ends[threadIdx.x] = row_end(a, pair, s, r0 + threadIdx.x);
+      __syncthreads();
+    }
 #pragma unroll
-    for (int r = 0; r < ADD_ROWS; ++r) {
-      const float2 end = ends[min(r0 + r, s.rows - 1)];
+    for (int r = 0; r < DEEP; ++r) {
+      const float2 end = ends[min(r0 + r, s.rows - 1) % AT_ONCE];
 #pragma unroll
       for (int k = 0; k < ADD_KEYS; ++k) sum[k] += x[r][k] == -INFINITY ? 0.f : share(x[r][k], sc, end);       // -inf: a key behind the query
     }
+    if (r0 + DEEP < s.rows) fetch(r0 + DEEP);
   }
 #pragma unroll
   for (int k = 0; k < ADD_KEYS; ++k)
@@ -115,7 +120,9 @@ __global__ void __launch_bounds__(ADD_THREADS) add_stored_kernel(KeyWeightArgs a
 
 inline int add_stored(const KeyWeightArgs& a, cudaStream_t stream) {
   const long long most = (long long)a.splits * a.split_keys;
-  cudaError_t e = llg_launch(add_stored_kernel, dim3((unsigned)((most + ADD_THREADS * ADD_KEYS - 1) / (ADD_THREADS * ADD_KEYS)), a.nkv, a.n_seqs), dim3(ADD_THREADS), 0, stream, a);
+  const dim3 grid((unsigned)((most + ADD_THREADS * ADD_KEYS - 1) / (ADD_THREADS * ADD_KEYS)), a.nkv, a.n_seqs);
+  auto kernel = a.nh / a.nkv * a.last <= 4 ? add_stored_kernel<4> : add_stored_kernel<8>;      // (rows asked for at once)
+  cudaError_t e = llg_launch(kernel, grid, dim3(ADD_THREADS), 0, stream, a);
   if (e != cudaSuccess) return llg_fail("key_weights: launch: %s", cudaGetErrorString(e));
   return llg_check_launch("key_weights");
 }
@@ -128,8 +135,6 @@ inline int check(const KeyWeightArgs& a) {
   LLG_REQUIRE(a.nkv <= 65535 && a.n_seqs <= 65535, "key_weights: %d heads, %d sequences: more than a grid takes", a.nkv, a.n_seqs);
   LLG_REQUIRE(a.scale > 0.f, "key_weights: the softmax scale must be positive");
   LLG_REQUIRE(a.stats, "key_weights: needs scratch");
-  LLG_REQUIRE(!a.scores || a.nh / a.nkv * a.last <= STORE_ROWS, "key_weights: %d rows' scores are not stored (at most %d)", a.nh / a.nkv * a.last,
-              STORE_ROWS);
   return 0;
 }
 

@@ -2586,6 +2586,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
 
 
 USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel with bfloat16
+KEY_SCORE_FLOATS = 1 << 24   # the most scores that key weights on the CUDA cores keep between their passes: 64 MB
 USE_TC_WEIGHTS = True        # and this, to reach the mma.sync kernel with more rows than have their scores stored
 
 
@@ -2621,7 +2622,9 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
         per = max(4 if mma else 2, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
     splits = -(-tiles // per)
     total = n_seqs * n_kv_heads * rows
-    scores = total * splits * per * tile if rows <= lib.llg_key_weights_store_rows() else 0
+    scores = total * splits * per * tile
+    if rows > lib.llg_key_weights_store_rows() if mma else scores > KEY_SCORE_FLOATS:
+        scores = 0                                       # they are worked out twice
     return KeyWeightPlan(kind, (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, splits, per * tile,
                          -(-2 * total * splits // 4) * 4, scores)
 

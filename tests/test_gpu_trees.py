@@ -447,6 +447,15 @@ def test_bfloat16_weights_on_the_cuda_cores(ops, hd, monkeypatch):
     test_weights_of_keys(ops, BF16, 8, 2, hd, [5, 0, 64], [1, 200, 64], 8)
 
 
+@pytest.mark.parametrize("keep", [True, False], ids=["kept", "twice"])
+@pytest.mark.parametrize("dtype,nh,nkv,hd,last", [(F32, 8, 2, 64, 40), (F32, 5, 1, 80, 20), (F32, 3, 3, 200, 9), (BF16, 8, 2, 20, 33), (F32, 8, 1, 128, 1)], ids=str)
+def test_weights_of_many_queries_on_the_cuda_cores(ops, dtype, nh, nkv, hd, last, keep, monkeypatch):
+    """Scores kept between the passes, and worked out twice; several row blocks, row ends worked out in several goes."""
+    monkeypatch.setattr(ops, "USE_MMA_WEIGHTS", False)
+    monkeypatch.setattr(ops, "KEY_SCORE_FLOATS", 1 << 24 if keep else 0)
+    test_weights_of_keys(ops, dtype, nh, nkv, hd, [300, 0, 127], [1, 230, 41], last)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_weights_of_many_queries_on_mma_sync(ops, hd, monkeypatch):
     monkeypatch.setattr(ops, "USE_TC_WEIGHTS", False)
