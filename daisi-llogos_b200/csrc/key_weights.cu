@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(THREADS) key_weights_kernel(KeyWeightArgs a) {
         float top = m[r];
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        float sum = m[r] == -INFINITY ? 0.f : l[r] * whole2(m[r] - top);
+        float sum = m[r] == -INFINITY ? l[r] : l[r] * whole2(m[r] - top);
 #pragma unroll
         for (int k = 8; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
         const int row = r0 + ty * RY + r;

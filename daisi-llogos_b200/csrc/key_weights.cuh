@@ -50,13 +50,12 @@ __device__ __forceinline__ float2 row_end(const KeyWeightArgs& a, long long pair
     float top = m;
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = fmaxf(top, v[k].x);
-    if (top == -INFINITY) continue;
-    l *= whole2(m - top);
+    if (m != -INFINITY) l *= whole2(m - top);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) l += v[k].x == -INFINITY ? 0.f : v[k].y * whole2(v[k].x - top);
+    for (int k = 0; k < 8; ++k) l += v[k].x == -INFINITY ? v[k].y : v[k].y * whole2(v[k].x - top);      // (without a maximum the sum is 0, or no number)
     m = top;
   }
-  return make_float2(m, 1.f / l);
+  return make_float2(l != l && m == -INFINITY ? 0.f : m, 1.f / l);      // scores that are no numbers: the row has to show it
 }
 
 // `again`: an earlier block of rows has written the key's entry in this launch already.

@@ -188,7 +188,10 @@ __global__ void __launch_bounds__(THREADS) key_weights_mma_kernel(const __grid_c
 #pragma unroll
             for (int t = 0; t < MT; ++t)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) y += fast_exp2(fmaf(x[t][n][2 * e + c], sc, -end[t][e].x)) * end[t][e].y;
+              for (int e = 0; e < 2; ++e) {
+                const float v = x[t][n][2 * e + c];        // -inf: a key behind the query, which a row of no numbers does not reach either
+                y += v == -INFINITY ? 0.f : fast_exp2(fmaf(v, sc, -end[t][e].x)) * end[t][e].y;
+              }
             sum[2 * n + c] = y;
           }
         // over the eight lanes of a key, by halves: a lane keeps the keys whose place has its bits

@@ -468,6 +468,31 @@ def test_weights_of_many_queries(ops, nh, nkv, hd, last):
     test_weights_of_keys(ops, BF16, nh, nkv, hd, [700, 0, 1023, 320], [1, 1153, 1, 64], last)
 
 
+@pytest.mark.parametrize("dtype,hd,last,keep", [(BF16, 64, 30, True), (BF16, 128, 6, True), (BF16, 80, 30, True), (F32, 64, 30, True), (F32, 64, 30, False),
+                                                (BF16, 20, 4, True)], ids=str)
+def test_a_query_that_is_no_number_shows_in_the_keys_it_sees(ops, dtype, hd, last, keep, monkeypatch):
+    """The rows of one head of one query hold NaN, the pages NaN behind the sequence: its keys' entries show it, later keys' and other heads' do not."""
+    monkeypatch.setattr(ops, "KEY_SCORE_FLOATS", 1 << 24 if keep else 0)
+    nh, nkv, before, count = 4, 2, 100, 40
+    total, bad = before + count, count - 3
+    k = normal(total, nkv, hd, seed=3).to(dtype)
+    (kp,), table = T.pages_of([[k]], nkv, (hd,), dtype, 4, 2, [1], hd, device=DEV)
+    q = normal(count, nh, hd, seed=5).to(dtype)
+    q[bad, 1] = float("nan")
+    plan = ops.key_weights_plan(dtype, 1, last, nh, nkv, hd, total)
+    weights = torch.zeros(2, nkv, 200, device=DEV)
+    ops.key_weights(q.to(DEV), kp, table, ints([1]), ints([0, count]), ints([before]), weights, torch.empty(plan.scratch_floats, device=DEV),
+                    scale=hd ** -0.5, last=last, plan=plan, counters=torch.zeros(plan.n_counters, dtype=torch.int32, device=DEV))
+    got = weights[1].cpu()
+    assert torch.isnan(got[0, :before + bad + 1]).all()
+    clean = q.clone()
+    clean[bad, 1] = 0
+    want, slack = T.key_weights(clean, k, before, last, hd ** -0.5, torch.zeros(nkv, 200))
+    late = slice(before + bad + 1, total)
+    assert ((got[0, late].double() - want[0, late]).abs() <= slack[0, late] + 1e-9).all()
+    assert ((got[1].double() - want[1]).abs() <= slack[1] + 1e-9).all()
+
+
 def test_weights_of_long_sequences_in_a_graph(ops):
     """Thousands of keys: many blocks' sums are joined; every query's shares add up to one."""
     nh, nkv, hd, before = 8, 2, 128, [3900, 100]
