@@ -4,7 +4,7 @@
 // The kernel streams the cache: with R query rows (nodes x heads of a group) a key's and a value's 4 hd bytes take 4 R hd flops, so up to 16 rows
 // of heads of 128, 32 of heads of 64, the memory system decides the time and mma.sync keeps up beside it (eight sequences of 8,190 keys, heads of
 // 128, 16 rows: 59 us, 69 % of the copy bandwidth); more go to attention_tree_tc.cu, heads of other sizes stay.  One tree of 8 nodes behind
-// 611 keys, 32 heads of 64 in groups of four: 11 us, the latency of two kernels.
+// 611 keys, 32 heads of 64 in groups of four: 10 us, the latency of two kernels (11 with the plan behind the wait for the kernel before).
 //
 //   copies     A fifth warp brings every key and value tile (one cache page of one key/value head) with TMA boxes of 64 x 64 elements into a
 //              ring of stages handed over by mbarriers; head sizes that are no multiple of 64 are filled up with zeros by the boxes.
@@ -66,7 +66,6 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   __shared__ float2 merge_ml[WK > 1 ? WORK_WARPS : 1][16];
 
   pdl_launch_dependents();
-  pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == WORK_WARPS * 32) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -90,25 +89,27 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int units = a.nkv * plan.sums[a.n_seqs];
   const int chunk = (unsigned)(units + gridDim.x - 1) / gridDim.x;
   const int u0 = min(units, (int)blockIdx.x * chunk), u1 = min(units, u0 + chunk);
+  const int n_units = u1 - u0;
+  // first row of the tile of the run's unit i in the pages, seen as [pages x kv heads x 64]
+  auto row_of = [&](int i) -> int {
+    if (i >= n_units) return 0;
+    const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + i);
+    const TreeShape sh = tree_shape(a, plan, c.b);
+    return (a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages] * a.nkv + c.kvh) * TK;
+  };
+  int row = warp == WORK_WARPS ? row_of(lane) : 0;
+  pdl_wait();                                          // all before it reads sizes, slots and tables alone, which no kernel of a step writes
   typedef Place<HDP, ROWS> P;
   if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
   if (u0 >= u1) return;
   volatile int* abortp = &abort_flag;
-  const int n_units = u1 - u0;
 
   if (warp == WORK_WARPS) {
     // ---- copies: the lanes look up the pages of 32 tiles side by side, then each in turn issues its tile's boxes ----
     int issued = 0;
     bool fine = true;
     for (int base = 0; base < n_units && fine; base += 32) {
-      const int idx = base + lane;
-      int row = 0;
-      if (idx < n_units) {
-        const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + idx);
-        const TreeShape sh = tree_shape(a, plan, c.b);
-        const int page = a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages];
-        row = (page * a.nkv + c.kvh) * TK;
-      }
+      if (base > 0) row = row_of(base + lane);
       const int n_here = min(32, n_units - base);
       for (int k = 0; k < n_here && fine; ++k) {
         if (lane == k) {

@@ -9,8 +9,9 @@
 // that one TMA box of [nodes][heads of the group] brings it; a row block is one or two of them.  Two (PLAIN): each group takes one, and all key
 // tiles: 2,700 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one every 1,660 cycles, where the memory
 // system brings one every 1,400.  (Row blocks of 128 alone, all of them SPLIT: every 128 rows read the keys again, sixteen full trees behind up
-// to 8,000 keys 277 us.)  Eight trees of 13 to 32 nodes behind 8,190 keys, 32 heads of 128 in groups of four: 60 us, of which 7 lie before the first
-// scores; sixteen trees of 64 nodes behind 350 to 7,990 keys, 40 heads in groups of five: 198 us, bound by the groups' chains.
+// to 8,000 keys 277 us.)  Eight trees of 13 to 32 nodes behind 8,190 keys, 32 heads of 128 in groups of four: 59 us, of which 7 lie before the first
+// scores; sixteen trees of 64 nodes behind 350 to 7,990 keys, 40 heads in groups of five: 192 us, bound by the groups' chains (61 and 198 with the
+// plan and the first page look-ups behind the wait for the kernel before).
 //
 //   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
 //              of equal weight, a PLAIN tile 3, a SPLIT tile 2 and a row block's end SEGMENT_WEIGHT; keys, values and queries of a run's next segment are
@@ -166,7 +167,40 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_wait();
+  const int G = a.nh / a.nkv, tile_nodes = BQ / G, tile_rows = tile_nodes * G, block_rows = QT * tile_rows;
+  plan_units<THREADS>(a, block_rows, plan, weigh, [&](int rows, int rbs, int tiles) {
+    const int split = QT == 1 ? rbs : rbs > 0 && rows - (rbs - 1) * block_rows <= tile_rows;
+    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split) + SEGMENT_WEIGHT * rbs;
+  });
+  // (a run's weight is at least a unit's, so no run between two others is without a unit)
+  const int weight = a.nkv * weigh[a.n_seqs];
+  const int chunk = max(PLAIN_WEIGHT, (int)((unsigned)(weight + gridDim.x - 1) / gridDim.x));
+  const int u0 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, (int)blockIdx.x * chunk));
+  const int u1 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, ((int)blockIdx.x + 1) * chunk));
+  const int n_units = u1 - u0;                       // (none: every role passes by)
+  // What a copying lane needs of the run's unit i: its tile's first row in the pages, seen as [pages x kv heads x 64], and where a segment begins its
+  // queries' first token and head, and how many tiles of them (for the values' warp, which brings them).
+  struct Copy {
+    int row, q_tok, q_head, q_tiles;
+  };
+  auto copy_of = [&](int i) -> Copy {
+    Copy x = {0, 0, 0, 0};
+    if (i < n_units) {
+      const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + i);
+      const TreeShape sh = tree_shape(a, plan, c.b);
+      if (warp == V_LOAD_WARP && (i == 0 || c.t == 0)) {
+        x.q_tok = sh.tok0 + c.rb * QT * tile_nodes;
+        x.q_head = c.kvh * G;
+        x.q_tiles = QT > 1 && sh.n - c.rb * QT * tile_nodes > tile_nodes ? 2 : 1;
+      }
+      const int page = a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages];
+      x.row = (page * a.nkv + c.kvh) * TK;
+    }
+    return x;
+  };
+  Copy next_copy = {0, 0, 0, 0};
+  if (warp == K_LOAD_WARP || warp == V_LOAD_WARP) next_copy = copy_of(lane);
+  pdl_wait();                                        // all before it reads sizes, slots and tables alone, which no kernel of a step writes
   if (warp == ISSUE_WARP) {
     warp_whole();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)),
@@ -175,22 +209,12 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  const int G = a.nh / a.nkv, tile_nodes = BQ / G, tile_rows = tile_nodes * G, block_rows = QT * tile_rows;
-  plan_units<THREADS>(a, block_rows, plan, weigh, [&](int rows, int rbs, int tiles) {
-    const int split = QT == 1 ? rbs : rbs > 0 && rows - (rbs - 1) * block_rows <= tile_rows;
-    return tiles * (PLAIN_WEIGHT * (rbs - split) + SPLIT_WEIGHT * split) + SEGMENT_WEIGHT * rbs;
-  });                                                // (its barriers also stand between the ones above and their use)
+  __syncthreads();
   // (not before: a block of the next kernel must not take tensor memory ahead of this one and then wait for it)
   pdl_launch_dependents();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  // (a run's weight is at least a unit's, so no run between two others is without a unit)
-  const int weight = a.nkv * weigh[a.n_seqs];
-  const int chunk = max(PLAIN_WEIGHT, (int)((unsigned)(weight + gridDim.x - 1) / gridDim.x));
-  const int u0 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, (int)blockIdx.x * chunk));
-  const int u1 = unit_at(plan, weigh, a.n_seqs, a.nkv, min(weight, ((int)blockIdx.x + 1) * chunk));
   typedef Place<HD, QT * BQ> P;
   if (tid == 0) P::notes(a.part, gridDim.x)[blockIdx.x].parts = 0;
-  const int n_units = u1 - u0;                       // (none: every role passes by)
   const uint32_t tmem = tmem_base_slot;
   volatile int* abortp = &abort_flag;
   auto give_up = [&](int code) {
@@ -210,19 +234,8 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     int issued = 0, segments = 0;
     bool fine = true;
     for (int first = 0; first < n_units && fine; first += 32) {
-      const int idx = first + lane;
-      int row = 0, q_tok = 0, q_head = 0, q_tiles = 0;        // q_tiles: of queries, where a segment begins
-      if (idx < n_units) {
-        const Unit c = locate(plan, a.n_seqs, a.nkv, u0 + idx);
-        const TreeShape sh = tree_shape(a, plan, c.b);
-        if (!keys && (idx == 0 || c.t == 0)) {
-          q_tok = sh.tok0 + c.rb * QT * tile_nodes;
-          q_head = c.kvh * G;
-          q_tiles = QT > 1 && sh.n - c.rb * QT * tile_nodes > tile_nodes ? 2 : 1;
-        }
-        const int page = a.page_table[(long long)sh.slot * a.table_width + (sh.t_first + c.t) % a.ring_pages];
-        row = (page * a.nkv + c.kvh) * TK;
-      }
+      const Copy at = first > 0 ? copy_of(first + lane) : next_copy;
+      const int row = at.row, q_tok = at.q_tok, q_head = at.q_head, q_tiles = at.q_tiles;
       const int n_here = min(32, n_units - first);
       for (int k = 0; k < n_here && fine; ++k) {
         int sent = 0;

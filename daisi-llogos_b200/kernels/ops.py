@@ -2494,7 +2494,8 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     were.  What a node does not see has no part in its result, whatever is stored there.
 
     ``plan`` (``attn_tree_plan`` for this batch shape) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left
-    zero) must hold; calls that may run at the same time need their own."""
+    zero) must hold; calls that may run at the same time need their own.  Like decode attention it reads sizes, slots and the page table while
+    the launch before it still runs: no kernel of a step writes those."""
     what, dt, i32 = "attn_tree", q.dtype, torch.int32
     n, nh, hd = q.shape
     n_pages, nkv = k_pages.shape[:2]
