@@ -14,7 +14,7 @@
 // plan and the first page look-ups behind the wait for the kernel before).
 //
 //   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
-//              of equal weight, a PLAIN tile 3, a SPLIT tile 2 and a row block's end SEGMENT_WEIGHT; keys, values and queries of a run's next segment are
+//              of equal weight (PLAIN_WEIGHT, SPLIT_WEIGHT a tile, SEGMENT_WEIGHT a row block); keys, values and queries of a run's next segment are
 //              copied while the last one ends.
 //   softmax    As in attention_tc.cu: weights 2^(x - M) with a whole number M that is raised only when a tile's weights add up to more than
 //              2^14, float32 sums, weights rounded to bfloat16 once.
