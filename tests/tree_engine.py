@@ -168,17 +168,17 @@ def check_evictions(make, weights, cfg, dtype, tol, seed, rounds=3, weights_tol=
     prompts = [[r.randrange(vocab) for _ in range(n)] for n in (70, 131, 9)]
     logits = eng.step(list(zip(slots, prompts)))
 
-    def judge(got, want, what):
+    def compare(got, want, what):
         for b, (x, y) in enumerate(zip(got, want)):
             off = float((x.detach().cpu().double() - y).abs().max()) / float(y.abs().max())
             assert off <= tol, (what, b, off, tol)
 
-    judge(logits, [m.step(p, last)[-1] for m, p in zip(models, prompts)], "prompt")
+    compare(logits, [m.step(p, last)[-1] for m, p in zip(models, prompts)], "prompt")
     for rnd in range(rounds):
         for _ in range(4):
             toks = [r.randrange(vocab) for _ in slots]
             logits = eng.step([(s, [t]) for s, t in zip(slots, toks)])
-            judge(logits, [m.step([t], 1)[0] for m, t in zip(models, toks)], ("decode", rnd))
+            compare(logits, [m.step([t], 1)[0] for m, t in zip(models, toks)], ("decode", rnd))
         g = eng.cache.kv_groups[0]
         for s, m in zip(slots, models):
             n = eng.length(s)
@@ -197,7 +197,7 @@ def check_evictions(make, weights, cfg, dtype, tol, seed, rounds=3, weights_tol=
         eng.cache.audit()
         more = [[r.randrange(vocab) for _ in range(n)] for n in (3, 20, 1)]        # the next turns, after keys are gone
         logits = eng.step(list(zip(slots, more)))
-        judge(logits, [m.step(t, last)[-1] for m, t in zip(models, more)], ("turn", rnd))
+        compare(logits, [m.step(t, last)[-1] for m, t in zip(models, more)], ("turn", rnd))
     held = eng.length(slots[0])
     eng.truncate(slots[0], held - 2)                               # tokens behind the eviction can be forgotten ...
     assert eng.position(slots[0]) == position[0] + 1
@@ -215,5 +215,5 @@ def check_evictions(make, weights, cfg, dtype, tol, seed, rounds=3, weights_tol=
     slot = eng.open()                                              # a new sequence in a slot that was shortened begins anew
     assert eng.position(slot) == 0
     m = T.KeptModel(weights, cfg)
-    judge(eng.step([(slot, prompts[2])]), [m.step(prompts[2], last)[-1]], "a new sequence")
+    compare(eng.step([(slot, prompts[2])]), [m.step(prompts[2], last)[-1]], "a new sequence")
     eng.close(slot)
