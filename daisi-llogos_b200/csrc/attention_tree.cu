@@ -15,7 +15,8 @@
 // not depend on who comes last.  The running maxima are raised, with the exchange that this takes, only when a weight would be more than 2^12 (with
 // an exchange per tile the softmax took 2,800 cycles of a tile's 9,300, now 600 of 7,500).  What bounds it: reads of shared memory for the
 // products, 2,500 cycles each, with two to three blocks a multiprocessor; 12 us lie before the first tile and in the join.  Three trees of 8 to 12
-// nodes behind 735 to 1,878 keys, 32 heads of 64 in groups of four: 38 us (13 splits of five tiles: 43; 21 of three: 37; 32 of two: 40.  One product
+// nodes behind 735 to 1,878 keys, 32 heads of 64 in groups of four: 37 us (with all of it behind the wait for the kernel before 38, then with 13 splits
+// of five tiles 43, 21 of three 37, 32 of two 40.  One product
 // an instruction and an exchange per tile, 13 splits: 54.  Without the copies ahead, a division and a page look-up per 16 bytes, and a warp that
 // joined a row run by run: 149).
 #include "common.cuh"
@@ -41,7 +42,6 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   __shared__ int depth[ROWS], node_depth[LLG_TREE_NODES];
   __shared__ int is_last;
   pdl_launch_dependents();
-  pdl_wait();
   const int kp = (a.hd + 3) / 4 * 4, vp = (a.vd + 3) / 4 * 4;       // padded row sizes
   const int ks = kp + 4, vs = vp + 4;
   float* Qs = smem;                       // [ROWS][ks]
@@ -56,7 +56,6 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   const int tok0 = a.cu_tokens[b];
   const int n = min(min(a.cu_tokens[b + 1], a.n_tokens) - tok0, a.max_nodes);
   const int row0 = rb * ROWS, n_rows = min(ROWS, n * G - row0);
-  if (n_rows <= 0) return;                // the same for all blocks of a row block: nobody waits for a ticket of theirs
   const int lb = a.len_before[b], slot = a.slots[b], total = lb + n;
   const T* qg = (const T*)a.q;
   const T* kg = (const T*)a.k_pages;
@@ -67,15 +66,24 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   // runs of equal length for all sequences, so that short ones have fewer (the second size: of a sequence that is longer than it may be)
   const int per = max(((a.max_len + TK - 1) / TK + a.n_splits - 1) / a.n_splits, (t_end - t0 + a.n_splits - 1) / a.n_splits);
   const int runs = (t_end - t0 + per - 1) / per;
-  if (split >= runs) return;
+  // (no rows: the same for all blocks of a row block, so nobody waits for a ticket of theirs)
+  const bool none = n_rows <= 0 || split >= runs;
   const int t_from = t0 + split * per, t_to = min(t_end, t_from + per);
 
-  for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
-  for (int r = tid; r < ROWS; r += THREADS) {
-    const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
-    bits[r] = mine;
-    depth[r] = __popcll(mine) - 1;
+  // the page of the tile that is asked for next is looked up a tile ahead
+  const int* table = a.page_table + (long long)slot * a.table_width;
+  auto page_of = [&](int t) { return t < t_to ? table[t / 2 % a.ring_pages] : 0; };
+  int page = none ? 0 : page_of(t_from);
+  if (!none) {
+    for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
+    for (int r = tid; r < ROWS; r += THREADS) {
+      const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
+      bits[r] = mine;
+      depth[r] = __popcll(mine) - 1;
+    }
   }
+  pdl_wait();                             // all before it reads sizes, slots, tables and words alone, which no kernel of a step writes
+  if (none) return;
   copy_rows<THREADS, T>(Qs, ks, ROWS, a.hd, kp, [&](int r) {
     return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
   });
@@ -91,10 +99,6 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
     for (int e = 0; e < VD * 2; ++e) o[r][e] = make_float2(0.f, 0.f);
   }
   const TileCopy<THREADS> copy_k(kp), copy_v(vp);
-  // the page of the tile that is asked for next is looked up a tile ahead
-  const int* table = a.page_table + (long long)slot * a.table_width;
-  auto page_of = [&](int t) { return t < t_to ? table[t / 2 % a.ring_pages] : 0; };
-  int page = page_of(t_from);
   auto request = [&](int t) {              // tile t into its stage: its keys lie in one page, one behind the other
     if (t < t_to) {
       const int p0 = t * TK, st = (t - t_from) % STAGES;
