@@ -1,6 +1,6 @@
 """Compiles the CUDA sources of this folder for sm_100a and loads them with ctypes.
 
-Each ``.cu`` file becomes one shared library under ``csrc/_build/`` whose name carries a
+Each ``.cu`` file (and the host code in ``.cpp``) becomes one shared library under ``csrc/_build/`` whose name carries a
 hash of its sources, so a changed source is rebuilt and a stale library is never loaded.
 A library is compiled when something first needs it (and all of them by ``build_all``);
 while nvcc runs, a line is printed every few seconds.  There is no fallback: if a library
@@ -25,7 +25,7 @@ from typing import Dict, List
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 
-# library name -> sources (first is the .cu that is compiled; the rest are hashed with it)
+# library name -> sources (first is the file that is compiled; the rest are hashed with it)
 SOURCES: Dict[str, List[str]] = {
     "elementwise": ["elementwise.cu", "common.cuh", "kernel_args.h"],
     "gemm_simt": ["gemm_simt.cu", "common.cuh", "kernel_args.h"],
@@ -54,6 +54,7 @@ SOURCES: Dict[str, List[str]] = {
     "key_weights_mma": ["key_weights_mma.cu", "key_weights.cuh", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "key_weights_tc": ["key_weights_tc.cu", "key_weights.cuh", "umma_tiles.cuh", "tree_tiles.cuh", "common.cuh", "cache_args.h"],
     "cache_rows": ["cache_rows.cu", "common.cuh", "cache_args.h"],
+    "tensor_args": ["tensor_args.cpp"],           # host code against torch's headers (g++)
 }
 
 NVCC_FLAGS = [
@@ -83,12 +84,37 @@ def _nvcc() -> str:
                      "the CUDA kernels cannot be built and there is no other path")
 
 
+def _host_command(source: str) -> List[str]:
+    """g++ for host code that looks into torch's tensors (torch's version and Python's are part of the library's name)."""
+    import sysconfig
+
+    import torch
+    gxx = os.environ.get("CXX") or shutil.which("g++")
+    if not gxx:
+        raise BuildError("g++ was not found (looked at $CXX and PATH); the host library cannot be built and there is no other path")
+    root = os.path.dirname(torch.__file__)
+    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I" + os.path.join(root, "include"),
+            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"),
+            "-I" + sysconfig.get_paths()["include"], os.path.join(_HERE, source), "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+            "-Wl,-rpath," + os.path.join(root, "lib")]
+
+
+def _command(name: str) -> List[str]:
+    source = SOURCES[name][0]
+    return _host_command(source) if source.endswith(".cpp") else [_nvcc(), *NVCC_FLAGS, os.path.join(_HERE, source)]
+
+
 def _digest(name: str) -> str:
     h = hashlib.sha256()
     for src in SOURCES[name]:
         with open(os.path.join(_HERE, src), "rb") as f:
             h.update(src.encode() + b"\0" + f.read() + b"\0")
-    h.update(" ".join(NVCC_FLAGS).encode())
+    if SOURCES[name][0].endswith(".cpp"):
+        import torch
+        h.update(f"{torch.__version__} {sys.version_info[:2]}".encode())
+    else:
+        h.update(" ".join(NVCC_FLAGS).encode())
     return h.hexdigest()[:16]
 
 
@@ -129,9 +155,9 @@ def compile_library(name: str, *, verbose: bool = True) -> str:
             if os.path.isfile(out):
                 return out
             tmp = f"{out}.{os.getpid()}.tmp"
-            cmd = [_nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(_HERE, SOURCES[name][0])]
+            cmd = _command(name) + ["-o", tmp]
             if verbose:
-                _say(f"compiling {SOURCES[name][0]} for sm_100a ...")
+                _say(f"compiling {SOURCES[name][0]}{' for sm_100a' if SOURCES[name][0].endswith('.cu') else ''} ...")
             t0 = time.time()
             env = dict(os.environ)
             env.setdefault("TMPDIR", tempfile.gettempdir())
@@ -149,7 +175,7 @@ def compile_library(name: str, *, verbose: bool = True) -> str:
             if proc.returncode != 0 or not os.path.isfile(tmp):
                 if os.path.exists(tmp):
                     os.unlink(tmp)
-                raise BuildError(f"nvcc failed on {SOURCES[name][0]} (exit {proc.returncode}):\n{log}")
+                raise BuildError(f"{os.path.basename(cmd[0])} failed on {SOURCES[name][0]} (exit {proc.returncode}):\n{log}")
             os.replace(tmp, out)
             if verbose:
                 _say(f"built {os.path.basename(out)} in {time.time() - t0:.1f} s")

@@ -11,7 +11,7 @@ from typing import Optional
 
 import torch
 
-from ..csrc.build import load_library
+from ..csrc.build import compile_library, load_library
 
 F32, BF16 = 0, 1
 PAGE = 64  # tokens per cache page; checked against the library at first use
@@ -2386,18 +2386,24 @@ _sample_scratch = {}
 
 # ---- drafted trees and shortened caches -----------------------------------------------
 
+_tensor_addresses = None
+
+
 def _pointers(what: str, specs) -> list:
-    """Addresses of a call's tensors, each ``(name, tensor, shape, dtype)`` (shape None: any).  They lie on one GPU, the current device, whose
-    current stream the launch goes to, and are contiguous.  (One pass of cheap questions: a call for one short sequence is bound by the host.)"""
+    """Addresses of a call's tensors, a tuple of ``(name, tensor, shape, dtype)`` (shape None: any).  They lie on one GPU, the current device, whose
+    current stream the launch goes to, and are contiguous.  (Looked over in native code: a call for one short sequence is bound by the host.)"""
+    global _tensor_addresses
     dev = specs[0][1].get_device()
     if dev < 0 or dev != (_raw_device() if _raw_device is not None else torch.cuda.current_device()):
         _refuse(what, specs)
-    out = []
-    for name, t, shape, dtype in specs:
-        if (shape is not None and t.shape != shape) or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
-            _refuse(what, specs)
-        out.append(t.data_ptr())
-    return out
+    if _tensor_addresses is None:
+        found = ctypes.PyDLL(compile_library("tensor_args")).llg_tensor_addresses      # (holds the interpreter: it reads Python's objects)
+        found.argtypes = [ctypes.py_object, c_int, c_void_p]
+        _tensor_addresses = found
+    out = (ctypes.c_ulonglong * len(specs))()
+    if _tensor_addresses(specs, dev, out):
+        _refuse(what, specs)
+    return out[:]
 
 
 def _refuse(what: str, specs) -> None:
@@ -2730,7 +2736,7 @@ class CacheRows:
                 raise KernelError(f"CacheRows: weights of shape {tuple(weights.shape)}, expected float32 [{len(self.k)}, slots, {self.nkv}, positions]")
         specs = [("a layer's key pages", t, first.shape, first.dtype) for t in self.k]
         specs += [("a layer's value pages", t, (self.n_pages, self.nkv, PAGE, self.v[0].shape[3]), first.dtype) for t in self.v or ()]
-        addresses = _pointers(what, specs + ([("weights", weights, None, torch.float32)] if weights is not None else []))
+        addresses = _pointers(what, tuple(specs + ([("weights", weights, None, torch.float32)] if weights is not None else [])))
         _wide(what, *addresses)
         self.weights = weights
         n = len(self.k)

@@ -182,3 +182,16 @@ def test_the_plain_forms_agree_with_a_softmax():
     assert T.walk([9, 1, 1, 4], [-1, 0, 0, 2], [1, 4, 4, 6]) == ([0, 1], 4)
     assert T.walk([9, 2, 1, 4], [-1, 0, 0, 2], [1, 0, 4, 6]) == ([0, 2, 3], 6)
     assert T.keep(torch.tensor([1.0, 5.0, 2.0, 5.0, 0.0]), 5, 3, 1, 1) == [0, 1, 4]
+
+
+def test_the_look_over_of_a_calls_tensors_takes_nothing_that_is_not_as_said():
+    """In native code; what is right on a GPU is in the operators' own tests."""
+    build = importlib.import_module("daisi-llogos_b200.csrc.build")
+    look = ctypes.PyDLL(build.compile_library("tensor_args")).llg_tensor_addresses
+    look.argtypes = [ctypes.py_object, ctypes.c_int, ctypes.c_void_p]
+    out = (ctypes.c_ulonglong * 4)(*[7] * 4)
+    t = torch.zeros(3, 4)
+    for specs in ([("t", t, None, F32)], (t,), (("t", t, None),), (("t", 5, None, F32),), (("t", t, None, "float32"),), (("t", t, ("x", 4), F32),),
+                  (("t", t, None, F32),), (("t", t, (3, 4), BF16),), (("t", t.to_sparse(), None, F32),), (("t", t.to("meta"), None, F32),)):
+        assert look(specs, 0, out) == 1
+    assert list(out) == [7] * 4 and look((), 0, out) == 0
