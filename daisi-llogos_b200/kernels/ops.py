@@ -2504,15 +2504,15 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     the launch before it still runs: no kernel of a step writes those."""
     what, dt, i32 = "attn_tree", q.dtype, torch.int32
     n, nh, hd = q.shape
-    n_pages, nkv = k_pages.shape[:2]
-    b, vd = slots.numel(), v_pages.shape[3]
+    n_pages, nkv = k_pages.size(0), k_pages.size(1)
+    b, vd = slots.numel(), v_pages.size(3)
     if plan.key != (dt, b, nh, nkv, hd, vd):
         raise KernelError(f"attn_tree: the plan is for {plan.key}, the call for {(dt, b, nh, nkv, hd, vd)}")
     if not scale > 0:
         raise KernelError("attn_tree: the softmax scale must be positive")
     if page_table.dim() != 2:
         raise KernelError("attn_tree: the page table is int32 [slots, pages]")
-    width = page_table.shape[1]
+    width = page_table.size(1)
     if window < 0 or not 0 < ring_pages <= width:
         raise KernelError(f"attn_tree: window {window}, {ring_pages} ring pages in a table of {width}")
     if ring_pages * PAGE < (min(window + PAGE, plan.max_len) if window > 0 else plan.max_len):
@@ -2583,7 +2583,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
         return
     if logits.dim() != 2:
         raise KernelError(f"tree_accept: logits of shape {tuple(logits.shape)}, expected [nodes, vocabulary]")
-    vocab = logits.shape[1]
+    vocab = logits.size(1)
     if scratch is None or scratch.dtype is not torch.int64 or scratch.numel() < n + b:
         raise KernelError(f"tree_accept: needs {n + b} zeroed int64 of scratch")
     tok, par, cu, to, count, nxt, rows, maxima = _pointers(what, specs + (("logits", logits, (n, vocab), torch.float32),
@@ -2648,14 +2648,14 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     that may run at the same time need their own.  A slot may be in a step once."""
     what, dt, i32 = "key_weights", q.dtype, torch.int32
     n, nh, hd = q.shape
-    n_pages, nkv = k_pages.shape[:2]
+    n_pages, nkv = k_pages.size(0), k_pages.size(1)
     b = slots.numel()
     if plan.key != (dt, b, nh, nkv, hd) or plan.last != last:
         raise KernelError(f"key_weights: the plan is for {plan.key} and {plan.last} queries, the call for {(dt, b, nh, nkv, hd)} and {last}")
     if weights.dim() != 3 or page_table.dim() != 2:
         raise KernelError(f"key_weights: weights of shape {tuple(weights.shape)}, expected [slots, heads, positions]")
     n_slots, width = page_table.shape
-    positions = weights.shape[2]
+    positions = weights.size(2)
     if plan.max_len > positions or plan.max_len > width * PAGE:
         raise KernelError(f"key_weights: {plan.max_len} keys, {positions} weights a row and {width} pages")
     if not scale > 0:
@@ -2704,7 +2704,7 @@ def keep_keys(weights: torch.Tensor, slots: torch.Tensor, lengths: torch.Tensor,
     if weights.dim() != 4 or chosen.dim() != 4:
         raise KernelError("keep_keys: weights are [layers, slots, heads, positions], the chosen [layers, sequences, heads, most]")
     layers, n_slots, nkv, width = weights.shape
-    b, most = slots.numel(), chosen.shape[3]
+    b, most = slots.numel(), chosen.size(3)
     bound = width if max_len is None else int(max_len)
     if not 0 < bound <= width:
         raise KernelError(f"keep_keys: lengths up to {bound} in rows of {width} weights")
@@ -2761,20 +2761,19 @@ class CacheRows:
         shape = source.shape
         if len(shape) != 4 or shape[0] not in (1, n) or shape[1] != b or shape[2] not in (1, self.nkv):
             raise KernelError(f"CacheRows.move: sources of shape {tuple(shape)}, expected int32 [1 or {n}, {b}, 1 or {self.nkv}, places]")
-        if page_table.dim() != 2 or not 0 < ring_pages <= page_table.shape[1]:
+        layers, _, heads, width = shape
+        if page_table.dim() != 2 or not 0 < ring_pages <= page_table.size(1):
             raise KernelError(f"CacheRows.move: {ring_pages} ring pages in a page table of shape {tuple(page_table.shape)}")
-        if self.weights is not None and self.weights.shape[1] != page_table.shape[0]:
+        if self.weights is not None and self.weights.size(1) != page_table.size(0):
             raise KernelError(f"CacheRows.move: weights of {self.weights.shape[1]} slots, a page table of {page_table.shape[0]}")
-        a = _MoveArgs()
-        ctypes.pointer(a)[0] = self.args
+        a = _MoveArgs.from_buffer_copy(self.args)
         a.page_table, a.slots, a.base, a.source, a.count, _ = _pointers(what, (
             ("page_table", page_table, None, i32), ("slots", slots, (b,), i32), ("base", base, (b,), i32), ("source", source, None, i32),
             ("count", count, (b,), i32), ("pools", self.pools, None, torch.int64)))
-        a.table_width, a.ring_pages = page_table.shape[1], ring_pages
-        width = source.shape[3]
-        a.source_seq = source.shape[2] * width
-        a.source_layer = b * a.source_seq if source.shape[0] > 1 else 0
-        a.source_head = width if source.shape[2] > 1 else 0
+        a.table_width, a.ring_pages = page_table.size(1), ring_pages
+        a.source_seq = heads * width
+        a.source_layer = b * heads * width if layers > 1 else 0
+        a.source_head = width if heads > 1 else 0
         a.n_seqs, a.most = b, width
         lib = _lib("cache_rows")
         _check(lib, lib.llg_move_rows(byref(a), _stream()))
