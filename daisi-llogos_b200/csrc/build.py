@@ -89,11 +89,11 @@ def _host_command(source: str) -> List[str]:
     import sysconfig
 
     import torch
-    gxx = os.environ.get("CXX") or shutil.which("g++")
+    gxx = shutil.which(os.environ.get("CXX") or "g++") or shutil.which("g++")
     if not gxx:
         raise BuildError("g++ was not found (looked at $CXX and PATH); the host library cannot be built and there is no other path")
     root = os.path.dirname(torch.__file__)
-    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    return [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
             "-I" + os.path.join(root, "include"),
             "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"),
             "-I" + sysconfig.get_paths()["include"], os.path.join(_HERE, source), "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
