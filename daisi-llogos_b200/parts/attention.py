@@ -267,10 +267,11 @@ class Attention(Mixer):
         form_kw = {"form": self.form} if self.form is not None else {}
 
         def planned(make, name, *sizes, **kw):
-            # (the same for all layers of the same sizes: worked out once a step)
-            plan = ctx.extras.get((name, *sizes))
+            # (the same for all layers of the same sizes and the same value size, which a decode plan has from the form: worked out once a step)
+            key = (name, *sizes, self.vd)
+            plan = ctx.extras.get(key)
             if plan is None:
-                plan = ctx.extras[(name, *sizes)] = make(ctx.dtype, *sizes, **kw)
+                plan = ctx.extras[key] = make(ctx.dtype, *sizes, **kw)
             return (plan, ctx.buffer(f"attn.{name}", (max(1, plan.scratch_floats),), torch.float32),
                     ctx.buffer(f"attn.{name}.counters", (max(1, plan.n_counters),), torch.int32, zero=True))
 
