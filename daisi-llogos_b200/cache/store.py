@@ -325,6 +325,18 @@ class SequenceCache:
             out.append((g, ups))
         return out
 
+    def ungrow(self, growth: Sequence[Tuple[int, int]], updates) -> None:
+        """Behind a ``grow`` (which returned ``updates``) whose step failed: exactly its pages go back, so that whoever has them next writes
+        their table entries anew.  What the step wrote counts for what a ring has overwritten (``truncate``)."""
+        for g, ups in updates:
+            for at, page in reversed(ups):
+                held = g.pages_of[at // g.table_width]
+                if held.pop() != page:
+                    raise CacheError(f"page {page} is not the last one that slot {at // g.table_width} got")
+            g.pool.give([page for _, page in ups])
+        for slot, add in growth:
+            self._longest[slot] = max(self.slots.length[slot] + add, self._longest.get(slot, 0))
+
     def commit(self, growth: Sequence[Tuple[int, int]]) -> None:
         for slot, add in growth:
             self.slots.length[slot] += add

@@ -245,13 +245,18 @@ class Engine:
         except CacheError as e:
             raise StepError(str(e)) from None
         host: List[np.ndarray] = []
-        plan = self._apply_updates(self.cache.grow(growth), host)
-        if plan:
-            block = np.concatenate(host)
-            meta = self._ensure_meta(block.size)
-            self._staging.upload(block, meta)
-            for g, off, k in plan:
-                self.ops.scatter_i32(g.page_table, meta[off:off + k], meta[off + k:off + 2 * k])
+        updates = self.cache.grow(growth)
+        try:
+            plan = self._apply_updates(updates, host)
+            if plan:
+                block = np.concatenate(host)
+                meta = self._ensure_meta(block.size)
+                self._staging.upload(block, meta)
+                for g, off, k in plan:
+                    self.ops.scatter_i32(g.page_table, meta[off:off + k], meta[off + k:off + 2 * k])
+        except BaseException:
+            self.cache.ungrow(growth, updates)
+            raise
         self.cache.commit(growth)
 
     # ---- the step ------------------------------------------------------------------------
@@ -326,10 +331,14 @@ class Engine:
         updates = self.cache.grow(growth)
         b = len(slots)
         decode = all(c == 1 for c in counts)
-        if decode:
-            logits = self._decode_step(b, slots, toks, len_before, updates, want, fed)
-        else:
-            logits = self._prompt_step(b, slots, toks, counts, len_before, updates, want)
+        try:
+            if decode:
+                logits = self._decode_step(b, slots, toks, len_before, updates, want, fed)
+            else:
+                logits = self._prompt_step(b, slots, toks, counts, len_before, updates, want)
+        except BaseException:
+            self.cache.ungrow(growth, updates)       # (pages whose entries may not have reached the table)
+            raise
         self.cache.commit(growth)
         return logits
 

@@ -125,7 +125,7 @@ class TreeSteps:
         return slots, toks, parents
 
     def step(self, entries) -> torch.Tensor:
-        from .engine import StepError, length_bucket
+        from .engine import StepError
         e = self.engine
         slots, toks, parents = self._check(entries)
         self.drop()
@@ -143,6 +143,18 @@ class TreeSteps:
         if limit is not None and longest > limit:
             raise StepError(f"a sequence would reach {longest} tokens, the position tables hold {limit}")
         updates = e.cache.grow(growth)
+        try:
+            meta, logits = self._launch(slots, toks, parents, counts, len_before, bits, depth, updates)
+        except BaseException:
+            e.cache.ungrow(growth, updates)          # (pages whose entries may not have reached the table)
+            raise
+        self.pending = _Pending(slots, counts, len_before, [t.tolist() for t in toks], self._views(meta, sum(counts), len(slots)), logits)
+        return logits
+
+    def _launch(self, slots, toks, parents, counts, len_before, bits, depth, updates):
+        """Uploads a checked step and runs it: its integers on the device and its logits."""
+        from .engine import length_bucket
+        e = self.engine
         n, b = sum(counts), len(slots)
         cu = np.zeros(b + 1, dtype=np.int32)
         np.cumsum(counts, out=cu[1:])
@@ -166,14 +178,7 @@ class TreeSteps:
         if rec is not None:
             rec.meta.copy_(meta[:fixed], non_blocking=True)
             meta = rec.meta
-        try:
-            logits = self._run(rec, meta, n, b, counts, bound)
-        except Exception:
-            for slot, lb, c in zip(slots, len_before, counts):
-                e.cache.settle(slot, lb, lb + c)
-            raise
-        self.pending = _Pending(slots, counts, len_before, [t.tolist() for t in toks], self._views(meta, n, b), logits)
-        return logits
+        return meta, self._run(rec, meta, n, b, counts, bound)
 
     @staticmethod
     def _views(meta: torch.Tensor, n: int, b: int) -> Dict[str, torch.Tensor]:

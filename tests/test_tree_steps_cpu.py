@@ -36,3 +36,46 @@ def test_layers_of_two_value_sizes_have_a_decode_plan_each(llogos, monkeypatch):
     eng.step([(slot, [1, 2, 3])])
     eng.step([(slot, [4])])
     assert seen == [(64, 64), (32, 32)]
+
+
+class Failure(Exception):
+    pass
+
+
+def table_is_the_hosts(eng):
+    """Every page that a sequence has stands in the table that the kernels read."""
+    for g in eng.cache.kv_groups:
+        for slot, pages in g.pages_of.items():
+            assert g.page_table[slot, :len(pages)].tolist() == pages
+    eng.cache.audit()
+
+
+@pytest.mark.parametrize("name", ["llama", "qwen3"])
+@pytest.mark.parametrize("where", ["upload", "meta", "scatter", "forward"])
+@pytest.mark.parametrize("kind", ["tree", "prompt", "decode", "assume"])
+def test_a_step_that_fails_leaves_no_page_without_its_entry(llogos, model_dirs, monkeypatch, name, where, kind):
+    """Pages that a step took and whose entries never reached the table went to the next step, which wrote through what stood there before: another
+    sequence's page.  In rings too, whose pages a step of more tokens than they hold takes all at once."""
+    if kind == "assume" and where == "forward":
+        pytest.skip("nothing runs")
+    model = llogos.weights.load_model(model_dirs[name], dtype=torch.float32, device="cpu", ops=tree_ops)
+    eng = engine_for(llogos, model)
+    other, slot = eng.open(), eng.open()
+    eng.step([(other, [3] * 100), (slot, [1] * 64)], [[], []])
+    free = [g.pool.free_count for g in eng.cache.kv_groups]
+    act = {"tree": lambda: eng.step_tree([(slot, [1, 2, 3], [-1, 0, 0])]), "prompt": lambda: eng.step([(slot, [4] * 130)]),
+           "decode": lambda: eng.step([(slot, [4])]), "assume": lambda: eng.assume(slot, 200)}[kind]
+
+    def fails(*args, **kw):
+        raise Failure
+
+    with monkeypatch.context() as m:
+        target = {"upload": (eng._staging, "upload"), "meta": (eng, "_ensure_meta"), "scatter": (tree_ops, "scatter_i32"),
+                  "forward": (model, "forward")}[where]
+        m.setattr(*target, fails)
+        with pytest.raises(Failure):
+            act()
+    assert [g.pool.free_count for g in eng.cache.kv_groups] == free and eng.length(slot) == 64
+    table_is_the_hosts(eng)
+    act()
+    table_is_the_hosts(eng)
