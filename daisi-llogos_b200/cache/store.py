@@ -154,16 +154,16 @@ class KvGroup:
     def shrink(self, slot: int, old_len: int, new_len: int) -> None:
         """Gives back the pages beyond ``new_len`` tokens.  A ring that has gone round keeps all of its pages:
         their order in the table is no longer their age."""
-        if pages_for(old_len) > self.ring_pages:
-            return
+        keep = self.pages_left(slot, old_len, new_len)
         have = self.pages_of.get(slot, [])
-        keep = self.pages_needed(new_len)
         if len(have) > keep:
             self.pool.give(have[keep:])
             del have[keep:]
 
-    def extra_pages(self, slot: int, new_len: int) -> int:
-        return max(0, self.pages_needed(new_len) - len(self.pages_of.get(slot, [])))
+    def pages_left(self, slot: int, old_len: int, new_len: int) -> int:
+        """How many pages a sequence has behind ``shrink``."""
+        have = len(self.pages_of.get(slot, []))
+        return have if pages_for(old_len) > self.ring_pages else min(have, self.pages_needed(new_len))
 
     def release(self, slot: int) -> None:
         pages = self.pages_of.pop(slot, [])
@@ -244,6 +244,19 @@ class SequenceCache:
         Inference/KvCache.cs:135); pages that hold none of the rest go back to the pool.  Refused, with
         nothing changed, where the past cannot be restored: fixed-size state, or a window whose older
         keys the ring has overwritten."""
+        self.check_truncate(slot, new_len)
+        old = self.slots.length[slot]
+        if new_len == old:
+            return
+        written = max(old, self._longest.get(slot, 0))
+        for g in self.kv_groups:
+            g.shrink(slot, written, new_len)
+        self._longest[slot] = written
+        self.slots.length[slot] = new_len
+
+    def check_truncate(self, slot: int, new_len: int, written: int = 0) -> None:
+        """Raises what ``truncate`` raises, nothing else; ``written``: tokens that the sequence's pages have held besides (a step that was not
+        committed)."""
         self.slots.check_live(slot)
         old = self.slots.length[slot]
         if not 0 <= new_len <= old:
@@ -253,15 +266,11 @@ class SequenceCache:
         if self.state:
             raise CacheError(f"slot {slot}: fixed-size state cannot be rolled back")
         # what a ring has overwritten follows from the longest the sequence has ever been
-        written = max(old, self._longest.get(slot, 0))
+        written = max(old, written, self._longest.get(slot, 0))
         for g in self.kv_groups:
             if not g.can_shrink(written, new_len):
                 raise CacheError(f"slot {slot}: the window of {g.window} keys before position {new_len} has been "
                                  f"overwritten (the sequence has held {written} tokens)")
-        for g in self.kv_groups:
-            g.shrink(slot, written, new_len)
-        self._longest[slot] = written
-        self.slots.length[slot] = new_len
 
     # ---- drafted tokens, and keys that are taken out -------------------------------------
     def weigh_keys(self) -> None:
@@ -295,8 +304,9 @@ class SequenceCache:
             g.shrink(slot, old, new_len)
         self.slots.length[slot] = new_len
 
-    def check_room(self, growth: Sequence[Tuple[int, int]]) -> None:
-        """``growth`` = (slot, tokens to add) for a whole step; raises before anything changes."""
+    def check_room(self, growth: Sequence[Tuple[int, int]], forget: Sequence[Tuple[int, int]] = ()) -> None:
+        """``growth`` = (slot, tokens to add) for a whole step; raises before anything changes.  ``forget`` = (slot, tokens written) of a step that
+        was not committed and that the new one will forget (``settle``): what it reserved counts as free."""
         seen = set()
         for slot, add in growth:
             self.slots.check_live(slot)
@@ -310,10 +320,13 @@ class SequenceCache:
                 raise CacheError(
                     f"slot {slot}: {new_len} tokens exceed the longest sequence the cache holds ({self.max_seq_len})")
         for g in self.kv_groups:
-            extra = sum(g.extra_pages(s, self.slots.length[s] + add) for s, add in growth)
-            if extra > g.pool.free_count:
+            left = {s: g.pages_left(s, max(written, self._longest.get(s, 0)), self.slots.length[s]) for s, written in forget}
+            held = {s: len(g.pages_of.get(s, [])) for s in (*left, *seen)}
+            extra = sum(max(0, g.pages_needed(self.slots.length[s] + add) - left.get(s, held[s])) for s, add in growth)
+            free = g.pool.free_count + sum(held[s] - n for s, n in left.items())
+            if extra > free:
                 raise CacheError(
-                    f"cache full: the step needs {extra} more pages of {PAGE} tokens, {g.pool.free_count} are free")
+                    f"cache full: the step needs {extra} more pages of {PAGE} tokens, {free} are free")
 
     def grow(self, growth: Sequence[Tuple[int, int]]) -> List[Tuple[KvGroup, List[Tuple[int, int]]]]:
         """Reserves pages for a step (after ``check_room``); lengths advance in ``commit``."""

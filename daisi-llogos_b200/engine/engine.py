@@ -191,19 +191,21 @@ class Engine:
 
     def close(self, slot: int) -> None:
         """Ends a sequence: its slot and pages go back to the free lists."""
+        self.cache.length(slot)              # (raises where the slot is not in use)
         self.trees.drop()
         self.cache.release(slot)
 
     def truncate(self, slot: int, length: int) -> None:
         """Forgets a sequence's keys from place ``length`` on; the next step continues there.  Of a sequence that keys were taken out of, only
         tokens that came later can be forgotten."""
-        self.trees.drop()
         if length < self._kept.get(slot, 0):
             raise StepError(f"slot {slot}: {self._kept[slot]} keys were left by an eviction, cannot truncate to {length}")
         try:
-            self.cache.truncate(slot, length)
+            self.cache.check_truncate(slot, length, dict(self.trees.uncommitted()).get(slot, 0))
         except CacheError as e:
             raise StepError(str(e)) from None
+        self.trees.drop()
+        self.cache.truncate(slot, length)
 
     def length(self, slot: int) -> int:
         """Keys that the sequence holds."""
@@ -218,7 +220,7 @@ class Engine:
         """Runs a tree of drafted tokens for every ``(slot, tokens, parents)`` entry; returns float32 logits of all nodes, ``[nodes, vocab]``, in
         the entries' order.  ``tokens[0]`` is the sequence's last certain token (what a decode step would be given), ``parents[0]`` -1;
         ``parents[i] < i`` is the node that node i follows.  Up to 64 nodes a tree.  No length changes: ``accept_tree`` says which path
-        stays; another step, ``truncate`` or ``close`` forgets the trees.  The logits are valid until the next step."""
+        stays; another step, ``truncate`` or ``close`` forgets the trees (one that is refused does not).  The logits are valid until the next step."""
         return self.trees.step(entries)
 
     def accept_tree(self, picked: Optional[torch.Tensor] = None):
@@ -239,11 +241,11 @@ class Engine:
         reserved and the length advances, the keys and values are whatever the pages hold.  For
         measurements of a step at a given context length; results after it mean nothing."""
         growth = [(int(slot), int(n_tokens))]
-        self.trees.drop()
         try:
-            self.cache.check_room(growth)
+            self.cache.check_room(growth, self.trees.uncommitted())
         except CacheError as e:
             raise StepError(str(e)) from None
+        self.trees.drop()
         host: List[np.ndarray] = []
         updates = self.cache.grow(growth)
         try:
@@ -317,9 +319,8 @@ class Engine:
 
     def _run(self, slots, toks, counts, want, fed) -> torch.Tensor:
         growth = list(zip(slots, counts))
-        self.trees.drop()
         try:
-            self.cache.check_room(growth)
+            self.cache.check_room(growth, self.trees.uncommitted())
         except CacheError as e:
             raise StepError(str(e)) from None
 
@@ -328,6 +329,7 @@ class Engine:
         limit = self.model.position_limit()
         if limit is not None and longest > limit:
             raise StepError(f"a sequence would reach {longest} tokens, the position tables hold {limit}")
+        self.trees.drop()
         updates = self.cache.grow(growth)
         b = len(slots)
         decode = all(c == 1 for c in counts)

@@ -95,6 +95,11 @@ class TreeSteps:
             for slot, lb, c in zip(p.slots, p.len_before, p.counts):
                 self.engine.cache.settle(slot, lb, lb + c)
 
+    def uncommitted(self) -> List[Tuple[int, int]]:
+        """Per slot of a tree step that was not accepted the tokens that its pages hold, the nodes included."""
+        p = self.pending
+        return [] if p is None else [(slot, lb + c) for slot, lb, c in zip(p.slots, p.len_before, p.counts)]
+
     def _check(self, entries):
         from .engine import StepError
         e = self.engine
@@ -128,11 +133,10 @@ class TreeSteps:
         from .engine import StepError
         e = self.engine
         slots, toks, parents = self._check(entries)
-        self.drop()
         counts = [int(t.size) for t in toks]
         growth = list(zip(slots, counts))
         try:
-            e.cache.check_room(growth)
+            e.cache.check_room(growth, self.uncommitted())
         except CacheError as err:
             raise StepError(str(err)) from None
         len_before = [e.cache.length(s) for s in slots]
@@ -142,6 +146,7 @@ class TreeSteps:
         longest = max(lb + max(d) + 1 for lb, d in zip(len_before, depth))
         if limit is not None and longest > limit:
             raise StepError(f"a sequence would reach {longest} tokens, the position tables hold {limit}")
+        self.drop()
         updates = e.cache.grow(growth)
         try:
             meta, logits = self._launch(slots, toks, parents, counts, len_before, bits, depth, updates)

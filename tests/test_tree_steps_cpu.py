@@ -79,3 +79,39 @@ def test_a_step_that_fails_leaves_no_page_without_its_entry(llogos, model_dirs, 
     table_is_the_hosts(eng)
     act()
     table_is_the_hosts(eng)
+
+
+@pytest.mark.parametrize("name", ["llama", "qwen3"])
+def test_a_refused_call_forgets_no_tree(llogos, model_dirs, name):
+    """Another step, truncate and close forget a tree that was not accepted; one that is refused changes nothing."""
+    E = llogos.engine.StepError
+    model = llogos.weights.load_model(model_dirs[name], dtype=torch.float32, device="cpu", ops=tree_ops)
+    eng = engine_for(llogos, model, max_tokens=64 * 4, max_seq_len=64 * 4, n_slots=3)
+    slot, other = eng.open(), eng.open()
+    eng.step([(slot, [1] * 60), (other, [2] * 60)], [[], []])
+    eng.step_tree([(slot, [1, 2, 3], [-1, 0, 1])])
+    for call, error in ((lambda: eng.truncate(other, 61), E), (lambda: eng.truncate(2, 1), E),
+                        (lambda: eng.close(2), RuntimeError), (lambda: eng.close(7), RuntimeError), (lambda: eng.step([(2, [1])]), E),
+                        (lambda: eng.step([(slot, [1] * 300)]), E), (lambda: eng.step([(other, [1] * 190)]), E), (lambda: eng.assume(2, 5), E),
+                        (lambda: eng.step_tree([(2, [1], [-1])]), E), (lambda: eng.step_tree([(slot, [1], [0])]), E),
+                        (lambda: eng.step_tree([(slot, [1], [-1]), (slot, [1], [-1])]), E)):
+        with pytest.raises(error):
+            call()
+        assert eng.trees.pending is not None and eng.length(slot) == 60
+    best = torch.tensor([2, 3, 9], dtype=torch.int32)
+    assert eng.accept_tree(best) == [([0, 1, 2], 9)] and eng.length(slot) == 63
+    eng.cache.audit()
+
+
+def test_a_forgotten_trees_pages_count_as_free(llogos, model_dirs):
+    """The pages of a tree that a step will forget are there for that step: for its own sequence and for another."""
+    model = llogos.weights.load_model(model_dirs["llama"], dtype=torch.float32, device="cpu", ops=tree_ops)
+    for own in (True, False):
+        eng = engine_for(llogos, model, max_tokens=64 * 3, max_seq_len=64 * 3, n_slots=2)
+        slot, other = eng.open(), eng.open()
+        eng.step([(slot, [1] * 60), (other, [2] * 60)], [[], []])
+        eng.step_tree([(slot, [1] * 20, [-1] + [0] * 19)])
+        assert eng.cache.free_pages() == 0
+        eng.step([(slot if own else other, [1] * 20)])
+        assert (eng.length(slot), eng.length(other)) == ((80, 60) if own else (60, 80))
+        table_is_the_hosts(eng)
