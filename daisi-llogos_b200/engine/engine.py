@@ -198,7 +198,7 @@ class Engine:
     def truncate(self, slot: int, length: int) -> None:
         """Forgets a sequence's keys from place ``length`` on; the next step continues there.  Of a sequence that keys were taken out of, only
         tokens that came later can be forgotten."""
-        if length < self._kept.get(slot, 0):
+        if slot in self._kept and length < self._kept[slot]:
             raise StepError(f"slot {slot}: {self._kept[slot]} keys were left by an eviction, cannot truncate to {length}")
         try:
             self.cache.check_truncate(slot, length, dict(self.trees.uncommitted()).get(slot, 0))

@@ -115,3 +115,15 @@ def test_a_forgotten_trees_pages_count_as_free(llogos, model_dirs):
         eng.step([(slot if own else other, [1] * 20)])
         assert (eng.length(slot), eng.length(other)) == ((80, 60) if own else (60, 80))
         table_is_the_hosts(eng)
+
+
+def test_a_truncation_to_a_negative_length_is_refused(llogos, model_dirs):
+    model = llogos.weights.load_model(model_dirs["llama"], dtype=torch.float32, device="cpu", ops=tree_ops)
+    eng = engine_for(llogos, model, weigh_keys=1)
+    slot = eng.open()
+    eng.step([(slot, [1] * 10)], [[]])
+    for says in ("cannot truncate 10 tokens", "6 keys were left by an eviction"):
+        with pytest.raises(llogos.engine.StepError, match=says):
+            eng.truncate(slot, -1)
+        eng.evict([(slot, 6)], first=1, recent=1) if eng.length(slot) == 10 else None
+    assert eng.length(slot) == 6
