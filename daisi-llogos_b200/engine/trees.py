@@ -21,6 +21,7 @@ from ..parts.base import Mixer
 from .context import StepContext, Workspace
 
 RECORDED_SIZES = 8       # tree sizes whose buffers and graph are kept; the ones used longest ago make room
+RECORDED_BYTES = 1 << 30      # and what their buffers may take together: logits of 512 nodes over 128,256 ids alone are 263 MB
 
 
 class _Pending:
@@ -59,6 +60,7 @@ class TreeSteps:
         self.pending: Optional[_Pending] = None
         self._seen: Dict[tuple, int] = {}
         self._recorded: Dict[tuple, _Recorded] = {}
+        self._large = set()              # sizes whose buffers alone are more than RECORDED_BYTES
         self._accept: Dict[int, Tuple[torch.Tensor, ...]] = {}
 
     @property
@@ -183,7 +185,10 @@ class TreeSteps:
         if rec is not None:
             rec.meta.copy_(meta[:fixed], non_blocking=True)
             meta = rec.meta
-        return meta, self._run(rec, meta, n, b, counts, bound)
+        logits = self._run(rec, meta, n, b, counts, bound)
+        if rec is not None:
+            self._make_room(key, rec)
+        return meta, logits
 
     @staticmethod
     def _views(meta: torch.Tensor, n: int, b: int) -> Dict[str, torch.Tensor]:
@@ -198,6 +203,8 @@ class TreeSteps:
         """Buffers of their own for sizes that have come before."""
         rec = self._recorded.pop(key, None)
         if rec is None:
+            if key in self._large:
+                return None
             if len(self._seen) > 256:
                 self._seen.clear()
             self._seen[key] = self._seen.get(key, 0) + 1
@@ -208,6 +215,17 @@ class TreeSteps:
             rec = _Recorded(ints, self.engine.device)
         self._recorded[key] = rec
         return rec
+
+    def _make_room(self, key, rec: _Recorded) -> None:
+        """The sizes used longest ago go until the buffers of the rest are no more than they may be."""
+        if rec.workspace.bytes() > RECORDED_BYTES:
+            if len(self._large) > 256:
+                self._large.clear()
+            self._large.add(key)
+            del self._recorded[key]
+            return
+        while sum(r.workspace.bytes() for r in self._recorded.values()) > RECORDED_BYTES:
+            del self._recorded[next(iter(self._recorded))]
 
     def _run(self, rec: Optional[_Recorded], meta, n, b, counts, bound) -> torch.Tensor:
         e = self.engine

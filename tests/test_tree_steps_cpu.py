@@ -127,3 +127,40 @@ def test_a_truncation_to_a_negative_length_is_refused(llogos, model_dirs):
             eng.truncate(slot, -1)
         eng.evict([(slot, 6)], first=1, recent=1) if eng.length(slot) == 10 else None
     assert eng.length(slot) == 6
+
+
+def test_what_tree_steps_are_recorded_in_is_bounded_in_bytes(llogos, model_dirs, monkeypatch):
+    """Sizes that come again have buffers of their own (their logits among them): the ones used longest ago make room, and sizes that are too
+    large by themselves have none."""
+    import importlib
+    trees = importlib.import_module("daisi-llogos_b200.engine.trees")
+    model = llogos.weights.load_model(model_dirs["llama"], dtype=torch.float32, device="cpu", ops=tree_ops)
+
+    def twice(eng, slot, n):
+        for _ in range(2):                                 # (the third of a size would be recorded on a GPU)
+            eng.step_tree([(slot, [1] * n, [-1] + [0] * (n - 1))])
+        return eng.trees._recorded
+
+    def made(limit):
+        monkeypatch.setattr(trees, "RECORDED_BYTES", limit)
+        eng = engine_for(llogos, model)
+        eng.use_graphs = True
+        slot = eng.open()
+        eng.step([(slot, [1, 2, 3])], [[]])
+        return eng, slot
+
+    eng, slot = made(1 << 40)
+    for n in (4, 8, 9):
+        kept = twice(eng, slot, n)
+    size = {key[0][0]: rec.workspace.bytes() for key, rec in kept.items()}
+    assert sorted(size) == [4, 8, 9] and size[4] >= 4 * 4 * 256        # logits of four nodes over 256 ids
+    eng, slot = made(size[8] + size[9] + 1000)
+    for n in (4, 8, 9):
+        kept = twice(eng, slot, n)
+        assert sum(r.workspace.bytes() for r in kept.values()) <= trees.RECORDED_BYTES
+    assert [key[0] for key in kept] == [(8,), (9,)]
+    eng, slot = made(size[8] - 1)
+    assert [key[0] for key in twice(eng, slot, 4)] == [(4,)]
+    for _ in range(2):
+        assert [key[0] for key in twice(eng, slot, 8)] == [(4,)]       # too large by itself, and nobody makes room for it
+    assert eng.accept_tree(torch.zeros(8, dtype=torch.int32)) == [([0], 0)]
