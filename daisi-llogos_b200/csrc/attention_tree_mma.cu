@@ -426,9 +426,11 @@ long long scratch_of(int blocks, int wr) {
 
 }  // namespace
 
-// 1 when this kernel takes the geometry (bfloat16 only).
-LLG_API int llg_attn_tree_mma_supported(int hd, int vd, int n_seqs) {
-  return hd >= 8 && hd <= 128 && hd % 8 == 0 && vd >= 8 && vd <= 128 && vd % 8 == 0 && n_seqs <= MAX_SEQS;
+// 1 when this kernel takes the geometry (bfloat16 only): trees of up to `rows` query rows per key/value head.
+LLG_API int llg_attn_tree_mma_supported(int hd, int vd, int n_seqs, int rows, int nkv, int max_len) {
+  const int per = 16 * row_warps(rows);
+  return hd >= 8 && hd <= 128 && hd % 8 == 0 && vd >= 8 && vd <= 128 && vd % 8 == 0 && n_seqs <= MAX_SEQS &&
+         list_fits(n_seqs, nkv, (rows + per - 1) / per, max_len, 1, 0);
 }
 
 // Floats of scratch of a launch over trees of up to `rows` query rows per key/value head and sequences of up to `max_len` positions.
@@ -440,8 +442,9 @@ LLG_API long long llg_attn_tree_mma_scratch_floats(int n_seqs, int rows, int nkv
 LLG_API int llg_attn_tree_mma(const TreeArgs* args, cudaStream_t stream) {
   const TreeArgs& a = *args;
   if (check_tree(a, "attn_tree_mma")) return 1;
-  LLG_REQUIRE(llg_attn_tree_mma_supported(a.hd, a.vd, a.n_seqs), "attn_tree_mma: heads of %d and %d elements (steps of 8 up to 128)", a.hd, a.vd);
   if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
+  LLG_REQUIRE(llg_attn_tree_mma_supported(a.hd, a.vd, a.n_seqs, a.max_nodes * (a.nh / a.nkv), a.nkv, a.max_len),
+              "attn_tree_mma: heads of %d and %d elements (steps of 8 up to 128), %d sequences of up to %d positions", a.hd, a.vd, a.n_seqs, a.max_len);
   CUtensorMap mk, mv;
   const long long rows = (long long)a.n_pages * a.nkv * TK;
   if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv))

@@ -672,9 +672,11 @@ int launch(const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cons
 
 }  // namespace
 
-// 1 when this kernel takes the geometry (bfloat16 only).
-LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs, int group) {
-  return (hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS && group <= BQ;
+// 1 when this kernel takes the geometry (bfloat16 only): trees of up to `nodes` nodes.
+LLG_API int llg_attn_tree_tc_supported(int hd, int vd, int n_seqs, int group, int nodes, int nkv, int max_len) {
+  if (!((hd == 64 || hd == 128) && vd == hd && n_seqs <= MAX_SEQS && group >= 1 && group <= BQ)) return 0;
+  const int per = query_tiles(nodes, group) * (BQ / group);
+  return list_fits(n_seqs, nkv, (nodes + per - 1) / per, max_len, PLAIN_WEIGHT, SEGMENT_WEIGHT);
 }
 
 // Floats of scratch of a launch over trees of up to `nodes` nodes and sequences of up to `max_len` positions.
@@ -693,9 +695,10 @@ LLG_API long long llg_attn_tree_tc_scratch_floats(int n_seqs, int nodes, int nkv
 LLG_API int llg_attn_tree_tc(const TreeArgs* args, cudaStream_t stream) {
   const TreeArgs& a = *args;
   if (check_tree(a, "attn_tree_tc")) return 1;
-  LLG_REQUIRE(llg_attn_tree_tc_supported(a.hd, a.vd, a.n_seqs, a.nh / a.nkv),
-              "attn_tree_tc: heads of %d and %d elements (64 or 128, the same), %d of them a group (at most %d)", a.hd, a.vd, a.nh / a.nkv, BQ);
   if (a.n_seqs <= 0 || a.n_tokens <= 0) return 0;
+  LLG_REQUIRE(llg_attn_tree_tc_supported(a.hd, a.vd, a.n_seqs, a.nh / a.nkv, a.max_nodes, a.nkv, a.max_len),
+              "attn_tree_tc: heads of %d and %d elements (64 or 128, the same), %d of them a group (at most %d), %d sequences of up to %d positions", a.hd, a.vd,
+              a.nh / a.nkv, BQ, a.n_seqs, a.max_len);
   CUtensorMap mk, mv, mq;
   const long long rows = (long long)a.n_pages * a.nkv * TK;
   if (!page_map(a.k_pages, rows, a.hd, &mk) || !page_map(a.v_pages, rows, a.vd, &mv) || !query_map(a.q, a.n_tokens, a.nh, a.hd, a.nh / a.nkv, BQ / (a.nh / a.nkv), &mq))

@@ -90,7 +90,7 @@ struct TreeShape {
 // The work of a launch is one list: sequence by sequence, key/value head by key/value head, row block by row block, key tile by key tile.
 // Blocks cut it into equal runs.  Every block works the list out itself, in shared memory: per sequence the units, the row blocks and the weight of
 // one head in the sequences before it, and what there is to know of the first STAGED sequences.  (Counts are 32-bit: a division of 64
-// bits takes a hundred instructions, and a block's begin is a chain of them; the host refuses launches whose list is longer.)
+// bits takes a hundred instructions, and a block's begin is a chain of them; calls whose list is longer go to another kernel, see list_fits.)
 constexpr int STAGED = 128;
 struct Plan {
   int sums[MAX_SEQS + 1], blocks[MAX_SEQS + 1];
@@ -310,6 +310,12 @@ inline bool page_map(const void* base, long long rows, int hd, CUtensorMap* resu
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whether a launch's list of work, `per_tile` for each key tile of a row block and `per_block` for each row block, fits the kernels' 32-bit counts if
+// every sequence is as long as it may be (a block's end lies up to a run behind the list's: a million blocks' worth of room).
+inline bool list_fits(long long n_seqs, long long nkv, long long row_blocks, long long max_len, long long per_tile, long long per_block) {
+  return (per_tile * ((max_len + TK - 1) / TK) + per_block) * row_blocks < ((1LL << 31) - (1LL << 20)) / (nkv * n_seqs);
+}
+
 // What a launch wants of its arguments.
 inline int check_tree(const TreeArgs& a, const char* what) {
   LLG_REQUIRE(a.nh > 0 && a.nkv > 0 && a.nh % a.nkv == 0, "%s: %d heads are no multiple of %d key/value heads", what, a.nh, a.nkv);
@@ -319,9 +325,6 @@ inline int check_tree(const TreeArgs& a, const char* what) {
   LLG_REQUIRE(a.scale > 0.f, "%s: the softmax scale must be positive", what);
   LLG_REQUIRE(a.part && a.max_len > 0 && a.n_pages > 0, "%s: needs scratch, a bound on the lengths and pages", what);
   LLG_REQUIRE((uintptr_t)a.k_pages % 16 == 0 && (uintptr_t)a.v_pages % 16 == 0 && (uintptr_t)a.q % 16 == 0, "%s: storage must be 16-byte aligned", what);
-  const long long tiles = (a.max_len + TK - 1) / TK, blocks = a.max_nodes * (a.nh / a.nkv) / 16 + 1;
-  LLG_REQUIRE(16 * tiles * blocks * a.nkv * a.n_seqs < 2147483647LL, "%s: %d sequences of %d positions are more work than one launch counts", what, a.n_seqs,
-              a.max_len);
   LLG_REQUIRE((long long)a.n_pages * a.nkv * TK < 2147483647LL, "%s: too many page rows for a tensor map coordinate", what);
   return 0;
 }

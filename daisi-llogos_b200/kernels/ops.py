@@ -565,13 +565,13 @@ def _load_lib(name: str):
             raise KernelError(f"the kernels take trees of {lib.llg_tree_max_nodes()} nodes, Python expects {TREE_MAX_NODES}")
     elif name == "attention_tree_mma":
         lib.llg_attn_tree_mma.argtypes = [POINTER(_TreeArgs), c_void_p]
-        lib.llg_attn_tree_mma_supported.argtypes = [c_int, c_int, c_int]
+        lib.llg_attn_tree_mma_supported.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_mma_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_mma_scratch_floats.restype = c_longlong
         lib.llg_attn_tree_mma_status.restype = c_int
     elif name == "attention_tree_tc":
         lib.llg_attn_tree_tc.argtypes = [POINTER(_TreeArgs), c_void_p]
-        lib.llg_attn_tree_tc_supported.argtypes = [c_int, c_int, c_int, c_int]
+        lib.llg_attn_tree_tc_supported.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_tc_scratch_floats.argtypes = [c_int, c_int, c_int, c_int, c_int, c_int]
         lib.llg_attn_tree_tc_scratch_floats.restype = c_longlong
         lib.llg_attn_tree_tc_status.restype = c_int
@@ -2468,12 +2468,12 @@ def attn_tree_plan(dtype: torch.dtype, n_seqs: int, max_nodes: int, n_heads: int
     rows = max_nodes * (n_heads // n_kv_heads)
     if USE_TC_TREE and dtype == torch.bfloat16 and rows > TREE_MMA_ROWS.get(head_dim, rows):
         lib = _lib("attention_tree_tc")
-        if lib.llg_attn_tree_tc_supported(head_dim, vd, n_seqs, n_heads // n_kv_heads):
+        if lib.llg_attn_tree_tc_supported(head_dim, vd, n_seqs, n_heads // n_kv_heads, max_nodes, n_kv_heads, max_len):
             return TreePlan("tc", key, 1, max_nodes, max_len,
                             lib.llg_attn_tree_tc_scratch_floats(n_seqs, max_nodes, n_kv_heads, n_heads // n_kv_heads, head_dim, max_len), 0)
     if USE_MMA_TREE and dtype == torch.bfloat16:
         lib = _lib("attention_tree_mma")
-        if lib.llg_attn_tree_mma_supported(head_dim, vd, n_seqs):
+        if lib.llg_attn_tree_mma_supported(head_dim, vd, n_seqs, rows, n_kv_heads, max_len):
             return TreePlan("mma", key, 1, max_nodes, max_len, lib.llg_attn_tree_mma_scratch_floats(n_seqs, rows, n_kv_heads, head_dim, vd, max_len),
                             0)
     lib = _lib("attention_tree")

@@ -33,3 +33,49 @@ def test_layers_of_two_value_sizes_are_weighed(llogos, ops, dtype, tol, sizes):
         assert float((a - b).abs().max()) <= tol * float(a.abs().max())
     weighed.evict([(0, 40)], first=2, recent=8)
     assert torch.isfinite(weighed.step([(0, [5]), (1, [6])])).all()
+
+
+def shared_pages(n_seqs, nkv, hd, before, width):
+    """A few pages that all sequences read, and a table as wide as the longest sequence that a plan allows for."""
+    g = torch.Generator().manual_seed(hd + n_seqs)
+    k, v = (torch.randn(5, nkv, 64, hd, generator=g).to(BF16) for _ in range(2))
+    table = torch.zeros(n_seqs, width, dtype=torch.int32)
+    table[:, :2] = torch.tensor([[i % 5, (i * 3 + 1) % 5] for i in range(n_seqs)], dtype=torch.int32)
+    return k, v, table, [before[i % len(before)] for i in range(n_seqs)]
+
+
+@pytest.mark.parametrize("kind,n_seqs,nkv,group,hd,max_len", [("tc", 256, 8, 8, 128, 131072), ("mma", 1024, 32, 2, 64, 1 << 20), ("simt", 1024, 32, 8, 64, 1 << 20)])
+def test_plans_for_long_sequences_of_many_fall_through_to_a_kernel_that_takes_them(ops, kind, n_seqs, nkv, group, hd, max_len):
+    """Sequences that may be long and are not, as an engine's bound for one long chat in a batch makes them: the plan is for what may be."""
+    import tree_plain as T
+    nh = nkv * group
+    k, v, table, before = shared_pages(n_seqs, nkv, hd, [5, 100, 64, 0], max_len // 64)
+    q = torch.randn(n_seqs, nh, hd, generator=torch.Generator().manual_seed(3)).to(BF16)
+    plan = ops.attn_tree_plan(BF16, n_seqs, 64, nh, nkv, hd, max_len)
+    assert plan.kind == kind
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda:0")
+    out = torch.full((n_seqs, nh * hd), 7.0, dtype=BF16, device="cuda:0")
+    ops.attn_tree(q.cuda(), k.cuda(), v.cuda(), table.cuda(), max_len // 64, ints(list(range(n_seqs))), ints(list(range(n_seqs + 1))), ints(before),
+                  torch.ones(n_seqs, dtype=torch.int64, device="cuda:0"), out, torch.empty(max(1, plan.scratch_floats), device="cuda:0"), scale=hd ** -0.5,
+                  plan=plan, counters=torch.zeros(max(1, plan.n_counters), dtype=torch.int32, device="cuda:0"))
+    got = out.cpu().double().view(n_seqs, nh, hd)
+    assert torch.isfinite(got).all() and not (got == 7.0).all(-1).any()
+    for i in (0, 1, 2, 3, 129, n_seqs // 2 + 1, n_seqs - 2, n_seqs - 1):
+        pages = table[i, :2].long()
+        rows = [x[pages].transpose(0, 1).reshape(nkv, 128, hd).transpose(0, 1)[:before[i] + 1] for x in (k, v)]
+        want, slack = T.attend(q[i:i + 1], *rows, [list(range(before[i] + 1))], hd ** -0.5, BF16)
+        assert ((got[i] - want[0]).abs() <= slack[0] + 1e-7).all()
+    assert ops.attn_tree_status() == 0
+
+
+@pytest.mark.parametrize("n_seqs", [130, 200, 500, 1024])
+@pytest.mark.parametrize("rows", [{}, {64: 0}], ids=["mma", "tc"])
+def test_batches_of_many_sequences(ops, n_seqs, rows, monkeypatch):
+    """More sequences than a block stages or has threads: each works out the list's sums over several of them."""
+    import test_gpu_trees as G
+    monkeypatch.setattr(ops, "TREE_MMA_ROWS", rows or {64: 1 << 30})
+    before = [(i * 37) % 150 for i in range(n_seqs)]
+    nodes = [(i * 5) % 4 for i in range(n_seqs)]
+    G.Case(BF16, 4, 2, 64, before, nodes, seed=n_seqs).check(ops)

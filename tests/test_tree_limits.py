@@ -1,0 +1,42 @@
+"""What plans of drafted trees and weighed keys go by at the ends of their ranges: rules on the host, asked without a GPU."""
+import importlib
+import random
+
+import pytest
+
+ops = importlib.import_module("daisi-llogos_b200.kernels.ops")
+LIMIT = 2 ** 31
+
+
+def up(x, y):
+    return -(-x // y)
+
+
+def tc_list(n_seqs, group, nodes, nkv, max_len):
+    """The weight of the tcgen05 kernel's list if every sequence is as long as it may be: 5 a tile of a row block and 8 a row block at most."""
+    tile = 128 // group
+    return n_seqs * nkv * up(nodes, tile if nodes <= tile else 2 * tile) * (5 * up(max_len, 64) + 8)
+
+
+def mma_list(n_seqs, rows, nkv, max_len):
+    return n_seqs * nkv * up(rows, 16 if rows <= 16 else 32 if rows <= 32 else 64) * up(max_len, 64)
+
+
+def test_kernels_take_the_trees_whose_lists_fit_their_counts():
+    """Each by its own list's length: 256 sequences of up to 131,072 positions, 64 nodes, 8 key/value heads of 8 query heads are 43 million units, no
+    reason to refuse them; where the list is too long the next kernel's turn comes."""
+    tc = ops._lib("attention_tree_tc").llg_attn_tree_tc_supported
+    mma = ops._lib("attention_tree_mma").llg_attn_tree_mma_supported
+    assert tc(128, 128, 256, 8, 64, 8, 131072) and mma(128, 128, 256, 512, 8, 131072)
+    rng, seen = random.Random(1), {(a, b): 0 for a in (0, 1) for b in (0, 1)}
+    for _ in range(20000):
+        n_seqs, group, nodes, nkv, max_len = (int(2 ** rng.uniform(low, high)) for low, high in ((0, 10), (0, 7), (0, 6), (0, 7), (0, 30)))
+        a, b = tc(64, 64, n_seqs, group, nodes, nkv, max_len), mma(64, 64, n_seqs, nodes * group, nkv, max_len)
+        for taken, units in ((a, tc_list(n_seqs, group, nodes, nkv, max_len)), (b, mma_list(n_seqs, nodes * group, nkv, max_len))):
+            assert not taken or units + 2 ** 20 < LIMIT
+            assert taken or units * 1.01 + 2 ** 21 > LIMIT      # (the room that is left: a million, rounded down to a head's)
+        seen[a, b] += 1
+    assert min(seen[1, 1], seen[0, 0]) > 100
+    assert not tc(64, 64, 1025, 4, 8, 8, 100) and not mma(64, 64, 1025, 32, 8, 100)
+    assert not tc(64, 64, 1024, 2, 64, 32, 1 << 20) and mma(64, 64, 1024, 128, 32, 1 << 20)
+    assert not tc(64, 64, 1024, 8, 64, 32, 1 << 20) and not mma(64, 64, 1024, 512, 32, 1 << 20)
