@@ -10,7 +10,7 @@ namespace {
 
 // ---- the confirmed path of drafted trees ---------------------------------------------------------------
 //
-// best_i = argmax of node i's logits (the lowest index of equal ones; NaN is never chosen); the path starts at node 0 and goes on to the lowest
+// best_i = argmax of node i's logits (the lowest index of equal ones; NaN is never chosen, 0 where there is nothing else); the path starts at node 0 and goes on to the lowest
 // child of the last node whose token is best of the last node; the next token is best of the path's last node.
 //
 // Reading the logits once is all the time there is: slices of a row over blocks, whose results meet in one 64-bit maximum per row (the
@@ -120,7 +120,18 @@ tree_accept_kernel(const float* __restrict__ logits, int vocab, int slice, const
       if (v > best) { best = v; at = i; }
     }
   }
-  unsigned long long key = warp_max_u64(key_of(best, at));
+  // A thread that saw nothing above minus infinity looks for that very number: the first of them in the slice, if all threads do (0: NaN alone).
+  unsigned long long key = 0;
+  if (best > -INFINITY) {
+    key = key_of(best, at);
+  } else {
+    for (int i = v0 + tid; i < v1; i += ACC_THREADS)
+      if (x[i] == -INFINITY) {
+        key = key_of(-INFINITY, i);
+        break;
+      }
+  }
+  key = warp_max_u64(key);
   if (lane == 0) warp_best[warp] = key;
   __syncthreads();
   if (warp != 0) return;
@@ -144,7 +155,8 @@ tree_accept_kernel(const float* __restrict__ logits, int vocab, int slice, const
     parent[e] = there ? parents[tok0 + i] : -1;
     top[e] = -1;
     if (there) {
-      top[e] = (int)(0xffffffffu - (unsigned)__ldcg(scratch + tok0 + i));
+      const unsigned long long most = __ldcg(scratch + tok0 + i);
+      top[e] = most ? (int)(0xffffffffu - (unsigned)most) : 0;
       scratch[tok0 + i] = 0;
     }
   }

@@ -2564,7 +2564,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
     Tree b's nodes are ``cu_tokens[b] .. cu_tokens[b + 1]`` (at most 64) with their ``tokens`` and ``parents`` (int32 ``[N]``; a parent is a place
     within the tree and lies before its node; node 0 is the token that is certain already, parent -1).  What follows a node is
     ``picked[node]`` (int32, a sampler's draws), or the largest of ``logits[node]`` (float32 ``[N, vocab]``; of equal ones the lowest id, NaN
-    never).  The path starts at node 0 and goes on to the first child whose token is what follows.  ``path`` (int32 ``[B, 64]``) gets its
+    never; of a row of NaN alone 0).  The path starts at node 0 and goes on to the first child whose token is what follows.  ``path`` (int32 ``[B, 64]``) gets its
     nodes, filled up with -1, ``n_path`` their number, and ``next_token`` what follows the last (of a tree without nodes: 0 and -1).
 
     ``scratch`` (with ``logits``): int64, ``tree_accept_scratch`` numbers, zero when first used, left zero; one call at a time."""
