@@ -9,7 +9,7 @@
 // A weight needs its row's whole sum, so there are two passes over a (sequence, head)'s keys, cut into splits: the first leaves every split's
 // maximum and sum per row; the blocks of the second join those for their rows and divide.  Few rows (a decode step: the heads of a group) leave
 // their scores on the way, 4 bytes a row beside a key's 2 hd bytes, and the second pass reads those; on the matrix instructions with more rows than
-// STORE_ROWS, and here where the scores would be more than a workspace should be, the second pass works them out again from the keys.
+// STORE_ROWS, and everywhere where the scores would be more than a workspace should be, the second pass works them out again from the keys.
 // Sums run in a fixed order everywhere.
 //
 // What bounds it: reads of shared memory for the products, and for small calls the two passes' latency.  float32, us with scores kept / worked out

@@ -265,15 +265,17 @@ int launch(const KeyWeightArgs& a, const CUtensorMap& mk, cudaStream_t stream) {
     return llg_check_launch("key_weights_mma");
   };
   if (go(key_weights_mma_kernel<HDP, MT, WR, STAGES, false>, first_allowed)) return 1;
-  if constexpr (16 * MT * WR <= STORE_ROWS) return add_stored(a, stream);
-  else return go(key_weights_mma_kernel<HDP, MT, WR, STAGES, true>, second_allowed);
+  if (a.scores) return add_stored(a, stream);
+  if constexpr (WR > 1) return go(key_weights_mma_kernel<HDP, MT, WR, STAGES, true>, second_allowed);
+  else return llg_fail("key_weights_mma: a warp's %d keys are fewer than the second pass adds up by halves", TK / WARPS);
 }
 
 // Rows of a group's queries: up to 16 and 32 one tile a warp, all warps along the keys or two of them; more: two tiles a warp, four along the rows.
+// Without scores on the way up to 16 rows are taken as 17 to 32 are: in the second pass a warp has to have 32 keys.
 template <int HDP, int STAGES>
 int run(const KeyWeightArgs& a, const CUtensorMap& mk, cudaStream_t stream) {
   const int rows = a.nh / a.nkv * a.last;
-  if (rows <= 16) return launch<HDP, 1, 1, STAGES>(a, mk, stream);
+  if (rows <= 16 && a.scores) return launch<HDP, 1, 1, STAGES>(a, mk, stream);
   if (rows <= 32) return launch<HDP, 1, 2, STAGES>(a, mk, stream);
   return launch<HDP, 2, 4, STAGES>(a, mk, stream);
 }
@@ -286,8 +288,7 @@ LLG_API int llg_key_weights_mma_supported(int hd) { return hd >= 8 && hd <= 128 
 LLG_API int llg_key_weights_mma(const KeyWeightArgs* args, int n_pages, cudaStream_t stream) {
   const KeyWeightArgs& a = *args;
   if (check(a)) return 1;
-  LLG_REQUIRE((a.nh / a.nkv * a.last <= STORE_ROWS) == (a.scores != nullptr), "key_weights_mma: %d rows of scores are %sstored", a.nh / a.nkv * a.last,
-              a.scores ? "not " : "");
+  LLG_REQUIRE(!a.scores || (long long)a.nh / a.nkv * a.last <= STORE_ROWS, "key_weights_mma: %d rows of scores are not stored", a.nh / a.nkv * a.last);
   LLG_REQUIRE(llg_key_weights_mma_supported(a.hd), "key_weights_mma: heads of %d elements (steps of 8 up to 128)", a.hd);
   LLG_REQUIRE((uintptr_t)a.k_pages % 16 == 0 && (uintptr_t)a.q % 16 == 0, "key_weights_mma: storage must be 16-byte aligned");
   LLG_REQUIRE((long long)n_pages * a.nkv * TK < 2147483647LL, "key_weights_mma: too many page rows for a tensor map coordinate");

@@ -2593,15 +2593,20 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Te
 
 
 USE_MMA_WEIGHTS = True       # tests switch it off to reach the CUDA-core kernel with bfloat16
-KEY_SCORE_FLOATS = 1 << 24   # the most scores that key weights on the CUDA cores keep between their passes: 64 MB
+KEY_SCORE_FLOATS = 1 << 24   # the most scores that key weights keep between their passes: 64 MB
+# Where a batch's are more, up to so many rows on mma.sync are taken a few sequences at a time and keep theirs, more have them worked out twice.  us, heads
+# of 128, in goes / twice: 4 rows 64 x 16,384 keys 420 / 780, 32 x 32,768 441 / 793, 128 x 8,190 420 / 696; 16 rows 16 x 16,384 194 / 222; 32 rows
+# 8 x 32,768 362 / 220.  (With all kept, whatever they take: 428, 426, 414, 158, 227.  One of 32,768 among 63 of 300, 4 rows: 107 / 567, all kept 225.)
+KEY_GOES_ROWS = 16
 USE_TC_WEIGHTS = True        # and this, to reach the mma.sync kernel with more rows than have their scores stored
 
 
 class KeyWeightPlan:
     """How ``key_weights`` will run for one batch shape.  Made by ``key_weights_plan``; callers read ``scratch_floats`` and ``n_counters``."""
 
-    def __init__(self, kind: str, key, last: int, max_len: int, splits: int, split_keys: int, stats: int, scores: int):
+    def __init__(self, kind: str, key, last: int, max_len: int, splits: int, split_keys: int, stats: int, scores: int, together: int = 0):
         self.kind, self.key, self.last, self.max_len, self.splits, self.split_keys = kind, key, last, max_len, splits, split_keys
+        self.together = together or key[1]               # sequences of one go; the next go's follow on the same scratch
         self.stats, self.scores, self.n_counters = stats, scores, 0
         self.scratch_floats = stats + scores
 
@@ -2619,21 +2624,34 @@ def key_weights_plan(dtype: torch.dtype, n_seqs: int, last: int, n_heads: int, n
     mma = USE_MMA_WEIGHTS and dtype == torch.bfloat16 and _lib("key_weights_mma").llg_key_weights_mma_supported(head_dim)
     tile, rows = lib.llg_key_weights_tile(), n_heads // n_kv_heads * last
     tiles = -(-max_len // tile)
-    kind = "mma" if mma else "simt"
+    kind, together = "mma" if mma else "simt", n_seqs
+
+    def cut(n, blocks, least, step):
+        """Splits of n sequences that give every multiprocessor ``blocks`` blocks, of at least ``least`` steps of tiles: (splits, tiles of one)."""
+        per = step * max(least, -(-tiles * n * n_kv_heads // (step * blocks * sm_count())))
+        return -(-tiles // per), per
+
     if mma and USE_TC_WEIGHTS and _lib("key_weights_tc").llg_key_weights_tc_supported(head_dim, n_heads // n_kv_heads, last):
-        kind = "tc"
-        # pairs of tiles, at least two a split
-        per = 2 * max(2, -(-tiles * n_seqs * n_kv_heads // (2 * 3 * sm_count())))
+        kind, scores = "tc", 0
+        splits, per = cut(n_seqs, 3, 2, 2)               # pairs of tiles, at least two a split
     else:
-        # splits of at least four tiles (two on the CUDA cores, whose tiles take several times as long), as many as give every multiprocessor six blocks
-        per = max(4 if mma else 2, -(-tiles * n_seqs * n_kv_heads // (6 * sm_count())))
-    splits = -(-tiles // per)
-    total = n_seqs * n_kv_heads * rows
-    scores = total * splits * per * tile
-    if rows > lib.llg_key_weights_store_rows() if mma else scores > KEY_SCORE_FLOATS:
-        scores = 0                                       # they are worked out twice
+        # at least four tiles a split (two on the CUDA cores, whose tiles take several times as long), and six blocks a multiprocessor
+        least, most = 4 if mma else 2, 0 if mma and rows > lib.llg_key_weights_store_rows() else KEY_SCORE_FLOATS
+        one = n_kv_heads * rows * tile                   # scores of a tile of one sequence
+        splits, per = cut(n_seqs, 6, least, 1)
+        if mma and rows <= KEY_GOES_ROWS and 0 < one * tiles <= most < one * n_seqs * splits * per:
+            for goes in range(max(2, -(-one * n_seqs * tiles // most)), n_seqs + 1):
+                together = -(-n_seqs // goes)
+                splits, per = cut(together, 6, least, 1)
+                per = -(-tiles // splits)                # (no room behind the last tile that scores would be kept for)
+                if one * together * splits * per <= most:
+                    break
+        scores = one * together * splits * per
+        if scores > most:                                # none are kept: they are worked out twice
+            scores, together = 0, n_seqs
+            splits, per = cut(n_seqs, 6, least, 1)
     return KeyWeightPlan(kind, (dtype, n_seqs, n_heads, n_kv_heads, head_dim), last, max_len, splits, per * tile,
-                         -(-2 * total * splits // 4) * 4, scores)
+                         -(-2 * together * n_kv_heads * rows * splits // 4) * 4, scores, together)
 
 
 def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor, slots: torch.Tensor, cu_tokens: torch.Tensor,
@@ -2674,18 +2692,22 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     a.table_width, a.weight_width = width, positions
     a.stats = base
     a.scores = base + 4 * plan.stats if plan.scores else None
-    a.n_seqs, a.n_tokens, a.nh, a.nkv, a.hd, a.last = b, n, nh, nkv, hd, last
+    a.n_tokens, a.nh, a.nkv, a.hd, a.last = n, nh, nkv, hd, last
     a.splits, a.split_keys = plan.splits, plan.split_keys
     a.scale = scale
-    if plan.kind == "tc":
-        lib = _lib("key_weights_tc")
-        _check(lib, lib.llg_key_weights_tc(byref(a), n_pages, _stream()), kernels=2)
-    elif plan.kind == "mma":
-        lib = _lib("key_weights_mma")
-        _check(lib, lib.llg_key_weights_mma(byref(a), n_pages, _stream()), kernels=2)
-    else:
-        lib = _lib("key_weights")
-        _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), _stream()), kernels=2)
+    stream = _stream()
+    for first in range(0, b, plan.together):             # (one go but where the scores are many)
+        a.n_seqs = min(plan.together, b - first)
+        a.slots, a.cu_tokens, a.len_before = p[3] + 4 * first, p[4] + 4 * first, p[5] + 4 * first
+        if plan.kind == "tc":
+            lib = _lib("key_weights_tc")
+            _check(lib, lib.llg_key_weights_tc(byref(a), n_pages, stream), kernels=2)
+        elif plan.kind == "mma":
+            lib = _lib("key_weights_mma")
+            _check(lib, lib.llg_key_weights_mma(byref(a), n_pages, stream), kernels=2)
+        else:
+            lib = _lib("key_weights")
+            _check(lib, lib.llg_key_weights_simt(byref(a), _dt(q), stream), kernels=2)
 
 
 def key_weights_status() -> int:

@@ -79,3 +79,55 @@ def test_batches_of_many_sequences(ops, n_seqs, rows, monkeypatch):
     before = [(i * 37) % 150 for i in range(n_seqs)]
     nodes = [(i * 5) % 4 for i in range(n_seqs)]
     G.Case(BF16, 4, 2, 64, before, nodes, seed=n_seqs).check(ops)
+
+
+FEW = [(8, 2, 64, 4), (8, 2, 128, 1), (8, 1, 128, 2), (5, 1, 80, 3), (12, 4, 24, 5)]
+MORE = [(8, 2, 64, 8), (8, 2, 128, 5), (5, 1, 80, 6), (12, 4, 24, 10), (4, 4, 64, 17)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,last,kept", [(*h, kept) for kept in (0, 3, 1) for h in FEW] + [(*h, kept) for kept in (0, 1) for h in MORE], ids=str)
+def test_weights_of_few_rows_with_a_bound_on_the_scores(ops, nh, nkv, hd, last, kept, monkeypatch):
+    """Up to 32 rows on mma.sync where the batch's scores are more than may be kept: worked out twice, or a few sequences at a time."""
+    import test_gpu_trees as G
+    before, brings = [300, 0, 127, 64, 1, 500, 9], [1, 230, 41, 1, 0, 3, 20]
+    max_len = max(x + y for x, y in zip(before, brings))
+    rows = nh // nkv * last
+    monkeypatch.setattr(ops, "KEY_SCORE_FLOATS", kept * nkv * rows * (-(-max_len // 256) * 256))
+    plan = ops.key_weights_plan(BF16, len(before), last, nh, nkv, hd, max_len)
+    assert plan.kind == "mma" and (bool(plan.scores), plan.together) == ((True, {3: 3, 1: 1}[kept]) if kept and rows <= ops.KEY_GOES_ROWS else (False, 7))
+    G.test_weights_of_keys(ops, BF16, nh, nkv, hd, before, brings, last)
+    assert ops.key_weights_status() == 0
+
+
+@pytest.mark.parametrize("kept", [0, 2], ids=["twice", "some"])
+def test_weights_with_a_bound_on_the_scores_in_a_graph(ops, kept, monkeypatch):
+    """Recorded and replayed over other keys: the goes of a call follow one another on its scratch."""
+    nh, nkv, hd, last, b = 8, 2, 64, 4, 5
+    monkeypatch.setattr(ops, "KEY_SCORE_FLOATS", kept * nkv * 16 * 1024)
+    plan = ops.key_weights_plan(BF16, b, last, nh, nkv, hd, 1000)
+    assert bool(plan.scores) == (kept > 0)
+    g = torch.Generator("cuda:0").manual_seed(1)
+    kp = torch.randn(b * 16, nkv, 64, hd, device="cuda:0", generator=g).to(BF16)
+    q = torch.randn(b * last, nh, hd, device="cuda:0", generator=g).to(BF16)
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda:0")
+    args = [q, kp, torch.arange(b * 16, dtype=torch.int32, device="cuda:0").view(b, 16), ints([4, 2, 0, 1, 3]), ints([last * i for i in range(b + 1)]),
+            ints([900, 20, 0, 64, 700])]
+    scratch, counters = torch.empty(plan.scratch_floats, device="cuda:0"), torch.zeros(1, dtype=torch.int32, device="cuda:0")
+    weights = [torch.zeros(b, nkv, 1000, device="cuda:0") for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    kw = dict(scale=hd ** -0.5, last=last, plan=plan, counters=counters)
+    ops.key_weights(*args, weights[0], scratch, **kw)
+    with torch.cuda.graph(graph):
+        ops.key_weights(*args, weights[1], scratch, **kw)
+    graph.replay()
+    assert torch.equal(*weights)
+    kp.copy_(torch.randn(kp.shape, device="cuda:0", generator=g))
+    for w in weights:
+        w.zero_()
+    graph.replay()
+    ops.key_weights(*args, weights[0], scratch, **kw)
+    assert torch.equal(*weights)
+    rows = nh // nkv * last
+    assert ((weights[0].double().sum(-1) - rows).abs() <= rows * 2 * (67 * 32 + 1000) * 2.0 ** -23).all()      # (as in the test of long sequences)

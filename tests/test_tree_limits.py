@@ -40,3 +40,26 @@ def test_kernels_take_the_trees_whose_lists_fit_their_counts():
     assert not tc(64, 64, 1025, 4, 8, 8, 100) and not mma(64, 64, 1025, 32, 8, 100)
     assert not tc(64, 64, 1024, 2, 64, 32, 1 << 20) and mma(64, 64, 1024, 128, 32, 1 << 20)
     assert not tc(64, 64, 1024, 8, 64, 32, 1 << 20) and not mma(64, 64, 1024, 512, 32, 1 << 20)
+
+
+def test_no_plan_keeps_more_scores_than_a_workspace_should(monkeypatch):
+    """What keys are weighed in is bounded whatever the batch and its longest sequence are, on every kernel: 64 MB of scores."""
+    import torch
+    monkeypatch.setattr(ops, "sm_count", lambda: 148)
+    rng = random.Random(2)
+    kinds = set()
+    for i in range(3000):
+        n_seqs, nkv, group, last, max_len = (int(2 ** rng.uniform(low, high)) for low, high in ((0, 8.1), (0, 5.1), (0, 3.1), (0, 5.1), (0, 17.1)))
+        if i == 0:
+            n_seqs, nkv, group, last, max_len = 32, 8, 4, 8, 131072
+        dtype, hd = rng.choice(((torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 80), (torch.bfloat16, 20), (torch.float32, 64)))
+        plan = ops.key_weights_plan(dtype, n_seqs, last, nkv * group, nkv, hd, max_len)
+        assert plan.scores <= 1 << 24, (plan.kind, plan.scores)
+        assert plan.scratch_floats >= plan.scores + 2 * plan.together * nkv * group * last * plan.splits and plan.splits * plan.split_keys >= max_len
+        assert plan.together == n_seqs or group * last <= ops.KEY_GOES_ROWS
+        if plan.scores:
+            assert plan.scores == plan.together * nkv * group * last * plan.splits * plan.split_keys and plan.together <= n_seqs
+        else:
+            assert plan.together == n_seqs
+        kinds.add((plan.kind, bool(plan.scores), plan.together < n_seqs))
+    assert kinds == {("mma", True, False), ("mma", True, True), ("mma", False, False), ("simt", True, False), ("simt", False, False), ("tc", False, False)}
