@@ -74,16 +74,14 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   const int* table = a.page_table + (long long)slot * a.table_width;
   auto page_of = [&](int t) { return t < t_to ? table[t / 2 % a.ring_pages] : 0; };
   int page = none ? 0 : page_of(t_from);
-  if (!none) {
-    for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
-    for (int r = tid; r < ROWS; r += THREADS) {
-      const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
-      bits[r] = mine;
-      depth[r] = __popcll(mine) - 1;
-    }
-  }
-  pdl_wait();                             // all before it reads sizes, slots, tables and words alone, which no kernel of a step writes
+  pdl_wait();                             // all before it reads sizes, slots and tables alone, which no kernel of a step writes
   if (none) return;
+  for (int i = tid; i < n; i += THREADS) node_depth[i] = __popcll(a.ancestors[tok0 + i]) - 1;
+  for (int r = tid; r < ROWS; r += THREADS) {
+    const long long mine = r < n_rows ? a.ancestors[tok0 + (row0 + r) / G] : 0;
+    bits[r] = mine;
+    depth[r] = __popcll(mine) - 1;
+  }
   copy_rows<THREADS, T>(Qs, ks, ROWS, a.hd, kp, [&](int r) {
     return r < n_rows ? qg + ((long long)(tok0 + (row0 + r) / G) * a.nh + kvh * G + (row0 + r) % G) * a.hd : nullptr;
   });

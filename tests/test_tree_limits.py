@@ -63,3 +63,16 @@ def test_no_plan_keeps_more_scores_than_a_workspace_should(monkeypatch):
             assert plan.together == n_seqs
         kinds.add((plan.kind, bool(plan.scores), plan.together < n_seqs))
     assert kinds == {("mma", True, False), ("mma", True, True), ("mma", False, False), ("simt", True, False), ("simt", False, False), ("tc", False, False)}
+
+
+@pytest.mark.parametrize("source", ["attention_tree.cu", "attention_tree_mma.cu", "attention_tree_tc.cu"])
+def test_only_sizes_slots_and_pages_are_read_before_the_wait(source):
+    """Ahead of its wait for the kernel before it an attention of trees reads what its entry point says: not the words of what nodes see, which a
+    caller's own kernel may just be writing."""
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(ops.__file__), "..", "csrc", source)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    ahead = text[text.index("__global__"):text.index("  pdl_wait();")]
+    assert set(re.findall(r"\ba\.(cu_tokens|len_before|slots|page_table|ancestors|q|k_pages|v_pages|out|part|counters)\s*\[", ahead)) <= {
+        "cu_tokens", "len_before", "slots", "page_table"}
