@@ -164,3 +164,42 @@ def test_what_tree_steps_are_recorded_in_is_bounded_in_bytes(llogos, model_dirs,
     for _ in range(2):
         assert [key[0] for key in twice(eng, slot, 8)] == [(4,)]       # too large by itself, and nobody makes room for it
     assert eng.accept_tree(torch.zeros(8, dtype=torch.int32)) == [([0], 0)]
+
+
+MIXERS = {"value_blend": dict(changes=[dict(value_blend="g")] * 2), "value_dim": dict(changes=[dict(value_dim=32), dict(value_dim=24)]),
+          "out_gate": dict(changes=[dict(out_gate=True)] * 2), "out_bias": dict(changes=[dict(out_bias=True), {}]),
+          "window": dict(changes=[dict(window=20), {}]), "borrowed": dict(changes=[{}, dict(own_kv=False)], cache_of=((1, 0),)),
+          "borrowed_window": dict(changes=[dict(window=20), dict(window=20, own_kv=False)], cache_of=((1, 0),))}
+
+
+@pytest.mark.parametrize("name", list(MIXERS))
+def test_a_chain_of_drafted_tokens_has_the_logits_of_a_prompts_step(llogos, name):
+    """For every form of the attention that takes tree steps, twice as long as a page: a chain is what a step brings, and what is accepted of it is what
+    the next step looks at."""
+    model = M.with_mixers(M.CFG, **MIXERS[name], dtype=torch.float32, device="cpu", ops=tree_ops)
+    eng = engine_for(llogos, model)
+    toks = [(7 * i + i * i) % 256 for i in range(200)]
+    trees, steps = eng.open(), eng.open()
+    for slot in (trees, steps):
+        eng.step([(slot, toks[:60])], [[]])
+    at = 60
+    for n in (9, 64, 30):
+        part = toks[at:at + n]
+        want = eng.step([(steps, part)], [list(range(n))]).clone()
+        got = eng.step_tree([(trees, part, list(range(-1, n - 1)))]).clone()
+        assert float((got - want).abs().max()) <= 2e-4 * float(want.abs().max())
+        assert eng.accept_tree(torch.tensor(part[1:] + [5], dtype=torch.int32)) == [(list(range(n)), 5)]
+        at += n
+    want, got = (eng.step([(slot, [11])]).clone() for slot in (steps, trees))
+    assert float((got - want).abs().max()) <= 2e-4 * float(want.abs().max())
+
+
+@pytest.mark.parametrize("name", ["value_blend", "value_dim", "out_gate", "out_bias"])
+def test_weighed_keys_leave_every_forms_logits(llogos, name):
+    """An engine that weighs its keys, before an eviction, and one that does not."""
+    model = M.with_mixers(M.CFG, **MIXERS[name], dtype=torch.float32, device="cpu", ops=tree_ops)
+    engines = [engine_for(llogos, model), engine_for(llogos, model, weigh_keys=3)]
+    slots = [e.open() for e in engines]
+    for part in ([3] * 70, [5], [9, 8, 7], [2]):
+        want, got = (e.step([(s, part)]).clone() for e, s in zip(engines, slots))
+        assert float((got - want).abs().max()) <= 2e-4 * float(want.abs().max())
