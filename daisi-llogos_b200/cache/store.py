@@ -44,8 +44,8 @@ class KvView:
     unit: int
     owner: bool = True               # False: this entry reads the unit, another entry writes it
     keep_step_kv: bool = False       # the unit is read by later entries: keep this step's packed k/v
-    weights: Optional[torch.Tensor] = None       # [n_slots + 1, n_kv, positions] float32: what queries gave each key (``SequenceCache.weigh_keys``)
     shared: Dict = field(default_factory=dict)   # owner leaves {"k_new", "v_new"} here for readers
+    weights: Optional[torch.Tensor] = None       # [n_slots + 1, n_kv, positions] float32: what queries gave each key (``SequenceCache.weigh_keys``)
 
 
 @dataclass
@@ -362,7 +362,7 @@ class SequenceCache:
         g = self._group_of_unit.get(unit)
         if g is not None:
             return KvView(g.k[unit], g.v[unit], g.page_table, g.ring_pages, g.window, unit, owner,
-                          keep_step_kv, None if g.weights is None else g.weights[g.units.index(unit)], shared if shared is not None else {})
+                          keep_step_kv, shared if shared is not None else {}, None if g.weights is None else g.weights[g.units.index(unit)])
         if unit in self.state:
             return StateView(self.state[unit], unit, owner)
         return None

@@ -203,3 +203,10 @@ def test_weighed_keys_leave_every_forms_logits(llogos, name):
     for part in ([3] * 70, [5], [9, 8, 7], [2]):
         want, got = (e.step([(s, part)]).clone() for e, s in zip(engines, slots))
         assert float((got - want).abs().max()) <= 2e-4 * float(want.abs().max())
+
+
+def test_a_view_of_keys_is_made_with_the_arguments_it_had(llogos):
+    """What a mixer's own tests make by position: what is shared between the entries of a step is the ninth."""
+    shared = {}
+    view = llogos.cache.store.KvView(None, None, None, 1, 0, 3, True, False, shared)
+    assert view.shared is shared and view.weights is None
