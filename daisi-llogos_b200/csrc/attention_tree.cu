@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
       s[r][0] = s2[r][0].x + s2[r][0].y;
       s[r][1] = s2[r][1].x + s2[r][1].y;
     }
-    // positions that some row may not see: the tree's, those behind it, the window's edge
-    const bool mixed = p0 + TK > lb || (a.window > 0 && p0 <= lb + n - a.window);
+    // positions that some row may not see: the tree's, those behind it, the window's edge (a word has up to 64 bits, whatever the tree's nodes)
+    const bool mixed = p0 + TK > lb || (a.window > 0 && p0 < lb + LLG_TREE_NODES - a.window);
     if (mixed) {
 #pragma unroll
       for (int r = 0; r < RY; ++r)

@@ -222,7 +222,7 @@ attn_tree_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           mma_16816(s[2 * jp], qf[ks], kb[0], kb[1]);
           mma_16816(s[2 * jp + 1], qf[ks], kb[2], kb[3]);
         }
-      const bool mixed = p0 + KEYS > sh.lb || (a.window > 0 && p0 <= sh.lb + sh.n - a.window);      // the same for the warp
+      const bool mixed = p0 + KEYS > sh.lb || (a.window > 0 && p0 < sh.lb + LLG_TREE_NODES - a.window);      // the same for the warp
       if (mixed) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)

@@ -450,7 +450,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             sv[48 + x] = __uint_as_float(r3_[x]);
           }
         }
-        const bool mixed = p0 + TK > sh.lb || (a.window > 0 && p0 <= sh.lb + sh.n - a.window);      // the same for the block
+        const bool mixed = p0 + TK > sh.lb || (a.window > 0 && p0 < sh.lb + LLG_TREE_NODES - a.window);      // the same for the block
         bool by_hand = false;
         if (mixed) {                          // uniform
           const int shift = sh.lb - p0;      // places of the tile that are cached keys

@@ -2494,8 +2494,8 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
 
     Sequence b holds ``len_before[b]`` keys; its tree's nodes are the packed tokens ``cu_tokens[b] .. cu_tokens[b + 1]`` (at most
     ``plan.max_nodes``), whose keys and values lie in the pages already, node i's at position ``len_before[b] + i``.  ``ancestors`` (int64
-    ``[N]``): bit j of a node's word says that it sees node j of its tree (its own bit included); a node sees every cached key
-    besides.  ``window`` W > 0: a node stands ``depth`` = (its bits) - 1 positions behind the cached keys and sees what stands less than W before
+    ``[N]``): bit j of a node's word says that it sees node j of its tree (its own bit included; bits behind the tree's nodes show nothing, and
+    count for its depth); a node sees every cached key besides.  ``window`` W > 0: a node stands ``depth`` = (its bits) - 1 positions behind the cached keys and sees what stands less than W before
     it.  ``q`` is ``[N, nh, hd]``, ``out`` ``[N, nh * vd]``; a node that sees nothing gets zeros, rows behind the last sequence are left as they
     were.  What a node does not see has no part in its result, whatever is stored there.
 

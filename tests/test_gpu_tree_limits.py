@@ -131,3 +131,13 @@ def test_weights_with_a_bound_on_the_scores_in_a_graph(ops, kept, monkeypatch):
     assert torch.equal(*weights)
     rows = nh // nkv * last
     assert ((weights[0].double().sum(-1) - rows).abs() <= rows * 2 * (67 * 32 + 1000) * 2.0 ** -23).all()      # (as in the test of long sequences)
+
+
+@pytest.mark.parametrize("dtype,nh,hd", [(F32, 4, 64), (BF16, 4, 64), (BF16, 4, 20), (BF16, 16, 64), (BF16, 32, 128)], ids=["f32", "mma", "simt", "tc64", "tc128"])
+@pytest.mark.parametrize("window", [40, 64, 100, 200])
+def test_a_nodes_depth_is_its_bits_however_few_nodes_there_are(ops, dtype, nh, hd, window):
+    """Words with more bits than the tree has nodes: they are no nodes' and show nothing, and they count for the depth that a window goes by."""
+    import test_gpu_trees as G
+    bits = [[1, 3 | ((1 << 50) - 1) << 5, 5, (1 << 64) - 1, 9, (1 << 40) - 1], [1, 3 | 1 << 60, (1 << 63) - 1, 2, 1 << 63]]
+    G.Case(dtype, nh, 2, hd, [330, 205], [6, 5], bits=bits, window=window, seed=window).check(ops)
+    G.Case(dtype, nh, 2, hd, [70, 0], [6, 5], bits=bits, window=window, seed=window + 1).check(ops)
