@@ -420,7 +420,7 @@ attn_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       const int i1 = min(n_units, i0 + sh.tiles - cur.t), step = plain ? 1 : 2;
       unsigned long long bits = next.bits;
       bits &= sh.n >= 64 ? ~0ull : (1ull << sh.n) - 1;
-      if (a.window > 0 && depth >= a.window)            // of its ancestors, those less than a window above it
+      if (a.window > 0 && depth + 1 >= a.window)        // of what it sees, what stands less than a window above it (a node of no bits: at -1)
         for (int j = 0; j < sh.n; ++j)
           if (((bits >> j) & 1) && depth - (__popcll(a.ancestors[sh.tok0 + j]) - 1) >= a.window) bits &= ~(1ull << j);
       float m_run = -INFINITY, l_run = 0.f;

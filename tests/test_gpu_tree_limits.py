@@ -141,3 +141,12 @@ def test_a_nodes_depth_is_its_bits_however_few_nodes_there_are(ops, dtype, nh, h
     bits = [[1, 3 | ((1 << 50) - 1) << 5, 5, (1 << 64) - 1, 9, (1 << 40) - 1], [1, 3 | 1 << 60, (1 << 63) - 1, 2, 1 << 63]]
     G.Case(dtype, nh, 2, hd, [330, 205], [6, 5], bits=bits, window=window, seed=window).check(ops)
     G.Case(dtype, nh, 2, hd, [70, 0], [6, 5], bits=bits, window=window, seed=window + 1).check(ops)
+
+
+@pytest.mark.parametrize("dtype,nh,hd", [(F32, 4, 64), (BF16, 4, 64), (BF16, 4, 20), (BF16, 16, 64), (BF16, 32, 128)], ids=["f32", "mma", "simt", "tc64", "tc128"])
+def test_a_window_ends_between_a_node_and_one_without_bits(ops, dtype, nh, hd):
+    """A node that sees nothing, itself included, stands one place before the tree's first: a node whose depth is the window less one is a window behind it."""
+    import test_gpu_trees as G
+    for window in (1, 2, 3, 5, 8):
+        bits = [[0, 0b10, 0b11, 0b111, 0b1111, 0b11111, 0b111111, 0b1111111, 0b11111111, 0b1], [1, 0, 0b111, 0b1111, 2]]
+        G.Case(dtype, nh, 2, hd, [200, 0], [10, 5], bits=bits, window=window, seed=window).check(ops)
