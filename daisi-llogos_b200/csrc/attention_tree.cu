@@ -305,6 +305,8 @@ __global__ void __launch_bounds__(THREADS) attn_tree_kernel(TreeArgs a) {
   }
 }
 
+// Blocks of 8 rows, or of 32 from 9 rows on.  float32, us with 8 / 32 rows a block, heads of 64: 8 rows behind 8 x 4,000 keys 65 / 98, 3 x 735..1,878 19 / 26,
+// 1 x 611 12 / 16; 12 rows 120 / 101, 21 / 29, 14 / 17; heads of 128: 8 rows 142 / 233, 27 / 53, 19 / 27; 12 rows 267 / 236, 51 / 56, 20 / 29.
 int rows_per_block(int rows) { return rows <= 8 ? 8 : 32; }
 
 template <typename T, int RY, int VD, int STAGES>

@@ -4,7 +4,8 @@
 // The kernel streams the cache: with R query rows (nodes x heads of a group) a key's and a value's 4 hd bytes take 4 R hd flops, so up to 16 rows
 // of heads of 128, 32 of heads of 64, the memory system decides the time and mma.sync keeps up beside it (eight sequences of 8,190 keys, heads of
 // 128, 16 rows: 59 us, 69 % of the copy bandwidth); more go to attention_tree_tc.cu, heads of other sizes stay.  One tree of 8 nodes behind
-// 611 keys, 32 heads of 64 in groups of four: 10 us, the latency of two kernels (11 with the plan behind the wait for the kernel before).
+// 611 keys, 32 heads of 64 in groups of four: 10 us, the latency of two kernels (11 with the plan behind the wait for the kernel before).  Both on the
+// device, twenty calls in a CUDA graph, inputs warm in L2; the short one called by itself takes 13, its host's time.
 //
 //   copies     A fifth warp brings every key and value tile (one cache page of one key/value head) with TMA boxes of 64 x 64 elements into a
 //              ring of stages handed over by mbarriers; head sizes that are no multiple of 64 are filled up with zeros by the boxes.
@@ -13,7 +14,7 @@
 //   products   A block's four warps share a tile of 64 keys and 16 WR query rows: WR warps along the rows, 4 / WR along the keys.  A warp's
 //              scores stay in registers and become the first operand of the second product.
 //   softmax    float32; the running maximum is a whole number of binary orders (as in attention_mma.cu), so rescaling is exact, and the rounding of
-//              weights to bfloat16 does not depend on how the list was cut.
+//              weights to bfloat16 (the second product's operands are) does not depend on how the list was cut.
 //   masks      Only tiles that hold nodes, the tree's end or the window's edge look at bits.  In those a value that is not finite must not meet
 //              a weight of zero: a warp that finds one among its keys adds that tile's products up itself, leaving out what a row does not see.
 //   joining    A run that ends inside a (sequence, head, row block) leaves partial rows, which a second kernel joins (tree_tiles.cuh).

@@ -7,17 +7,19 @@
 // softmax needs no exchange; a group's chain of scores, softmax and product takes about 2,000 cycles a tile, half of them exponentials (attention_tc.cu
 // says what of; with two threads a row, which meet once a tile, it took longer).  A tile of queries is as many whole nodes as 128 rows hold, so
 // that one TMA box of [nodes][heads of the group] brings it; a row block is one or two of them.  Two (PLAIN): each group takes one, and all key
-// tiles: 2,700 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one every 1,660 cycles, where the memory
+// tiles: 2,700 to 2,800 cycles a key tile.  One (SPLIT): both groups take it, and every second key tile each: one every 1,660 cycles, where the memory
 // system brings one every 1,400.  (Row blocks of 128 alone, all of them SPLIT: every 128 rows read the keys again, sixteen full trees behind up
 // to 8,000 keys 277 us.)  Eight trees of 13 to 32 nodes behind 8,190 keys, 32 heads of 128 in groups of four: 59 us, of which 7 lie before the first
 // scores; sixteen trees of 64 nodes behind 350 to 7,990 keys, 40 heads in groups of five: 192 us, bound by the groups' chains (61 and 198 with the
-// plan and the first page look-ups behind the wait for the kernel before).
+// plan and the first page look-ups behind the wait for the kernel before).  Both are the device's share: twenty calls in a CUDA graph, inputs as the call
+// before left them in L2; calls one by one, with other work's data in L2, 65 and 209.
 //
 //   work       The units (sequence, key/value head, row block, key tile) of the batch are one list that blocks, one a multiprocessor, cut into runs
 //              of equal weight (PLAIN_WEIGHT, SPLIT_WEIGHT a tile, SEGMENT_WEIGHT a row block); keys, values and queries of a run's next segment are
 //              copied while the last one ends.
 //   softmax    As in attention_tc.cu: weights 2^(x - M) with a whole number M that is raised only when a tile's weights add up to more than
-//              2^14, float32 sums, weights rounded to bfloat16 once.
+//              2^14, float32 sums, weights rounded to bfloat16 once, because the second product's operands are: half a step each, which makes results
+//              1.4 to 1.5 times as far from 64 bits as weights of 32 bits would (0.0025 of the largest and 0.0017).
 //   masks      A tile that holds nodes, the tree's end or the window's edge gives every row a 64-bit word of what it sees.  In such a tile a value
 //              that is not finite must not meet a weight of zero: the group looks its values over, and where it finds one adds the tile's products
 //              up itself, in tensor memory, leaving out what a row does not see; the issuing lane then leaves that tile out.
@@ -33,7 +35,7 @@ LLG_API const char* llg_last_error() { return g_llg_error; }
 namespace {
 
 constexpr int BQ = 128;                       // rows of a block: lanes of tensor memory
-// what a run's parts take, measured: 2,800 cycles a PLAIN tile, 1,660 a SPLIT tile
+// what a run's parts take, measured: 2,700 to 2,800 cycles a PLAIN tile, 1,660 a SPLIT tile
 constexpr int PLAIN_WEIGHT = 5, SPLIT_WEIGHT = 3, SEGMENT_WEIGHT = 8;
 constexpr int GROUPS = 2, WORKERS = GROUPS * BQ;
 constexpr int ISSUE_WARP = WORKERS / 32, K_LOAD_WARP = ISSUE_WARP + 1, V_LOAD_WARP = ISSUE_WARP + 2, ISSUE_WARP_2 = ISSUE_WARP + 3;

@@ -176,6 +176,8 @@ int run(const KeyWeightArgs& a, cudaStream_t stream) {
   return a.scores ? add_stored(a, stream) : go(key_weights_kernel<T, RY, true, STAGES>, 1);      // (a key's shares are added up by one block)
 }
 
+// Blocks of 8 rows, or of 32 from 9 rows on.  float32, us with 8 / 32 rows a block, heads of 64: 8 rows of 8 x 4,000 keys 32 / 55, 4 x 2,199..6,454 28 / 33; 12
+// rows 55 / 59, 42 / 36; heads of 128: 8 rows 63 / 99, 50 / 59; 12 rows 114 / 103, 72 / 62.
 template <typename T>
 int dispatch(const KeyWeightArgs& a, cudaStream_t stream) {
   const bool few = a.nh / a.nkv * a.last <= 8;

@@ -7,7 +7,13 @@
 namespace {
 
 constexpr int WEIGHT_TILE = 64;     // keys of a tile (a page); a split is a whole number of them
-constexpr int STORE_ROWS = 32;      // most rows of a (sequence, head) whose scores the matrix instructions' kernels keep between the passes
+// Most rows of a (sequence, head) whose scores the matrix instructions' kernels keep between the passes; more go to tcgen05 where it takes the head size.
+// us kept / worked out twice on mma.sync / tcgen05, 32 heads in groups of four, 8 x 8,190 keys, 8 x 500..8,190, 4 x 2,199..6,454: heads of 64, 16 rows
+// 37 / 47 / 61, 20 / 27 / 38, 16 / 17 / 20; 24 rows 48 / 48 / 61, 25 / 28 / 38, 19 / 17 / 20; 32 rows 57 / 49 / 53, 29 / 28 / 33, 22 / 18 / 18; 40 rows
+// - / 85 / 69, - / - / 43, - / 37 / 22.  Heads of 128, 16 rows 48 / 68 / 72, 24 / 35 / 41, 19 / 20 / 21; 24 rows 58 / 70 / 72, 30 / 36 / 42, 22 / 22 / 22;
+// 32 rows 67 / 72 / 64, 35 / 37 / 36, 25 / 23 / 20; 40 rows - / 127 / 78, - / - / 45, - / 51 / 23.  (32 rows of heads of 64 would be a fifth faster
+// worked out twice: their scores are as many bytes as the keys.)
+constexpr int STORE_ROWS = 32;
 
 // The rows of sequence b: its last queries' heads of one group.
 struct Rows {

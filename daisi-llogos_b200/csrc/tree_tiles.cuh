@@ -67,7 +67,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-// 2^x by the special-function unit alone; arguments are <= 0 or -inf, or bounded by the caller
+// 2^x by the special-function unit alone; arguments are <= 0 or -inf, or bounded by the caller.  (Somewhat less exact than
+// exp2f: key weights of a decode step are off by 4.5e-7 of the largest, a plain form in 32 bits by 3.1e-7.)
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -2497,7 +2497,8 @@ def attn_tree(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pag
     ``[N]``): bit j of a node's word says that it sees node j of its tree (its own bit included; bits behind the tree's nodes show nothing, and
     count for its depth); a node sees every cached key besides.  ``window`` W > 0: a node stands ``depth`` = (its bits) - 1 positions behind the cached keys and sees what stands less than W before
     it.  ``q`` is ``[N, nh, hd]``, ``out`` ``[N, nh * vd]``; a node that sees nothing gets zeros, rows behind the last sequence are left as they
-    were.  What a node does not see has no part in its result, whatever is stored there.
+    were.  What a node does not see has no part in its result, whatever is stored there.  Sums and softmax statistics are float32; with bfloat16
+    on the matrix instructions each softmax weight is rounded to bfloat16 once, for the product with the values, and the result once more.
 
     ``plan`` (``attn_tree_plan`` for this batch shape) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left
     zero) must hold; calls that may run at the same time need their own.  Like decode attention it reads sizes, slots and the page table while
@@ -2662,8 +2663,10 @@ def key_weights(q: torch.Tensor, k_pages: torch.Tensor, page_table: torch.Tensor
     len_before ? the entry : 0) + the sum`` for all its keys, the step's included; entries behind them and other slots' rows are left as
     they were.  The keys lie in the pages already (a cache that keeps every key).
 
-    ``plan`` (``key_weights_plan``) says what ``scratch`` (float32) and ``counters`` (int32, zero when first used, left zero) must hold; calls
-    that may run at the same time need their own.  A slot may be in a step once."""
+    ``plan`` (``key_weights_plan``) says what ``scratch`` (float32) must hold; calls that may run at the same time need their own.  ``counters``
+    (int32, ``plan.n_counters``: 0 for all kernels so far, none of which reads them) is there as the other attention operators have it.  Scores kept on
+    the way are at most ``KEY_SCORE_FLOATS``: a batch with more is taken a few sequences at a time, or its scores are worked out twice.  A slot may be
+    in a step once."""
     what, dt, i32 = "key_weights", q.dtype, torch.int32
     n, nh, hd = q.shape
     n_pages, nkv = k_pages.size(0), k_pages.size(1)
