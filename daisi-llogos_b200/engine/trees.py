@@ -281,8 +281,8 @@ class TreeSteps:
             e.ops.tree_accept(m["tokens"], m["parents"], m["cu"], path, count, nxt, logits=p.logits, scratch=scratch)
         else:
             e.ops.tree_accept(m["tokens"], m["parents"], m["cu"], path, count, nxt, picked=picked.contiguous())
-        for g in e.cache.kv_groups:
-            g.rows(e.ops).move(g.page_table, g.ring_pages, m["slots"], m["len_before"], path.view(1, b, 1, 64), count)
+        for g, rows in [(g, g.rows(e.ops)) for g in e.cache.kv_groups]:      # (made before the first row moves)
+            rows.move(g.page_table, g.ring_pages, m["slots"], m["len_before"], path.view(1, b, 1, 64), count)
         got = whole.cpu().numpy()
         self.pending = None
         out = []
@@ -319,10 +319,13 @@ class TreeSteps:
         meta = e._ensure_meta(block.size)
         e._staging.upload(block, meta)
         slots, keep, lengths, base = (meta[i * b:(i + 1) * b] for i in range(4))
-        for g in e.cache.kv_groups:
+        moves = []
+        for g in e.cache.kv_groups:                       # (all that can fail for want of memory is done before the first row moves)
             chosen = torch.empty((len(g.units), b, g.need.num_kv_heads, most), dtype=torch.int32, device=e.device)
             e.ops.keep_keys(g.weights, slots, lengths, keep, chosen, first=first, recent=recent, max_len=longest)
-            g.rows(e.ops).move(g.page_table, g.ring_pages, slots, base, chosen, keep)
+            moves.append((g, g.rows(e.ops), chosen))
+        for g, rows, chosen in moves:
+            rows.move(g.page_table, g.ring_pages, slots, base, chosen, keep)
         for slot, k, n in work:
             e.cache.shorten(slot, k)
             e._taken[slot] = e._taken.get(slot, 0) + n - k

@@ -210,3 +210,59 @@ def test_a_view_of_keys_is_made_with_the_arguments_it_had(llogos):
     shared = {}
     view = llogos.cache.store.KvView(None, None, None, 1, 0, 3, True, False, shared)
     assert view.shared is shared and view.weights is None
+
+
+def two_groups(llogos, **kw):
+    """An engine whose layers keep their keys in two groups (values of two sizes)."""
+    model = M.with_mixers(M.CFG, [dict(value_dim=32), dict(value_dim=24)], dtype=torch.float32, device="cpu", ops=tree_ops)
+    eng = engine_for(llogos, model, **kw)
+    assert len(eng.cache.kv_groups) == 2
+    return eng
+
+
+def fails_second(monkeypatch, target, name):
+    """The second call of ``target.name`` fails, once."""
+    real, calls = getattr(target, name), []
+
+    def act(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise Failure
+        return real(*args, **kw)
+    monkeypatch.setattr(target, name, act)
+
+
+@pytest.mark.parametrize("where", ["keep_keys", "CacheRows"])
+def test_an_eviction_that_fails_has_moved_nothing(llogos, monkeypatch, where):
+    """One group's keys at their new places and another's not would be an answer from keys that are not the tokens'."""
+    eng = two_groups(llogos, weigh_keys=2)
+    slot = eng.open()
+    eng.step([(slot, [(5 * i) % 256 for i in range(90)])], [[]])
+    before = [[t.clone() for t in (*g.k.values(), *g.v.values(), g.weights)] for g in eng.cache.kv_groups]
+    with monkeypatch.context() as m:
+        fails_second(m, tree_ops, where)
+        with pytest.raises(Failure):
+            eng.evict([(slot, 40)], first=2, recent=8)
+    for g, old in zip(eng.cache.kv_groups, before):
+        assert all(torch.equal(a, b) for a, b in zip((*g.k.values(), *g.v.values(), g.weights), old))
+    assert eng.length(slot) == eng.position(slot) == 90
+    eng.evict([(slot, 40)], first=2, recent=8)
+    assert (eng.length(slot), eng.position(slot)) == (40, 90)
+
+
+def test_an_acceptance_that_fails_can_be_made_again(llogos, monkeypatch):
+    eng, other = two_groups(llogos), two_groups(llogos)
+    parts = [3] * 70, ([1, 2, 3, 4], [-1, 0, 0, 2]), torch.tensor([3, 9, 4, 7], dtype=torch.int32)
+    logits = []
+    for e in (eng, other):
+        slot = e.open()
+        e.step([(slot, parts[0])], [[]])
+        e.step_tree([(slot, *parts[1])])
+        if e is eng:
+            with monkeypatch.context() as m:
+                fails_second(m, tree_ops, "CacheRows")
+                with pytest.raises(Failure):
+                    e.accept_tree(parts[2])
+        assert e.accept_tree(parts[2]) == [([0, 2, 3], 7)]
+        logits.append(e.step([(slot, [7])]).clone())
+    assert torch.equal(*logits)
