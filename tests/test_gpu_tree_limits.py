@@ -150,3 +150,42 @@ def test_a_window_ends_between_a_node_and_one_without_bits(ops, dtype, nh, hd):
     for window in (1, 2, 3, 5, 8):
         bits = [[0, 0b10, 0b11, 0b111, 0b1111, 0b11111, 0b111111, 0b1111111, 0b11111111, 0b1], [1, 0, 0b111, 0b1111, 2]]
         G.Case(dtype, nh, 2, hd, [200, 0], [10, 5], bits=bits, window=window, seed=window).check(ops)
+
+
+def test_calls_on_two_streams_at_once_give_what_they_give_alone(ops):
+    """Every kernel beside every other, each with a scratch of its own; no block of one waits for another's."""
+    import test_gpu_trees as G
+
+    def ints(x):
+        return torch.tensor(x, dtype=torch.int32, device="cuda:0")
+    jobs = []
+    for dtype, nh, hd, nodes in ((BF16, 16, 128, 64), (BF16, 8, 64, 4), (F32, 8, 64, 9), (BF16, 8, 64, 40)):
+        c = G.Case(dtype, nh, 2, hd, [900, 33, 257], [nodes, 1, nodes // 2], seed=nodes)
+        out, go = c.call(ops)
+        jobs.append((go, out, out.clone()))
+    for dtype, hd, last in ((BF16, 128, 40), (BF16, 64, 4), (F32, 64, 3)):
+        nh, nkv, before, brings = 8, 2, [900, 60], [50, 45]
+        kp = torch.randn(32, nkv, 64, hd, device="cuda:0", generator=torch.Generator("cuda:0").manual_seed(last)).to(dtype)
+        q = torch.randn(95, nh, hd, device="cuda:0", generator=torch.Generator("cuda:0").manual_seed(hd)).to(dtype)
+        plan = ops.key_weights_plan(dtype, 2, last, nh, nkv, hd, 1000)
+        scratch, counters, weights = torch.empty(plan.scratch_floats, device="cuda:0"), ints([0]), torch.zeros(2, nkv, 1000, device="cuda:0")
+        args = (q, kp, torch.arange(32, dtype=torch.int32, device="cuda:0").view(2, 16), ints([1, 0]), ints([0, 50, 95]), ints(before), weights, scratch)
+
+        def go(args=args, hd=hd, last=last, plan=plan, counters=counters, weights=weights):
+            weights.zero_()
+            ops.key_weights(*args, scale=hd ** -0.5, last=last, plan=plan, counters=counters)
+        go()
+        jobs.append((go, weights, weights.clone()))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(len(jobs)):
+        for j in range(len(jobs)):
+            if i == j:
+                continue
+            for _ in range(3):
+                for stream, (go, _, _) in zip(streams, (jobs[i], jobs[j])):
+                    with torch.cuda.stream(stream):
+                        go()
+            torch.cuda.synchronize()
+            assert torch.equal(jobs[i][1], jobs[i][2]) and torch.equal(jobs[j][1], jobs[j][2]), (i, j)
+    assert ops.attn_tree_status() == 0 and ops.key_weights_status() == 0
